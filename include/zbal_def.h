@@ -182,6 +182,33 @@ typedef struct {
  */
 #define ZBAL_WEIGHT_FORMAT_ND      0 /* logical [E, K, N], N contiguous */
 #define ZBAL_WEIGHT_FORMAT_PREPACKED 1 /* made by zbal_moe_weight_prepack */
+#define ZBAL_WEIGHT_FORMAT_NK      2 /* [E, N, K], K contiguous (zbal_moe_expert_linear) */
+
+/* zbal_moe_expert_linear (extension). SWIGLU: silu of the first half of the columns times the second half */
+typedef enum {
+    ZBAL_ACTIVATION_NONE = 0,
+    ZBAL_ACTIVATION_RELU = 1,
+    ZBAL_ACTIVATION_SILU = 2,
+    ZBAL_ACTIVATION_GELU = 3,      /* with the error function */
+    ZBAL_ACTIVATION_GELU_TANH = 4,
+    ZBAL_ACTIVATION_SWIGLU = 5,
+
+    ZBAL_ACTIVATION_BUTT
+} zbal_activation_t;
+
+/* zbal_moe_group_route (extension) */
+typedef enum {
+    ZBAL_SCORE_SIGMOID = 0,
+    ZBAL_SCORE_SOFTMAX = 1,
+
+    ZBAL_SCORE_BUTT
+} zbal_score_t;
+typedef enum {
+    ZBAL_GROUP_SCORE_TOP2 = 0,     /* the sum of a group's two largest choices */
+    ZBAL_GROUP_SCORE_MAX = 1,      /* its largest */
+
+    ZBAL_GROUP_SCORE_BUTT
+} zbal_group_score_t;
 
 /*
  * Activation quantisation modes, reference zbal_def.h:149-155 (0 and 1

@@ -400,6 +400,68 @@ ZBALHIP_API int32_t zbalhip_gmm2_dequant_shared(const void *a, const float *a_sc
  */
 ZBALHIP_API int32_t zbalhip_gemm_prepare(void);
 
+/*
+ * Routing by groups of experts (no reference counterpart). s = sigmoid (score 0) or softmax (1) of the logits [T,E] (dtype fp32, bf16 or
+ * fp16), c = s + bias [E] fp32 (may be null). The experts form `groups` groups of consecutive ones; the kept_groups groups of the
+ * largest sum of two c (group_score 0) or largest c (1) are kept, and the topk experts of the largest c in those are the
+ * picks, in falling order, ties to the lower index. An expert whose logit is minus infinity, or whose c is that or no number, is none:
+ * slots without a pick get the id -1 and the weight 0. weight = scale * s, over the sum of the picks' s if renormalize (0 where that sum is
+ * 0). topk_idx [T,K] as in zbalhip_topk_route, topk_w [T,K] fp32. E <= 1024, K <= 32, groups <= 64, K <= experts of the kept groups.
+ * The gradient takes logits, score, renormalize, scale and the picks (ids outside [0,E) are none; equal ones add up): grad_w [T,K] fp32 ->
+ * grad_logits [T,E] of the logits' type. The bias has none.
+ */
+typedef struct {
+    const void *logits;
+    int32_t dtype, score, group_score, renormalize;
+    double scale;
+    const float *bias;
+    int64_t tokens, experts, topk, groups, kept_groups;
+} zbalhip_group_route_t;
+ZBALHIP_API int32_t zbalhip_group_route(const zbalhip_group_route_t *route, void *topk_idx, int32_t idx_is_i64, float *topk_w, void *stream);
+ZBALHIP_API int32_t zbalhip_group_route_backward(const zbalhip_group_route_t *route, const float *grad_w, const void *topk_idx,
+                                     int32_t idx_is_i64, void *grad_logits, void *stream);
+
+/*
+ * The experts' products in half precision (no reference counterpart). x [rows, K] (dtype bf16 or fp16), sorted by expert: the first
+ * counts[0] rows are expert 0's and so on (device memory, int32 or int64; null with one expert: all rows). Counts below 0 are none, and rows
+ * past `rows` are nobody's; rows past the last expert's are neither read nor written. weight [E, K, N], or [E, N, K] with weight_is_nk, of x's type.
+ *   z = x W + bias, y = act(z) + residual, each output rounded once from 32 bits.
+ * activation: 0 none, 1 relu, 2 silu, 3 gelu, 4 gelu with tanh, 5 swiglu (silu of z's first N / 2 columns times the others; y is [rows, N / 2]).
+ * bias [E, N] of x's type or fp32, residual of y's shape and type, preact [rows, N] of x's type = z: each may be null. y: x's type or fp32.
+ * Backward: grad of y's shape, x's type or fp32. grad_preact = grad act'(preact), rounded to x's type (needed where there is an activation or
+ * grad is fp32; else dz is grad itself), grad_x = dz W^T of x's type, grad_weight [E, K, N] (or [E, N, K]) = x^T dz and grad_bias [E, N] = sum of
+ * dz, both of x's type or both fp32; zeros for experts without rows. grad_x, grad_weight and grad_bias may be null (grad_bias comes with
+ * grad_weight only). The sums are in 32 bits, always in the same order.
+ * workspace: zbalhip_expert_linear_workspace bytes at least (-1: the sizes are not allowed), 16-byte aligned, undefined before and after; the call's own
+ * until it has run. Less, or none, changes how a product is split, not what it is. K, N <= ZBALHIP_EXPERT_MAX_WIDTH, rows <= ZBALHIP_EXPERT_MAX_ROWS, E <= 1024.
+ */
+#define ZBALHIP_EXPERT_MAX_WIDTH 65536
+#define ZBALHIP_EXPERT_MAX_ROWS (1 << 24)
+typedef struct {
+    const void *weight;
+    int32_t weight_is_nk, dtype;
+    const void *counts;
+    int32_t counts_are_i64, activation;
+    int64_t rows, k, n, experts;
+} zbalhip_expert_linear_t;
+ZBALHIP_API int64_t zbalhip_expert_linear_workspace(const zbalhip_expert_linear_t *linear, int32_t backward);
+ZBALHIP_API int32_t zbalhip_expert_linear(const zbalhip_expert_linear_t *linear, const void *x, const void *bias, int32_t bias_is_f32,
+                              const void *residual, void *y, int32_t y_is_f32, void *preact, void *workspace,
+                              int64_t workspace_bytes, void *stream);
+ZBALHIP_API int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t *linear, const void *grad, int32_t grad_is_f32, const void *x,
+                                       const void *preact, void *grad_x, void *grad_weight, void *grad_bias,
+                                       int32_t weight_grad_is_f32, void *grad_preact, void *workspace, int64_t workspace_bytes,
+                                       void *stream);
+
+/*
+ * Gradient of zbalhip_combine on one rank (exclusive offsets): grad [T,H] (bf16 or fp16) -> grad_y [y_rows,H] of its type, the row of pick (t,k) =
+ * w[t,k] grad[t], and grad_w [T,K] fp32 = <grad[t], y[row]>, 0 for a pick that went nowhere. Rows that no pick went to are left as they are.
+ */
+ZBALHIP_API int32_t zbalhip_combine_backward(const void *grad, const void *y, int64_t y_rows, int32_t dtype, const int32_t *base,
+                                 const float *w, const void *topk_idx, int32_t idx_is_i64, const int32_t *send_token_idx,
+                                 int64_t tokens, int64_t hidden, int64_t topk, int64_t experts, void *grad_y, float *grad_w,
+                                 void *stream);
+
 #ifdef __cplusplus
 }
 #endif

@@ -241,6 +241,74 @@ int32_t zbal_moe_topk_route(const zbal_tensor_info_t *logits, int64_t topkNum, c
 int32_t zbal_moe_weight_prepack(const zbal_tensor_info_t *src, const zbal_tensor_info_t *dst, zbal_comm_t comm,
                                 aclrtStream stream, int64_t flags);
 
+/*
+ * extension: routing by groups of experts. score s = sigmoid or softmax of the logits [T, E] (fp32, bf16 or fp16), choice c = s + bias
+ * ([E] fp32, may be null). Of groupNum groups of consecutive experts the topkGroupNum best are kept, and the topkNum largest
+ * choices in those are the picks, in falling order, ties to the lower index. weight = scale * s, over the sum of the picks' s if
+ * renormalize (0 where that is 0). An expert is no pick if its logit is minus infinity or its choice is that or no number; slots that are left
+ * get the id -1 and the weight 0. topkIndex, topkWeight: as in zbal_moe_topk_route. Up to 1024 experts, 64 groups, 32 picks.
+ */
+int32_t zbal_moe_group_route(const zbal_tensor_info_t *logits, const zbal_tensor_info_t *bias, int64_t topkNum,
+                             int64_t groupNum, int64_t topkGroupNum, zbal_score_t score, zbal_group_score_t groupScore,
+                             int64_t renormalize, double scale, const zbal_tensor_info_t *topkIndex,
+                             const zbal_tensor_info_t *topkWeight, zbal_comm_t comm, aclrtStream stream, int64_t flags);
+
+/*
+ * extension: its gradient. gradWeight [T, K] fp32, topkIndex as the router left it -> gradLogits [T, E] of the logits' type. Ids outside
+ * [0, E) are no picks. The bias, which only decides, has no gradient.
+ */
+int32_t zbal_moe_group_route_backward(const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *logits,
+                                      const zbal_tensor_info_t *topkIndex, zbal_score_t score, int64_t renormalize,
+                                      double scale, const zbal_tensor_info_t *gradLogits, zbal_comm_t comm,
+                                      aclrtStream stream, int64_t flags);
+
+/*
+ * extension: the experts' products on rows as zbal_dispatch_normal leaves them without quantisation. z = x W + bias, y = act(z) + residual.
+ * x [rows, K] bf16 or fp16, sorted by expert; weight [E, K, N] (ZBAL_WEIGHT_FORMAT_ND) or [E, N, K] (ZBAL_WEIGHT_FORMAT_NK in
+ * reserved[0]) of x's type; with one expert the leading dimension may be left out. tokensPerExpert [E] int32 or int64; with one expert it may be null: all
+ * rows. Rows past their sum are neither read nor written. bias [E, N] of x's type or fp32, residual of y's shape and type, preact
+ * [rows, N] of x's type (receives z): each may be null. y [rows, N] (swiglu: [rows, N / 2]) of x's type or fp32. Sums are held in 32
+ * bits, every output is rounded once. workspace: zbal_moe_expert_linear_workspace_size bytes (null where that is 0); it may not be
+ * shared with a call that can run at the same time.
+ */
+int32_t zbal_moe_expert_linear(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                               const zbal_tensor_info_t *tokensPerExpert, const zbal_tensor_info_t *bias,
+                               zbal_activation_t activation, const zbal_tensor_info_t *residual, const zbal_tensor_info_t *y,
+                               const zbal_tensor_info_t *preact, const zbal_tensor_info_t *workspace, zbal_comm_t comm,
+                               aclrtStream stream, int64_t flags);
+
+/*
+ * extension: its gradients. grad of y's shape, of x's type or fp32; preact: what the forward call left (null without an activation).
+ * gradPreact [rows, N] of x's type = grad act'(preact), rounded once; the other gradients are of that tensor (without an activation, and with
+ * grad of x's type, it is grad itself, and gradPreact may be null). gradX [rows, K] of x's type, gradWeight of weight's shape, gradBias
+ * [E, N], both of x's type or both fp32; experts without rows get zeros. gradX, gradWeight and gradBias may be null; gradBias comes
+ * with gradWeight. The residual's gradient is grad.
+ */
+int32_t zbal_moe_expert_linear_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x,
+                                        const zbal_tensor_info_t *weight, const zbal_tensor_info_t *tokensPerExpert,
+                                        zbal_activation_t activation, const zbal_tensor_info_t *preact,
+                                        const zbal_tensor_info_t *gradX, const zbal_tensor_info_t *gradWeight,
+                                        const zbal_tensor_info_t *gradBias, const zbal_tensor_info_t *gradPreact,
+                                        const zbal_tensor_info_t *workspace, zbal_comm_t comm, aclrtStream stream,
+                                        int64_t flags);
+
+/* extension: bytes of workspace for either call (backward != 0: the second), often 0. -1 on sizes that are not allowed. */
+int64_t zbal_moe_expert_linear_workspace_size(int64_t rows, int64_t k, int64_t n, int64_t expertNum,
+                                              zbal_activation_t activation, zbal_datatype_t dataType, int64_t weightFormat,
+                                              int64_t backward);
+
+/*
+ * extension: the gradient of zbal_combine_normal on a group of one rank. grad [T, H], srcTokens [rows, H] and the others as the combine took
+ * them -> gradTokens [rows, H]: the row of a pick gets its weight times its token's gradient (rows of no pick are left as they are),
+ * gradWeight [T, K] fp32: the product of the two rows, 0 for a pick that went nowhere.
+ */
+int32_t zbal_combine_normal_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *srcTokens,
+                                     const zbal_tensor_info_t *srcTokensPerEp, const zbal_tensor_info_t *topKWeight,
+                                     const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *sendTokensIndex,
+                                     int64_t expertNum, const zbal_tensor_info_t *gradTokens,
+                                     const zbal_tensor_info_t *gradWeight, zbal_comm_t comm, aclrtStream stream,
+                                     int64_t flags);
+
 #ifdef __cplusplus
 }
 #endif

@@ -80,6 +80,12 @@ def _no_hook() -> None:
     """The receive hook of the low-latency calls: there is nothing to wait for."""
 
 
+class DispatchHandle(tuple):
+    """What dispatch returns for combine: the reference's five entries (zbal_deepep.cpp:388), and where each pick's row lies
+    within its expert's (`send_token_idx`), so that a handle stays good when other layers have dispatched since."""
+    send_token_idx: Optional[torch.Tensor] = None
+
+
 PADDING_SIZE = 1      # an empty batch is padded to this many tokens (zbal_deepep.cpp:85, 470-490)
 
 
@@ -208,7 +214,8 @@ class Buffer:
         recv_x, recv_x_scales, num_recv_tokens_per_expert_list, put_offset, balance_matrix = self.runtime.dispatch_counts(
             x, topk_idx, num_tokens_per_expert, capi.QUANT_INT8 if use_quant else capi.NO_QUANT, num_worst_tokens,
             token_nums_type == 0)
-        handle = (is_token_in_rank, topk_idx, topk_weights, put_offset, balance_matrix)
+        handle = DispatchHandle((is_token_in_rank, topk_idx, topk_weights, put_offset, balance_matrix))
+        handle.send_token_idx = self.runtime.send_token_idx
         return ((recv_x, recv_x_scales) if use_quant else recv_x, None, None, num_recv_tokens_per_expert_list, handle,
                 self._event(async_finish))
 
@@ -219,6 +226,12 @@ class Buffer:
                 ) -> Tuple[torch.Tensor, Optional[torch.Tensor], EventOverlap]:
         """zbal_buffer.py:350-411, zbal_deepep.cpp:395-452: out[t] = sum_k w[t, k] * x[row(t, k)] with the weights the
         handle carries (those given to dispatch), as the reference. Returns (combined_x, None, event)."""
+        h, topk_weights_ori = self._combine_operands(x, handle)
+        self._wait(previous_event)
+        out = self.runtime.combine(x, h, topk_weights_ori)
+        return out, None, self._event(async_finish)
+
+    def _combine_operands(self, x, handle):
         is_token_in_rank, topk_idx, topk_weights_ori, put_offset, balance_matrix = handle
         if x.dim() != 2 or not x.is_contiguous():
             raise ValueError("x dim not 2 or not contiguous")
@@ -227,11 +240,29 @@ class Buffer:
         if topk_weights_ori.dim() != 2 or topk_weights_ori.size(1) != topk_idx.size(1) or \
                 topk_weights_ori.dtype != torch.float32:
             raise ValueError("topk_weights check failed")
-        self._wait(previous_event)
-        h = dict(put_offset=put_offset, balance_matrix=balance_matrix, expert_ids=topk_idx,
-                 send_token_idx=self.runtime.send_token_idx, num_experts=put_offset.size(1))
-        out = self.runtime.combine(x, h, topk_weights_ori)
-        return out, None, self._event(async_finish)
+        # a handle without its own positions (one that a caller has put together) means the last layout's, as in the reference
+        send_token_idx = getattr(handle, "send_token_idx", None)
+        return dict(put_offset=put_offset, balance_matrix=balance_matrix, expert_ids=topk_idx,
+                    send_token_idx=self.runtime.send_token_idx if send_token_idx is None else send_token_idx,
+                    num_experts=put_offset.size(1)), topk_weights_ori
+
+    def combine_backward(self, grad: torch.Tensor, x: torch.Tensor, handle: Tuple
+                         ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Extension: the gradients of combine(x, handle) from that of its result, grad [tokens, hidden]: grad_x [rows, hidden] (a
+        pick's row: its weight times its token's gradient) and grad_topk_weights [tokens, topk] fp32 (the product of the two
+        rows; 0 for a pick that went nowhere). Rows that no pick went to, past the last expert's, are not written.
+        The dispatch's gradient is dispatch_backward."""
+        h, topk_weights_ori = self._combine_operands(x, handle)
+        return self.runtime.combine_backward(grad, x, h, topk_weights_ori)
+
+    def dispatch_backward(self, grad: torch.Tensor, handle: Tuple) -> torch.Tensor:
+        """Extension: the gradient of an unquantised dispatch's x [tokens, hidden] from that of the received rows, grad [rows,
+        hidden]: a token's is the sum of its picks' rows, the combine with weights of one."""
+        is_token_in_rank, topk_idx, _, put_offset, balance_matrix = handle
+        ones = DispatchHandle((is_token_in_rank, topk_idx, torch.ones(topk_idx.shape, dtype=torch.float32, device=grad.device),
+                               put_offset, balance_matrix))
+        ones.send_token_idx = getattr(handle, "send_token_idx", None)
+        return self.combine(grad, ones)[0]
 
     # ---- low-latency mode -----------------------------------------------------------------------------
     def clean_low_latency_buffer(self, num_max_dispatch_tokens_per_rank: int, hidden: int, num_experts: int) -> None:
@@ -356,6 +387,57 @@ class Buffer:
     def topk_route(self, logits: torch.Tensor, num_topk: int, idx_dtype=torch.int64):
         """Extension: softmax + top-k router; returns (topk_idx, topk_weights)."""
         return self.runtime.topk_route(logits, num_topk, idx_dtype)
+
+    def group_route(self, logits: torch.Tensor, num_topk: int, num_groups: int = 1, topk_groups: int = 1, score: str = "sigmoid",
+                    bias: Optional[torch.Tensor] = None, group_score: str = "top2", renormalize: bool = True, scale: float = 1.0,
+                    idx_dtype=torch.int64) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Extension: routing by groups of experts. logits [tokens, experts] fp32, bf16 or fp16. A score is the sigmoid of a logit
+        or the softmax of a row (`score`); the choice is the score plus bias [experts] fp32, which balances the experts' load. Of
+        num_groups groups of consecutive experts the topk_groups are kept whose two largest choices have the largest sum
+        (group_score "top2"; "max": whose largest choice is largest), and the num_topk experts of the largest choices in those
+        are the token's, in falling order; equal ones go to the lower index. The weights are the scores, over their sum if
+        renormalize, times scale. Logits of minus infinity, and choices that are no number, are no picks: slots left over get
+        the id -1 (no selection, to get_dispatch_layout) and the weight 0.
+        Returns (topk_idx [tokens, topk] of idx_dtype, topk_weights [tokens, topk] fp32)."""
+        return self.runtime.group_route(logits, num_topk, num_groups, topk_groups, score, bias, group_score, renormalize, scale,
+                                        idx_dtype)
+
+    def group_route_backward(self, grad_weights: torch.Tensor, logits: torch.Tensor, topk_idx: torch.Tensor,
+                             score: str = "sigmoid", renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
+        """Extension: the logits' gradient from that of group_route's weights, with the picks as they were made (the picking itself
+        and the bias have none). Ids outside [0, experts) are no picks."""
+        return self.runtime.group_route_backward(grad_weights, logits, topk_idx, score, renormalize, scale)
+
+    # ---- unquantised experts ----------------------------------------------------------------------------
+    def expert_linear(self, x: torch.Tensor, weight: torch.Tensor, tokens_per_expert: Optional[torch.Tensor] = None,
+                      bias: Optional[torch.Tensor] = None, activation: str = "none", residual: Optional[torch.Tensor] = None,
+                      out_dtype: Optional[torch.dtype] = None, transposed: bool = False, return_preact: bool = False,
+                      out: Optional[torch.Tensor] = None):
+        """Extension: the experts' product y = act(x W + bias) + residual on rows as an unquantised dispatch leaves them. x [rows, k]
+        bf16 or fp16, sorted by expert; weight [experts, k, n] of x's type ([experts, n, k] if transposed; one expert's may
+        leave out the first dimension); tokens_per_expert [experts] int32 or int64 on the device: what get_dispatch_layout and
+        low_latency_dispatch return (one expert: None means all rows). Rows past their sum are neither read nor written. bias
+        [experts, n] of x's type or fp32. activation: none, relu, silu, gelu, gelu_tanh or swiglu (silu of the first n / 2
+        columns times the others, y is [rows, n / 2]). residual of y's shape and type. y is of x's type or, with out_dtype,
+        torch.float32; out: a tensor to write it to. Sums are held in 32 bits, every output is rounded once.
+        Returns y, or (y, x W + bias of x's type) with return_preact."""
+        y, preact = self.runtime.expert_linear(x, weight, tokens_per_expert, bias, activation, residual, out_dtype, transposed,
+                                               return_preact, out)
+        return (y, preact) if return_preact else y
+
+    def expert_linear_backward(self, grad: torch.Tensor, x: torch.Tensor, weight: torch.Tensor,
+                               tokens_per_expert: Optional[torch.Tensor] = None, activation: str = "none",
+                               preact: Optional[torch.Tensor] = None, transposed: bool = False, bias: bool = False,
+                               weight_grad_dtype: Optional[torch.dtype] = None, need_x: bool = True, need_weight: bool = True
+                               ) -> Tuple[Optional[torch.Tensor], ...]:
+        """Extension: expert_linear's gradients. grad is that of y, of x's type or fp32; preact is what the forward call returned.
+        grad_preact = grad act'(preact), rounded to x's type, is a tensor of its own, and the other gradients are of it: grad_x
+        of x's type, grad_weight of weight's shape and (with bias) grad_bias [experts, n] of x's type or, with weight_grad_dtype,
+        torch.float32; zeros for experts without rows. The residual's gradient is grad.
+        Returns (grad_x, grad_weight, grad_bias, grad_preact): None for what was not asked for, and for grad_preact where it is
+        grad itself."""
+        return self.runtime.expert_linear_backward(grad, x, weight, tokens_per_expert, activation, preact, transposed, bias,
+                                                   weight_grad_dtype, need_x, need_weight)
 
     def fused_deep_moe(self, x: torch.Tensor, topk_idx: torch.Tensor, gmm1_permuted_weight: torch.Tensor,
                        gmm1_permuted_weight_scale: torch.Tensor, gmm2_weight: torch.Tensor,

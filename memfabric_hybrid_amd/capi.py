@@ -28,7 +28,11 @@ SWIGLU_VALUES = 0x800    # ZBALHIP_SWIGLU_VALUES: OR-ed into the mode of both GE
 ROWMAX_CLEARED = 0x200   # ZBALHIP_ROWMAX_CLEARED: OR-ed into the mode of zbalhip_gmm1_swiglu_quant
 # zbal_backend_t
 BACKEND_GPU, BACKEND_DUMMY = 0, 1
-WEIGHT_FORMAT_ND, WEIGHT_FORMAT_PREPACKED = 0, 1
+WEIGHT_FORMAT_ND, WEIGHT_FORMAT_PREPACKED, WEIGHT_FORMAT_NK = 0, 1, 2
+# zbal_activation_t, zbal_score_t, zbal_group_score_t
+ACTIVATIONS = {"none": 0, "relu": 1, "silu": 2, "gelu": 3, "gelu_tanh": 4, "swiglu": 5}
+SCORES = {"sigmoid": 0, "softmax": 1}
+GROUP_SCORES = {"top2": 0, "max": 1}
 
 Z_OK, Z_ERROR, Z_INVALID_PARAM = 0, -1, -2
 Z_NOT_BOOTSTRAPPED, Z_CREATE_COMM_FAILED = -15, -16
@@ -87,6 +91,20 @@ class CommGroupInfo(ctypes.Structure):
                 ("groupIndex", ctypes.c_uint16), ("dataOpType", ctypes.c_uint32)]
 
 
+class GroupRoute(ctypes.Structure):
+    """zbalhip_group_route_t"""
+    _fields_ = [("logits", ctypes.c_void_p), ("dtype", ctypes.c_int32), ("score", ctypes.c_int32), ("group_score", ctypes.c_int32),
+                ("renormalize", ctypes.c_int32), ("scale", ctypes.c_double), ("bias", ctypes.c_void_p), ("tokens", ctypes.c_int64),
+                ("experts", ctypes.c_int64), ("topk", ctypes.c_int64), ("groups", ctypes.c_int64), ("kept_groups", ctypes.c_int64)]
+
+
+class ExpertLinear(ctypes.Structure):
+    """zbalhip_expert_linear_t"""
+    _fields_ = [("weight", ctypes.c_void_p), ("weight_is_nk", ctypes.c_int32), ("dtype", ctypes.c_int32), ("counts", ctypes.c_void_p),
+                ("counts_are_i64", ctypes.c_int32), ("activation", ctypes.c_int32), ("rows", ctypes.c_int64), ("k", ctypes.c_int64),
+                ("n", ctypes.c_int64), ("experts", ctypes.c_int64)]
+
+
 _TI = ctypes.POINTER(TensorInfo)
 _i64, _i32, _vp, _u16, _u32, _u64 = (ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint16,
                                      ctypes.c_uint32, ctypes.c_uint64)
@@ -139,6 +157,12 @@ SIGNATURES = {
     "zbal_fused_deep_moe": (_i32, [_TI] * 18 + [_i64] * 6 + [_vp, _vp, _i64]),
     "zbal_fused_deep_moe_workspace_size": (_u64, [_i64] * 7),
     "zbal_moe_topk_route": (_i32, [_TI, _i64, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_group_route": (_i32, [_TI, _TI, _i64, _i64, _i64, _i32, _i32, _i64, ctypes.c_double, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_group_route_backward": (_i32, [_TI, _TI, _TI, _i32, _i64, ctypes.c_double, _TI, _vp, _vp, _i64]),
+    "zbal_moe_expert_linear": (_i32, [_TI, _TI, _TI, _TI, _i32, _TI, _TI, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_expert_linear_backward": (_i32, [_TI, _TI, _TI, _TI, _i32, _TI, _TI, _TI, _TI, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_expert_linear_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32, _i64, _i64]),
+    "zbal_combine_normal_backward": (_i32, [_TI, _TI, _TI, _TI, _TI, _TI, _i64, _TI, _TI, _vp, _vp, _i64]),
     "zbal_moe_weight_prepack": (_i32, [_TI, _TI, _vp, _vp, _i64]),
     # zbal_hip_kernels.h
     "zbalhip_topk_route": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp]),
@@ -175,6 +199,13 @@ SIGNATURES = {
     "zbalhip_gmm2_dequant": (_i32, [_vp, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _i32, _i32, _vp, _vp]),
     "zbalhip_gmm2_takes_values": (_i32, [_i64, _i64, _i64, _i32]),
     "zbalhip_gemm_prepare": (_i32, []),
+    "zbalhip_group_route": (_i32, [ctypes.POINTER(GroupRoute), _vp, _i32, _vp, _vp]),
+    "zbalhip_group_route_backward": (_i32, [ctypes.POINTER(GroupRoute), _vp, _vp, _i32, _vp, _vp]),
+    "zbalhip_expert_linear_workspace": (_i64, [ctypes.POINTER(ExpertLinear), _i32]),
+    "zbalhip_expert_linear": (_i32, [ctypes.POINTER(ExpertLinear), _vp, _vp, _i32, _vp, _vp, _i32, _vp, _vp, _i64, _vp]),
+    "zbalhip_expert_linear_backward": (_i32, [ctypes.POINTER(ExpertLinear), _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64,
+                                              _vp]),
+    "zbalhip_combine_backward": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
 }
 
 _lib = None

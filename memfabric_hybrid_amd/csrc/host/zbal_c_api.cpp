@@ -420,3 +420,81 @@ ZBAL_API int32_t zbal_moe_weight_prepack(const zbal_tensor_info_t *src, const zb
     if (!c) return Z_INVALID_PARAM;
     return c->WeightPrepack(src, dst, stream, flags);
 }
+
+ZBAL_API int32_t zbal_moe_group_route(const zbal_tensor_info_t *logits, const zbal_tensor_info_t *bias, int64_t topkNum,
+                                      int64_t groupNum, int64_t topkGroupNum, zbal_score_t score,
+                                      zbal_group_score_t groupScore, int64_t renormalize, double scale,
+                                      const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *topkWeight,
+                                      zbal_comm_t comm, aclrtStream stream, int64_t)
+{
+    if (!Present("GroupRoute", {{"logits", logits}, {"topkIndex", topkIndex}, {"topkWeight", topkWeight}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(topkNum > 0, "GroupRoute failed as topkNum " << topkNum << " is invalid", Z_INVALID_PARAM);
+    ZBAL_VALIDATE_RETURN(groupNum > 0, "GroupRoute failed as groupNum " << groupNum << " is invalid", Z_INVALID_PARAM);
+    ZBAL_VALIDATE_RETURN(topkGroupNum > 0 && topkGroupNum <= groupNum, "GroupRoute failed as topkGroupNum " << topkGroupNum << " is invalid", Z_INVALID_PARAM);
+    ZBAL_VALIDATE_RETURN(score >= 0 && score < ZBAL_SCORE_BUTT, "GroupRoute failed as score " << score << " is invalid", Z_INVALID_PARAM);
+    ZBAL_VALIDATE_RETURN(groupScore >= 0 && groupScore < ZBAL_GROUP_SCORE_BUTT, "GroupRoute failed as groupScore " << groupScore << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("GroupRoute", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->GroupRoute(logits, bias, topkNum, groupNum, topkGroupNum, score, groupScore, renormalize, scale, topkIndex, topkWeight, stream);
+}
+
+ZBAL_API int32_t zbal_moe_group_route_backward(const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *logits,
+                                               const zbal_tensor_info_t *topkIndex, zbal_score_t score, int64_t renormalize,
+                                               double scale, const zbal_tensor_info_t *gradLogits, zbal_comm_t comm,
+                                               aclrtStream stream, int64_t)
+{
+    if (!Present("GroupRouteBackward", {{"gradWeight", gradWeight}, {"logits", logits}, {"topkIndex", topkIndex}, {"gradLogits", gradLogits}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(score >= 0 && score < ZBAL_SCORE_BUTT, "GroupRouteBackward failed as score " << score << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("GroupRouteBackward", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->GroupRouteBackward(gradWeight, logits, topkIndex, score, renormalize, scale, gradLogits, stream);
+}
+
+ZBAL_API int32_t zbal_moe_expert_linear(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                        const zbal_tensor_info_t *tokensPerExpert, const zbal_tensor_info_t *bias,
+                                        zbal_activation_t activation, const zbal_tensor_info_t *residual,
+                                        const zbal_tensor_info_t *y, const zbal_tensor_info_t *preact,
+                                        const zbal_tensor_info_t *workspace, zbal_comm_t comm, aclrtStream stream, int64_t)
+{
+    if (!Present("ExpertLinear", {{"x", x}, {"weight", weight}, {"y", y}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(activation >= 0 && activation < ZBAL_ACTIVATION_BUTT, "ExpertLinear failed as activation " << activation << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("ExpertLinear", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->ExpertLinear(x, weight, tokensPerExpert, bias, activation, residual, y, preact, workspace, stream);
+}
+
+ZBAL_API int32_t zbal_moe_expert_linear_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x,
+                                                 const zbal_tensor_info_t *weight, const zbal_tensor_info_t *tokensPerExpert,
+                                                 zbal_activation_t activation, const zbal_tensor_info_t *preact,
+                                                 const zbal_tensor_info_t *gradX, const zbal_tensor_info_t *gradWeight,
+                                                 const zbal_tensor_info_t *gradBias, const zbal_tensor_info_t *gradPreact,
+                                                 const zbal_tensor_info_t *workspace, zbal_comm_t comm, aclrtStream stream,
+                                                 int64_t)
+{
+    if (!Present("ExpertLinearBackward", {{"grad", grad}, {"x", x}, {"weight", weight}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(activation >= 0 && activation < ZBAL_ACTIVATION_BUTT, "ExpertLinearBackward failed as activation " << activation << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("ExpertLinearBackward", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->ExpertLinearBackward(grad, x, weight, tokensPerExpert, activation, preact, gradX, gradWeight, gradBias, gradPreact, workspace, stream);
+}
+
+ZBAL_API int64_t zbal_moe_expert_linear_workspace_size(int64_t rows, int64_t k, int64_t n, int64_t expertNum,
+                                                       zbal_activation_t activation, zbal_datatype_t dataType,
+                                                       int64_t weightFormat, int64_t backward)
+{
+    return ExpertLinearWorkspaceBytes(rows, k, n, expertNum, activation, dataType, weightFormat, backward != 0);
+}
+
+ZBAL_API int32_t zbal_combine_normal_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *srcTokens,
+                                              const zbal_tensor_info_t *srcTokensPerEp, const zbal_tensor_info_t *topKWeight,
+                                              const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *sendTokensIndex,
+                                              int64_t expertNum, const zbal_tensor_info_t *gradTokens,
+                                              const zbal_tensor_info_t *gradWeight, zbal_comm_t comm, aclrtStream stream,
+                                              int64_t)
+{
+    if (!Present("CombineNormalBackward", {{"grad", grad}, {"srcTokens", srcTokens}, {"srcTokensPerEp", srcTokensPerEp}, {"topKWeight", topKWeight}, {"topkIndex", topkIndex}, {"sendTokensIndex", sendTokensIndex}, {"gradTokens", gradTokens}, {"gradWeight", gradWeight}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(expertNum > 0 && expertNum <= 1024, "CombineNormalBackward failed as expertNum " << expertNum << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("CombineNormalBackward", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->CombineNormalBackward(grad, srcTokens, srcTokensPerEp, topKWeight, topkIndex, sendTokensIndex, expertNum, gradTokens, gradWeight, stream);
+}

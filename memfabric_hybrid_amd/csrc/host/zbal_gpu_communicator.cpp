@@ -68,6 +68,13 @@ bool CheckTensor(const char *op, const char *name, const zbal_tensor_info_t *t, 
     return true;
 }
 
+/* the router's logits, of three types */
+bool CheckRouteLogits(const char *op, const char *name, const zbal_tensor_info_t *t, int64_t min_elems)
+{
+    const int other = t->dataType == ZBAL_DATA_TYPE_FP16 ? ZBAL_DATA_TYPE_FP16 : ZBAL_DATA_TYPE_BFP16;
+    return CheckTensor(op, name, t, ZBAL_DATA_TYPE_FP32, other, min_elems);
+}
+
 #define ZB_CHECK(...)                           \
     do {                                        \
         if (!CheckTensor(__VA_ARGS__)) return Z_INVALID_PARAM; \
@@ -902,6 +909,209 @@ public:
                                                stream));
     }
 
+    int32_t GroupRoute(const zbal_tensor_info_t *logits, const zbal_tensor_info_t *bias, int64_t topkNum, int64_t groupNum,
+                       int64_t topkGroupNum, zbal_score_t score, zbal_group_score_t groupScore, int64_t renormalize, double scale,
+                       const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *topkWeight, aclrtStream stream) override
+    {
+        const char *op = "GroupRoute";
+        ZBAL_VALIDATE_RETURN(logits->dim == 2, op << " failed as logits must be [tokens, experts]", Z_INVALID_PARAM);
+        const int64_t T = logits->shape[0], E = logits->shape[1];
+        ZBAL_VALIDATE_RETURN(E > 0 && E <= 1024 && groupNum <= 64 && E % groupNum == 0,
+                             op << " failed as " << E << " experts do not make " << groupNum << " groups (up to 1024, up to 64)", Z_INVALID_PARAM);
+        ZBAL_VALIDATE_RETURN(topkNum <= 32 && topkNum <= topkGroupNum * (E / groupNum),
+                             op << " failed as topk " << topkNum << " exceeds 32 or the experts of " << topkGroupNum << " groups", Z_INVALID_PARAM);
+        if (T == 0) return Z_OK;
+        if (!CheckRouteLogits(op, "logits", logits, T * E)) return Z_INVALID_PARAM;
+        const bool biased = bias != nullptr && bias->data != nullptr;
+        if (biased) ZB_CHECK(op, "bias", bias, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, E);
+        ZB_CHECK(op, "topkIndex", topkIndex, ZBAL_DATA_TYPE_INT64, ZBAL_DATA_TYPE_INT32, T * topkNum);
+        ZB_CHECK(op, "topkWeight", topkWeight, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, T * topkNum);
+        const zbalhip_group_route_t d = {logits->data, logits->dataType, score, groupScore, renormalize != 0, scale,
+                                         biased ? (const float *)bias->data : nullptr, T, E, topkNum, groupNum, topkGroupNum};
+        return Launched(op, zbalhip_group_route(&d, topkIndex->data, topkIndex->dataType == ZBAL_DATA_TYPE_INT64,
+                                                (float *)topkWeight->data, stream));
+    }
+
+    int32_t GroupRouteBackward(const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *logits, const zbal_tensor_info_t *topkIndex,
+                               zbal_score_t score, int64_t renormalize, double scale, const zbal_tensor_info_t *gradLogits,
+                               aclrtStream stream) override
+    {
+        const char *op = "GroupRouteBackward";
+        ZBAL_VALIDATE_RETURN(logits->dim == 2, op << " failed as logits must be [tokens, experts]", Z_INVALID_PARAM);
+        const int64_t T = logits->shape[0], E = logits->shape[1];
+        ZBAL_VALIDATE_RETURN(topkIndex->dim == 2 && topkIndex->shape[0] == T, op << " failed as topkIndex must be [tokens, topk]", Z_INVALID_PARAM);
+        const int64_t K = topkIndex->shape[1];
+        ZBAL_VALIDATE_RETURN(E > 0 && E <= 1024 && K > 0 && K <= 32, op << " failed as experts " << E << " / topk " << K << " are out of range",
+                             Z_INVALID_PARAM);
+        if (T == 0) return Z_OK;
+        if (!CheckRouteLogits(op, "logits", logits, T * E)) return Z_INVALID_PARAM;
+        ZB_CHECK(op, "topkIndex", topkIndex, ZBAL_DATA_TYPE_INT64, ZBAL_DATA_TYPE_INT32, T * K);
+        ZB_CHECK(op, "gradWeight", gradWeight, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, T * K);
+        ZB_CHECK(op, "gradLogits", gradLogits, logits->dataType, logits->dataType, T * E);
+        const zbalhip_group_route_t d = {logits->data, logits->dataType, score, 0, renormalize != 0, scale, nullptr, T, E, K, 1, 1};
+        return Launched(op, zbalhip_group_route_backward(&d, (const float *)gradWeight->data, topkIndex->data,
+                                                         topkIndex->dataType == ZBAL_DATA_TYPE_INT64, gradLogits->data, stream));
+    }
+
+    /* the operands that both directions of the experts' products share */
+    bool ExpertLinearOperands(const char *op, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                              const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation, zbalhip_expert_linear_t *d)
+    {
+        ZBAL_VALIDATE_RETURN(x->dim == 2, op << " failed as x must be [rows, k]", false);
+        ZBAL_VALIDATE_RETURN(weight->dim == 3 || weight->dim == 2, op << " failed as weight must be [experts, k, n], or [k, n] of one expert", false);
+        const uint16_t format = weight->reserved[0];
+        ZBAL_VALIDATE_RETURN(format == ZBAL_WEIGHT_FORMAT_ND || format == ZBAL_WEIGHT_FORMAT_NK, op << " failed as weight has format " << format, false);
+        const int lead = weight->dim - 2;
+        d->experts = lead ? weight->shape[0] : 1;
+        d->weight_is_nk = format == ZBAL_WEIGHT_FORMAT_NK;
+        d->k = weight->shape[lead + (d->weight_is_nk ? 1 : 0)];
+        d->n = weight->shape[lead + (d->weight_is_nk ? 0 : 1)];
+        d->rows = x->shape[0];
+        d->dtype = x->dataType;
+        d->activation = activation;
+        ZBAL_VALIDATE_RETURN(d->experts > 0 && d->experts <= 1024, op << " failed as experts " << d->experts << " is out of range", false);
+        ZBAL_VALIDATE_RETURN(d->k > 0 && d->k <= ZBALHIP_EXPERT_MAX_WIDTH && d->n > 0 && d->n <= ZBALHIP_EXPERT_MAX_WIDTH &&
+                                 d->rows <= ZBALHIP_EXPERT_MAX_ROWS,
+                             op << " failed as rows " << d->rows << ", k " << d->k << " and n " << d->n << " are out of range", false);
+        ZBAL_VALIDATE_RETURN(x->shape[1] == d->k, op << " failed as x has " << x->shape[1] << " columns, weight takes " << d->k, false);
+        ZBAL_VALIDATE_RETURN(activation != ZBAL_ACTIVATION_SWIGLU || d->n % 2 == 0, op << " failed as swiglu needs an even n, got " << d->n, false);
+        ZBAL_VALIDATE_RETURN(x->dataType == ZBAL_DATA_TYPE_BFP16 || x->dataType == ZBAL_DATA_TYPE_FP16,
+                             op << " failed as x has type " << DtName(x->dataType) << ", expected bf16 or fp16", false);
+        if (d->rows > 0 && !CheckTensor(op, "x", x, x->dataType, x->dataType, d->rows * d->k)) return false;
+        if (!CheckTensor(op, "weight", weight, x->dataType, x->dataType, d->experts * d->k * d->n)) return false;
+        d->weight = weight->data;
+        const bool counted = tokensPerExpert != nullptr && tokensPerExpert->data != nullptr;
+        ZBAL_VALIDATE_RETURN(counted || d->experts == 1, op << " failed as tokensPerExpert is null", false);
+        if (counted) {
+            if (!CheckTensor(op, "tokensPerExpert", tokensPerExpert, ZBAL_DATA_TYPE_INT32, ZBAL_DATA_TYPE_INT64, d->experts)) return false;
+            d->counts = tokensPerExpert->data;
+            d->counts_are_i64 = tokensPerExpert->dataType == ZBAL_DATA_TYPE_INT64;
+        }
+        return true;
+    }
+
+    static bool Given(const zbal_tensor_info_t *t) { return t != nullptr && t->data != nullptr; }
+
+    /* an output must not lie on what the call still reads, or on another output */
+    struct Extent {
+        const char *name;
+        const zbal_tensor_info_t *t;
+    };
+    static bool Apart(const char *op, std::initializer_list<Extent> outputs, std::initializer_list<Extent> inputs)
+    {
+        auto overlap = [](const zbal_tensor_info_t *a, const zbal_tensor_info_t *b) {
+            const uintptr_t a0 = (uintptr_t)a->data, b0 = (uintptr_t)b->data;
+            return a0 < b0 + Numel(b) * ElemSize(b->dataType) && b0 < a0 + Numel(a) * ElemSize(a->dataType);
+        };
+        for (const Extent &o : outputs) {
+            if (!Given(o.t)) continue;
+            for (const auto *set : {&inputs, &outputs})
+                for (const Extent &i : *set)
+                    if (Given(i.t) && i.t != o.t && overlap(o.t, i.t)) {
+                        ZBAL_LOG_AND_SET_LAST_ERROR(op << " failed as " << o.name << " lies on " << i.name);
+                        return false;
+                    }
+        }
+        return true;
+    }
+
+    int32_t ExpertLinear(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, const zbal_tensor_info_t *tokensPerExpert,
+                         const zbal_tensor_info_t *bias, zbal_activation_t activation, const zbal_tensor_info_t *residual,
+                         const zbal_tensor_info_t *y, const zbal_tensor_info_t *preact, const zbal_tensor_info_t *workspace,
+                         aclrtStream stream) override
+    {
+        const char *op = "ExpertLinear";
+        zbalhip_expert_linear_t d = {};
+        if (!ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
+        if (d.rows == 0) return Z_OK;
+        const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.n / 2 : d.n;
+        ZB_CHECK(op, "y", y, x->dataType, ZBAL_DATA_TYPE_FP32, d.rows * cols);
+        if (Given(bias)) ZB_CHECK(op, "bias", bias, x->dataType, ZBAL_DATA_TYPE_FP32, d.experts * d.n);
+        if (Given(residual)) ZB_CHECK(op, "residual", residual, y->dataType, y->dataType, d.rows * cols);
+        if (Given(preact)) ZB_CHECK(op, "preact", preact, x->dataType, x->dataType, d.rows * d.n);
+        if (Given(workspace)) ZB_CHECK(op, "workspace", workspace, workspace->dataType, workspace->dataType, 0);
+        /* in place is all right for the residual: every element is read by the lane that writes it */
+        const zbal_tensor_info_t *apart = Given(residual) && residual->data != y->data ? residual : nullptr;
+        if (!Apart(op, {{"y", y}, {"preact", preact}, {"workspace", workspace}},
+                   {{"x", x}, {"weight", weight}, {"tokensPerExpert", tokensPerExpert}, {"bias", bias}, {"residual", apart}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_expert_linear(&d, x->data, Given(bias) ? bias->data : nullptr, Given(bias) && bias->dataType == ZBAL_DATA_TYPE_FP32,
+                                                  Given(residual) ? residual->data : nullptr, y->data, y->dataType == ZBAL_DATA_TYPE_FP32,
+                                                  Given(preact) ? preact->data : nullptr, Given(workspace) ? workspace->data : nullptr,
+                                                  Given(workspace) ? Numel(workspace) * (int64_t)ElemSize(workspace->dataType) : 0, stream));
+    }
+
+    int32_t ExpertLinearBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                 const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation, const zbal_tensor_info_t *preact,
+                                 const zbal_tensor_info_t *gradX, const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *gradBias,
+                                 const zbal_tensor_info_t *gradPreact, const zbal_tensor_info_t *workspace, aclrtStream stream) override
+    {
+        const char *op = "ExpertLinearBackward";
+        zbalhip_expert_linear_t d = {};
+        if (!ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
+        const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.n / 2 : d.n;
+        const bool rounds = activation != ZBAL_ACTIVATION_NONE || grad->dataType != x->dataType;
+        if (d.rows > 0) {
+            ZB_CHECK(op, "grad", grad, x->dataType, ZBAL_DATA_TYPE_FP32, d.rows * cols);
+            if (activation != ZBAL_ACTIVATION_NONE) {
+                ZBAL_VALIDATE_RETURN(preact != nullptr, op << " failed as preact is null", Z_INVALID_PARAM);
+                ZB_CHECK(op, "preact", preact, x->dataType, x->dataType, d.rows * d.n);
+            }
+            if (rounds) {
+                ZBAL_VALIDATE_RETURN(gradPreact != nullptr, op << " failed as gradPreact is null", Z_INVALID_PARAM);
+                ZB_CHECK(op, "gradPreact", gradPreact, x->dataType, x->dataType, d.rows * d.n);
+            }
+            if (Given(gradX)) ZB_CHECK(op, "gradX", gradX, x->dataType, x->dataType, d.rows * d.k);
+        }
+        if (Given(gradWeight)) ZB_CHECK(op, "gradWeight", gradWeight, x->dataType, ZBAL_DATA_TYPE_FP32, d.experts * d.k * d.n);
+        if (Given(gradBias)) {
+            ZBAL_VALIDATE_RETURN(Given(gradWeight), op << " failed as gradBias comes with gradWeight", Z_INVALID_PARAM);
+            ZB_CHECK(op, "gradBias", gradBias, gradWeight->dataType, gradWeight->dataType, d.experts * d.n);
+        }
+        if (Given(workspace)) ZB_CHECK(op, "workspace", workspace, workspace->dataType, workspace->dataType, 0);
+        if (!Apart(op, {{"gradX", gradX}, {"gradWeight", gradWeight}, {"gradBias", gradBias}, {"gradPreact", rounds ? gradPreact : nullptr}, {"workspace", workspace}},
+                   {{"grad", grad}, {"x", x}, {"weight", weight}, {"tokensPerExpert", tokensPerExpert}, {"preact", preact}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_expert_linear_backward(&d, grad->data, grad->dataType == ZBAL_DATA_TYPE_FP32, x->data,
+                                                           Given(preact) ? preact->data : nullptr, Given(gradX) ? gradX->data : nullptr,
+                                                           Given(gradWeight) ? gradWeight->data : nullptr, Given(gradBias) ? gradBias->data : nullptr,
+                                                           Given(gradWeight) && gradWeight->dataType == ZBAL_DATA_TYPE_FP32,
+                                                           rounds && gradPreact ? gradPreact->data : nullptr, Given(workspace) ? workspace->data : nullptr,
+                                                           Given(workspace) ? Numel(workspace) * (int64_t)ElemSize(workspace->dataType) : 0, stream));
+    }
+
+    int32_t CombineNormalBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *srcTokens, const zbal_tensor_info_t *srcTokensPerEp,
+                                  const zbal_tensor_info_t *topKWeight, const zbal_tensor_info_t *topkIndex,
+                                  const zbal_tensor_info_t *sendTokensIndex, int64_t expertNum, const zbal_tensor_info_t *gradTokens,
+                                  const zbal_tensor_info_t *gradWeight, aclrtStream stream) override
+    {
+        const char *op = "CombineNormalBackward";
+        ZBAL_VALIDATE_RETURN(info_.groupSize == 1, op << " failed as it runs on a group of one rank", Z_INVALID_PARAM);
+        int64_t T = 0, H = 0;
+        if (!TokensShape(op, grad, &T, &H)) return Z_INVALID_PARAM;
+        ZBAL_VALIDATE_RETURN(topkIndex->dim == 2 && topkIndex->shape[0] == T, op << " failed as topkIndex must be [tokens, topk]", Z_INVALID_PARAM);
+        const int64_t K = topkIndex->shape[1];
+        ZBAL_VALIDATE_RETURN(K > 0 && K <= 32, op << " failed as topk " << K << " is out of range", Z_INVALID_PARAM);
+        ZBAL_VALIDATE_RETURN((H * 2) % 32 == 0, op << " failed as hidden " << H << " gives rows that are not a multiple of 32 bytes", Z_INVALID_PARAM);
+        if (T == 0) return Z_OK;
+        ZB_CHECK(op, "grad", grad, ZBAL_DATA_TYPE_BFP16, ZBAL_DATA_TYPE_FP16, T * H);
+        ZB_CHECK(op, "srcTokens", srcTokens, grad->dataType, grad->dataType, H);
+        const int64_t rows = Numel(srcTokens) / H;
+        ZB_CHECK(op, "gradTokens", gradTokens, grad->dataType, grad->dataType, rows * H);
+        ZB_CHECK(op, "srcTokensPerEp", srcTokensPerEp, ZBAL_DATA_TYPE_INT32, ZBAL_DATA_TYPE_INT32, expertNum);
+        ZB_CHECK(op, "topKWeight", topKWeight, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, T * K);
+        ZB_CHECK(op, "topkIndex", topkIndex, ZBAL_DATA_TYPE_INT32, ZBAL_DATA_TYPE_INT64, T * K);
+        ZB_CHECK(op, "sendTokensIndex", sendTokensIndex, ZBAL_DATA_TYPE_INT32, ZBAL_DATA_TYPE_INT32, T * K);
+        ZB_CHECK(op, "gradWeight", gradWeight, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, T * K);
+        if (!Apart(op, {{"gradTokens", gradTokens}, {"gradWeight", gradWeight}},
+                   {{"grad", grad}, {"srcTokens", srcTokens}, {"srcTokensPerEp", srcTokensPerEp}, {"topKWeight", topKWeight}, {"topkIndex", topkIndex}, {"sendTokensIndex", sendTokensIndex}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_combine_backward(grad->data, srcTokens->data, rows, grad->dataType, (const int32_t *)srcTokensPerEp->data,
+                                                     (const float *)topKWeight->data, topkIndex->data, topkIndex->dataType == ZBAL_DATA_TYPE_INT64,
+                                                     (const int32_t *)sendTokensIndex->data, T, H, K, expertNum, gradTokens->data,
+                                                     (float *)gradWeight->data, stream));
+    }
+
     int32_t WeightPrepack(const zbal_tensor_info_t *src, const zbal_tensor_info_t *dst, aclrtStream stream, int64_t) override
     {
         const char *op = "WeightPrepack";
@@ -919,6 +1129,21 @@ public:
 };
 
 } // namespace
+
+int64_t ExpertLinearWorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t experts, zbal_activation_t activation,
+                                   zbal_datatype_t dataType, int64_t weightFormat, bool backward)
+{
+    if (weightFormat != ZBAL_WEIGHT_FORMAT_ND && weightFormat != ZBAL_WEIGHT_FORMAT_NK) return -1;
+    zbalhip_expert_linear_t d = {};
+    d.weight_is_nk = weightFormat == ZBAL_WEIGHT_FORMAT_NK;
+    d.dtype = dataType;
+    d.activation = activation;
+    d.rows = rows;
+    d.k = k;
+    d.n = n;
+    d.experts = experts;
+    return zbalhip_expert_linear_workspace(&d, backward);
+}
 
 CommunicatorPtr MakeGpuCommunicator(const GroupInfo &info) { return std::make_shared<GpuCommunicator>(info); }
 

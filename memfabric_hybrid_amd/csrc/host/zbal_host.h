@@ -206,6 +206,28 @@ public:
                                  int64_t shareGmm1HLen, bool isTensorList, aclrtStream stream, int64_t flags) = 0;
     virtual int32_t TopkRoute(const zbal_tensor_info_t *logits, int64_t topkNum, const zbal_tensor_info_t *topkIndex,
                               const zbal_tensor_info_t *topkWeight, aclrtStream stream, int64_t flags) = 0;
+    virtual int32_t GroupRoute(const zbal_tensor_info_t *logits, const zbal_tensor_info_t *bias, int64_t topkNum, int64_t groupNum,
+                               int64_t topkGroupNum, zbal_score_t score, zbal_group_score_t groupScore, int64_t renormalize,
+                               double scale, const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *topkWeight,
+                               aclrtStream stream) = 0;
+    virtual int32_t GroupRouteBackward(const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *logits,
+                                       const zbal_tensor_info_t *topkIndex, zbal_score_t score, int64_t renormalize,
+                                       double scale, const zbal_tensor_info_t *gradLogits, aclrtStream stream) = 0;
+    virtual int32_t ExpertLinear(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                 const zbal_tensor_info_t *tokensPerExpert, const zbal_tensor_info_t *bias,
+                                 zbal_activation_t activation, const zbal_tensor_info_t *residual, const zbal_tensor_info_t *y,
+                                 const zbal_tensor_info_t *preact, const zbal_tensor_info_t *workspace, aclrtStream stream) = 0;
+    virtual int32_t ExpertLinearBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                         const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation,
+                                         const zbal_tensor_info_t *preact, const zbal_tensor_info_t *gradX,
+                                         const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *gradBias,
+                                         const zbal_tensor_info_t *gradPreact, const zbal_tensor_info_t *workspace,
+                                         aclrtStream stream) = 0;
+    virtual int32_t CombineNormalBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *srcTokens,
+                                          const zbal_tensor_info_t *srcTokensPerEp, const zbal_tensor_info_t *topKWeight,
+                                          const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *sendTokensIndex,
+                                          int64_t expertNum, const zbal_tensor_info_t *gradTokens,
+                                          const zbal_tensor_info_t *gradWeight, aclrtStream stream) = 0;
     virtual int32_t WeightPrepack(const zbal_tensor_info_t *src, const zbal_tensor_info_t *dst, aclrtStream stream,
                                   int64_t flags) = 0;
 
@@ -264,6 +286,10 @@ int64_t MostRidingTokens(int64_t topk, int64_t experts);
  */
 uint64_t FusedWorkspaceBytes(int64_t tokens, int64_t hidden, int64_t topk, int64_t experts, int64_t n1, int64_t shareN1,
                              int64_t quantMode);
+
+/* bytes of workspace of the experts' products, or -1 */
+int64_t ExpertLinearWorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t experts, zbal_activation_t activation,
+                                   zbal_datatype_t dataType, int64_t weightFormat, bool backward);
 
 } // namespace zbal
 

@@ -70,6 +70,19 @@ public:
                          int64_t, int64_t, int64_t, int64_t, bool, aclrtStream, int64_t) override { return Z_OK; }
     int32_t TopkRoute(const zbal_tensor_info_t *, int64_t, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
                       aclrtStream, int64_t) override { return Z_OK; }
+    int32_t GroupRoute(const zbal_tensor_info_t *, const zbal_tensor_info_t *, int64_t, int64_t, int64_t, zbal_score_t, zbal_group_score_t,
+                       int64_t, double, const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t GroupRouteBackward(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, zbal_score_t, int64_t,
+                               double, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t ExpertLinear(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                         zbal_activation_t, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                         const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t ExpertLinearBackward(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                                 zbal_activation_t, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                                 const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t CombineNormalBackward(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                                  const zbal_tensor_info_t *, const zbal_tensor_info_t *, int64_t, const zbal_tensor_info_t *,
+                                  const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
     int32_t WeightPrepack(const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream, int64_t) override { return Z_OK; }
 };
 

@@ -1,0 +1,400 @@
+/*
+ * The experts' products in half precision: rows sorted by expert times the experts' weights, with bias, activation and residual
+ * in the epilogue, and the gradients of the rows, the weights, the bias and the pre-activation.
+ */
+#include "zbal_expert_tile.h"
+
+namespace {
+
+constexpr int XSLOTS = 64;       /* workgroups an XCD runs at a time (32 CUs), for the tile order */
+
+/*
+ * Any sizes: operands pass through registers, sixteen bytes at a time from wherever they start (two bytes' alignment), the last
+ * elements of a row or column one by one.
+ */
+template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN>
+__global__ void __launch_bounds__(WM * WN * 64)
+expert_gemm_any_kernel(XgemmParams p)
+{
+    constexpr int THREADS = WM * WN * 64, MT = TM / WM / 16, NT = TN / WN / 16;
+    constexpr int A_CHUNKS = TM * 8 / THREADS, B_CHUNKS = TN * 8 / THREADS;
+    static_assert(A_CHUNKS * THREADS == TM * 8 || TM * 8 < THREADS, "every thread moves as many chunks");
+    constexpr int AC = A_CHUNKS > 0 ? A_CHUNKS : 1;
+    __shared__ __attribute__((aligned(1024))) uint8_t lds_a[TM * 128];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds_b[TN * 128];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int wm = wave / WN, wn = wave % WN;
+    typedef u32x4 __attribute__((aligned(2))) loose_t;
+
+    const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN, n_tiles = (cols + tile_cols - 1) / tile_cols;
+    int expert, m0, m_end, n0, k_begin, k_end;
+    const int split = p.splits > 1 ? blockIdx.y : 0;
+    if constexpr (REDUCE) {
+        const int m_tiles = (p.M + TM - 1) / TM, per = m_tiles * n_tiles;
+        expert = blockIdx.x / per;
+        const int in = blockIdx.x - expert * per;
+        m0 = in % m_tiles * TM;
+        m_end = p.M;
+        n0 = in / m_tiles * tile_cols;
+        const XSpan s = x_rows_of(p, expert);
+        k_begin = s.begin;
+        k_end = s.end;
+    } else {
+        const XTile t = x_locate<TM>(p, n_tiles, blockIdx.x, XSLOTS);
+        if (t.expert < 0) return;
+        expert = t.expert;
+        m0 = t.row_begin;
+        m_end = t.row_end;
+        n0 = t.n_tile * tile_cols;
+        k_begin = 0;
+        k_end = p.K;
+    }
+    if (p.splits > 1) {          /* whole steps for everyone, in order */
+        const int steps = (k_end - k_begin + XBK - 1) / XBK, each = (steps + p.splits - 1) / p.splits;
+        const int from = k_begin + split * each * XBK;
+        k_end = k_end - from > each * XBK ? from + each * XBK : k_end;
+        k_begin = from < k_end ? from : k_end;
+    }
+    const uint16_t *b = p.b + (REDUCE ? 0 : expert * p.b_stride);
+
+    /* tile column -> column of B; columns past the end of their half are none */
+    auto b_col = [&](int c, int *end) __attribute__((always_inline)) {
+        if (!p.n_half) { *end = p.N; return n0 + c; }
+        *end = c < TN / 2 ? p.n_half : p.N;
+        return c < TN / 2 ? n0 + c : p.n_half + n0 + c - TN / 2;
+    };
+    auto eight = [&](const uint16_t *at, int valid) __attribute__((always_inline)) -> u32x4 {
+        u32x4 v = {0, 0, 0, 0};
+        if (valid >= 8) return *reinterpret_cast<const loose_t *>(at);
+        for (int i = 0; i < valid; ++i) v[i >> 1] |= (uint32_t)at[i] << ((i & 1) * 16);
+        return v;
+    };
+    auto load_a = [&](int c, int k0) __attribute__((always_inline)) -> u32x4 {
+        if constexpr (REDUCE) {
+            const int k = k0 + c / (TM / 8), m = m0 + c % (TM / 8) * 8;
+            return k < k_end ? eight(p.a + (int64_t)k * p.lda + m, m_end - m) : u32x4{0, 0, 0, 0};
+        } else {
+            const int row = m0 + (c >> 3), k = k0 + (c & 7) * 8;
+            return row < m_end ? eight(p.a + (int64_t)row * p.lda + k, k_end - k) : u32x4{0, 0, 0, 0};
+        }
+    };
+    auto load_b = [&](int c, int k0) __attribute__((always_inline)) -> u32x4 {
+        int end;
+        if constexpr (REDUCE || B_TR) {
+            const int k = k0 + c / (TN / 8), n = b_col(c % (TN / 8) * 8, &end);
+            return k < k_end ? eight(b + (int64_t)k * p.ldb + n, end - n) : u32x4{0, 0, 0, 0};
+        } else {
+            const int n = b_col(c >> 3, &end), k = k0 + (c & 7) * 8;
+            return n < end ? eight(b + (int64_t)n * p.ldb + k, k_end - k) : u32x4{0, 0, 0, 0};
+        }
+    };
+
+    f32x4 acc[MT][NT], bias_acc[REDUCE ? (MT > NT ? MT : NT) : 1];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt)
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    for (auto &v : bias_acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    /* the tiles of the other operand's first columns sum this one's, as a product with ones */
+    const bool bias_b = REDUCE && p.bias_side == 1 && m0 == 0 && wm == 0, bias_a = REDUCE && p.bias_side == 2 && n0 == 0 && wn == 0;
+    const uint32_t one2 = DT == ZDT_BF16 ? 0x3f803f80u : 0x3c003c00u;
+    const u32x4 ones = {one2, one2, one2, one2};
+
+    u32x4 ra[AC], rb[B_CHUNKS];
+    auto fetch = [&](int k0) __attribute__((always_inline)) {
+#pragma unroll
+        for (int i = 0; i < AC; ++i)
+            if (A_CHUNKS > 0 || tid < TM * 8) ra[i] = load_a(tid + i * THREADS, k0);
+#pragma unroll
+        for (int i = 0; i < B_CHUNKS; ++i) rb[i] = load_b(tid + i * THREADS, k0);
+    };
+    if (k_begin < k_end) fetch(k_begin);
+    for (int k0 = k_begin; k0 < k_end; k0 += XBK) {
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < AC; ++i)
+            if (A_CHUNKS > 0 || tid < TM * 8) {
+                const int c = tid + i * THREADS;
+                *reinterpret_cast<u32x4 *>(lds_a + (REDUCE ? tr_at<TM>(c / (TM / 8), c % (TM / 8)) : kc_at(c >> 3, c & 7))) = ra[i];
+            }
+#pragma unroll
+        for (int i = 0; i < B_CHUNKS; ++i) {
+            const int c = tid + i * THREADS;
+            *reinterpret_cast<u32x4 *>(lds_b + (REDUCE || B_TR ? tr_at<TN>(c / (TN / 8), c % (TN / 8)) : kc_at(c >> 3, c & 7))) = rb[i];
+        }
+        __syncthreads();
+        if (k0 + XBK < k_end) fetch(k0 + XBK);
+#pragma unroll
+        for (int s = 0; s < 2; ++s) {
+            u32x4 fa[MT];
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) {
+                const int r = wm * (MT * 16) + mt * 16;
+                fa[mt] = REDUCE ? tr_fragment<TM>(lds_a, r, s, lane) : kc_fragment(lds_a, r, s, lane);
+                if (bias_a) bias_acc[mt] = x_mfma<DT>(ones, fa[mt], bias_acc[mt]);
+            }
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt) {
+                const int c = !p.n_half ? wn * (NT * 16) + nt * 16
+                                        : (nt < NT / 2 ? wn * (NT * 8) + nt * 16 : TN / 2 + wn * (NT * 8) + (nt - NT / 2) * 16);
+                const u32x4 fb = REDUCE || B_TR ? tr_fragment<TN>(lds_b, c, s, lane) : kc_fragment(lds_b, c, s, lane);
+                if (bias_b) bias_acc[nt] = x_mfma<DT>(fb, ones, bias_acc[nt]);
+#pragma unroll
+                for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = x_mfma<DT>(fb, fa[mt], acc[mt][nt]);
+            }
+        }
+    }
+
+    /* a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile */
+    const int q4 = (lane >> 4) * 4;
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        const int row = m0 + wm * (MT * 16) + mt * 16 + (lane & 15);
+        if (row >= m_end) continue;
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            if (p.n_half && nt >= NT / 2) break;
+            const int j = n0 + (p.n_half ? wn * (NT * 8) : wn * (NT * 16)) + nt * 16 + q4;
+            for (int i = 0; i < 4; ++i) {
+                if (j + i >= cols) break;
+                if (p.splits > 1) {
+                    float *to = p.partial + ((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + i;
+                    to[0] = acc[mt][nt][i];
+                    if (p.n_half) to[p.n_half] = acc[mt][(nt + NT / 2) % NT][i];
+                } else if constexpr (REDUCE) {
+                    x_store<DT>(p.out, p.out_f32, expert * p.out_stride + row * p.ldo + j + i, acc[mt][nt][i]);
+                } else {
+                    x_finish<DT>(p, expert, row, j + i, acc[mt][nt][i], acc[mt][(nt + NT / 2) % NT][i]);
+                }
+            }
+        }
+    }
+    if constexpr (REDUCE) {
+        auto put = [&](int j, int end, float v) __attribute__((always_inline)) {
+            if (j >= end) return;
+            if (p.splits > 1) p.bias_partial[split * p.ldp + j] = v;
+            else x_store<DT>(p.bias_grad, p.out_f32, (int64_t)expert * end + j, v);
+        };
+        if (bias_b && (lane & 15) == 0)
+#pragma unroll
+            for (int nt = 0; nt < NT; ++nt)
+                for (int i = 0; i < 4; ++i) put(n0 + wn * (NT * 16) + nt * 16 + q4 + i, p.N, bias_acc[nt][i]);
+        if (bias_a && lane < 16)
+#pragma unroll
+            for (int mt = 0; mt < MT; ++mt) put(m0 + wm * (MT * 16) + mt * 16 + lane, p.M, bias_acc[mt][0]);
+    }
+}
+
+/* the sums of a product split along k, in order, and what the epilogue does with them; one expert */
+template <int DT, bool REDUCE>
+__global__ void __launch_bounds__(256)
+expert_join_kernel(XgemmParams p)
+{
+    const int cols = p.n_half ? p.n_half : p.N;
+    const int rows = REDUCE ? p.M : x_rows_of(p, 0).end;
+    const int64_t plane = (int64_t)(REDUCE ? p.M : p.rows) * p.ldp;
+    const int j = blockIdx.x * blockDim.x + threadIdx.x;
+    if (j >= cols) {
+        if (!REDUCE || p.bias_side == 0) return;
+    }
+    for (int row = blockIdx.y; row < rows && j < cols; row += gridDim.y) {
+        const float *from = p.partial + (int64_t)row * p.ldp + j;
+        float z = 0.0f, up = 0.0f;
+        for (int s = 0; s < p.splits; ++s) {
+            z += from[s * plane];
+            if (p.n_half) up += from[s * plane + p.n_half];
+        }
+        if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, row * p.ldo + j, z);
+        else x_finish<DT>(p, 0, row, j, z, up);
+    }
+    if constexpr (REDUCE) {
+        const int n = p.bias_side == 1 ? p.N : (p.bias_side == 2 ? p.M : 0);
+        for (int i = j; blockIdx.y == 0 && i < n; i += gridDim.x * blockDim.x) {
+            float z = 0.0f;
+            for (int s = 0; s < p.splits; ++s) z += p.bias_partial[s * p.ldp + i];
+            x_store<DT>(p.bias_grad, p.out_f32, i, z);
+        }
+    }
+}
+
+/*
+ * The pre-activation's gradient: dz = dy act'(z), for swiglu of both halves; with no activation the rounding of a gradient in 32 bits.
+ * A stream of the three tensors.
+ */
+template <int DT>
+__global__ void __launch_bounds__(256)
+expert_slope_kernel(XgemmParams p, const void *__restrict__ dy, int dy_f32, const uint16_t *__restrict__ z, uint16_t *__restrict__ dz)
+{
+    const int cols = p.n_half ? p.n_half : p.N;
+    int rows = p.rows;
+    if (p.counts) {
+        rows = x_rows_of(p, p.experts - 1).end;
+    }
+    const int64_t n = (int64_t)rows * cols, step = (int64_t)gridDim.x * blockDim.x;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
+        const float d = x_load<DT>(dy, dy_f32, i);
+        if (p.act == ACT_SWIGLU) {
+            const int64_t row = i / cols, at = row * p.N + (i - row * cols);
+            const float g = zb_half_to_f32<DT>(z[at]), u = zb_half_to_f32<DT>(z[at + cols]);
+            dz[at] = (uint16_t)zb_f32_to_half<DT>(d * u * x_slope(ACT_SILU, g));
+            dz[at + cols] = (uint16_t)zb_f32_to_half<DT>(d * x_silu(g));
+        } else {
+            const float s = p.act == ACT_NONE ? 1.0f : x_slope(p.act, zb_half_to_f32<DT>(z[i]));
+            dz[i] = (uint16_t)zb_f32_to_half<DT>(d * s);
+        }
+    }
+}
+
+template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN>
+void launch_any(const XgemmParams &p, hipStream_t st)
+{
+    const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN;
+    const int64_t n_tiles = (cols + tile_cols - 1) / tile_cols;
+    int64_t blocks;
+    if (REDUCE) {
+        blocks = (int64_t)p.experts * ((p.M + TM - 1) / TM) * n_tiles;
+    } else {
+        /* every expert may end with a tile that is not full */
+        const int64_t most = p.rows / TM + p.experts;
+        blocks = (most < p.rows ? most : p.rows) * n_tiles;
+        blocks = (blocks + 7) / 8 * 8;
+    }
+    zb_launch(expert_gemm_any_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN>, dim3((unsigned)blocks, (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
+}
+
+template <int DT, bool REDUCE, bool B_TR> void launch_product(const XgemmParams &p, hipStream_t st)
+{
+    if (!REDUCE && p.rows <= 32 * (int64_t)p.experts) launch_any<DT, REDUCE, B_TR, 16, 128, 1, 4>(p, st);
+    else launch_any<DT, REDUCE, B_TR, 128, 128, 2, 2>(p, st);
+    if (p.splits > 1) {
+        const int cols = p.n_half ? p.n_half : p.N, rows = REDUCE ? p.M : p.rows;
+        zb_launch(expert_join_kernel<DT, REDUCE>, dim3((cols + 255) / 256, rows < 4096 ? rows : 4096), dim3(256), 0, st, p);
+    }
+}
+
+template <bool REDUCE> void launch_types(const XgemmParams &p, int dtype, bool b_tr, hipStream_t st)
+{
+    if (dtype == ZDT_BF16) {
+        if (b_tr) launch_product<ZDT_BF16, REDUCE, true>(p, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_BF16, REDUCE, false>(p, st);
+    } else {
+        if (b_tr) launch_product<ZDT_FP16, REDUCE, true>(p, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_FP16, REDUCE, false>(p, st);
+    }
+}
+
+bool linear_sizes_ok(const zbalhip_expert_linear_t *d)
+{
+    if (!d || d->rows < 0 || d->k <= 0 || d->n <= 0 || d->experts <= 0 || d->experts > 1024) return false;
+    if (d->dtype != ZDT_BF16 && d->dtype != ZDT_FP16) return false;
+    if (d->activation < ACT_NONE || d->activation > ACT_SWIGLU || (d->activation == ACT_SWIGLU && d->n % 2 != 0)) return false;
+    /* the numbers of tiles stay in 32 bits */
+    return d->rows <= ZBALHIP_EXPERT_MAX_ROWS && d->k <= ZBALHIP_EXPERT_MAX_WIDTH && d->n <= ZBALHIP_EXPERT_MAX_WIDTH;
+}
+
+XgemmParams common_params(const zbalhip_expert_linear_t *d)
+{
+    XgemmParams p = {};
+    p.counts = d->counts;
+    p.counts_i64 = d->counts_are_i64;
+    p.experts = (int)d->experts;
+    p.rows = (int)d->rows;
+    p.splits = 1;
+    return p;
+}
+
+} // namespace
+
+extern "C" int64_t zbalhip_expert_linear_workspace(const zbalhip_expert_linear_t *d, int32_t backward)
+{
+    (void)backward;
+    return linear_sizes_ok(d) ? 0 : -1;
+}
+
+extern "C" int32_t zbalhip_expert_linear(const zbalhip_expert_linear_t *d, const void *x, const void *bias, int32_t bias_is_f32,
+                                         const void *residual, void *y, int32_t y_is_f32, void *preact, void *workspace,
+                                         int64_t workspace_bytes, void *stream)
+{
+    if (!linear_sizes_ok(d) || !d->weight || (d->experts > 1 && !d->counts)) return ZBALHIP_INVALID;
+    if (d->rows == 0) return ZBALHIP_OK;
+    if (!x || !y) return ZBALHIP_INVALID;
+    (void)workspace;
+    (void)workspace_bytes;
+    XgemmParams p = common_params(d);
+    p.a = (const uint16_t *)x;
+    p.lda = d->k;
+    p.b = (const uint16_t *)d->weight;
+    p.ldb = d->weight_is_nk ? d->k : d->n;
+    p.b_stride = d->k * d->n;
+    p.K = (int)d->k;
+    p.N = (int)d->n;
+    p.act = d->activation;
+    p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
+    p.out = y;
+    p.out_f32 = y_is_f32;
+    p.ldo = p.n_half ? p.n_half : p.N;
+    p.bias = bias;
+    p.bias_f32 = bias_is_f32;
+    p.residual = residual;
+    p.preact = (uint16_t *)preact;
+    launch_types<false>(p, d->dtype, !d->weight_is_nk, (hipStream_t)stream);
+    return zbalhip_check_launch();
+}
+
+extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t *d, const void *grad, int32_t grad_is_f32, const void *x,
+                                                  const void *preact, void *grad_x, void *grad_weight, void *grad_bias,
+                                                  int32_t weight_grad_is_f32, void *grad_preact, void *workspace,
+                                                  int64_t workspace_bytes, void *stream)
+{
+    if (!linear_sizes_ok(d) || !d->weight || (d->experts > 1 && !d->counts)) return ZBALHIP_INVALID;
+    const bool rounds = d->activation != ACT_NONE || grad_is_f32;
+    if (d->rows > 0 && (!grad || (grad_weight && !x) || (d->activation != ACT_NONE && !preact) || (rounds && !grad_preact))) return ZBALHIP_INVALID;
+    if (grad_bias && !grad_weight) return ZBALHIP_INVALID;
+    if (!grad_x && !grad_weight && !(rounds && d->rows > 0)) return ZBALHIP_OK;
+    (void)workspace;
+    (void)workspace_bytes;
+    hipStream_t st = (hipStream_t)stream;
+    const uint16_t *dz = (const uint16_t *)grad;
+    if (rounds && d->rows > 0) {
+        XgemmParams p = common_params(d);
+        p.N = (int)d->n;
+        p.act = d->activation;
+        p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
+        int64_t blocks = (d->rows * (p.n_half ? p.n_half : p.N) + 1023) / 1024;
+        blocks = blocks < 2048 ? blocks : 2048;
+        if (d->dtype == ZDT_BF16) zb_launch(expert_slope_kernel<ZDT_BF16>, dim3((unsigned)blocks), dim3(256), 0, st, p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact);
+        else zb_launch(expert_slope_kernel<ZDT_FP16>, dim3((unsigned)blocks), dim3(256), 0, st, p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact);
+        dz = (const uint16_t *)grad_preact;
+    }
+    if (grad_x && d->rows > 0) {
+        XgemmParams p = common_params(d);
+        p.a = dz;
+        p.lda = d->n;
+        p.b = (const uint16_t *)d->weight;
+        p.ldb = d->weight_is_nk ? d->k : d->n;
+        p.b_stride = d->k * d->n;
+        p.K = (int)d->n;
+        p.N = (int)d->k;
+        p.out = grad_x;
+        p.ldo = d->k;
+        launch_types<false>(p, d->dtype, d->weight_is_nk != 0, st);
+    }
+    if (grad_weight) {           /* also of experts without rows: zeros */
+        XgemmParams p = common_params(d);
+        const bool nk = d->weight_is_nk != 0;
+        p.a = nk ? dz : (const uint16_t *)x;
+        p.b = nk ? (const uint16_t *)x : dz;
+        p.lda = nk ? d->n : d->k;
+        p.ldb = nk ? d->k : d->n;
+        p.M = (int)p.lda;
+        p.N = (int)p.ldb;
+        p.out = grad_weight;
+        p.out_f32 = weight_grad_is_f32;
+        p.ldo = p.N;
+        p.out_stride = d->k * d->n;
+        p.bias_grad = grad_bias;
+        p.bias_side = grad_bias ? (nk ? 2 : 1) : 0;
+        launch_types<true>(p, d->dtype, true, st);
+    }
+    return zbalhip_check_launch();
+}

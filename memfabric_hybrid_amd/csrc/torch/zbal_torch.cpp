@@ -44,6 +44,12 @@ struct Library {
     decltype(&zbal_combine_low_latency) ll_combine;
     decltype(&zbal_fused_deep_moe) fused;
     decltype(&zbal_fused_deep_moe_workspace_size) fused_workspace;
+    decltype(&zbal_moe_group_route) group_route;
+    decltype(&zbal_moe_group_route_backward) group_route_backward;
+    decltype(&zbal_moe_expert_linear) expert_linear;
+    decltype(&zbal_moe_expert_linear_backward) expert_linear_backward;
+    decltype(&zbal_moe_expert_linear_workspace_size) expert_linear_workspace;
+    decltype(&zbal_combine_normal_backward) combine_backward;
 };
 Library L;
 PyObject *g_check = nullptr;        /* capi.check(op, code): raises ZbalError */
@@ -550,6 +556,221 @@ PyObject *fused(PyObject *const *args, Py_ssize_t nargs)
     return tuple_of(wrap(out), shared ? wrap(share_out) : Owned(Py_None), wrap(nums));
 }
 
+/* ---- unquantised experts and gradients ------------------------------------------------------------------------------ */
+
+/* makes the device of args[1] the current one while a call runs, so that its stream and allocations are that device's */
+struct OnDevice {
+    c10::OptionalDeviceGuard guard;
+    explicit OnDevice(PyObject *const *args, Py_ssize_t n)
+    {
+        if (n < 2) fail(PyExc_TypeError, "wrong number of arguments");
+        const c10::DeviceIndex dev = (c10::DeviceIndex)integer(args[1]);
+        if (c10::hip::getCurrentHIPStream().device_index() != dev) guard.reset_device(c10::Device(c10::DeviceType::CUDA, dev));
+    }
+};
+
+/* a tensor of the device that the call runs on */
+const at::Tensor &local(const Frame &f, const at::Tensor &t)
+{
+    if (t.device() != f.dev) {
+        PyErr_Format(PyExc_ValueError, "expected a tensor on %s, got one on %s", f.dev.str().c_str(), t.device().str().c_str());
+        throw PyFail{};
+    }
+    return t;
+}
+const at::Tensor &local(const Frame &f, int i) { return local(f, f.t(i)); }
+Info local_or_null(const Frame &f, int i) { return f.args[i] == Py_None ? Info() : Info(local(f, i)); }
+
+Owned wrap_or_none(const at::Tensor &t)
+{
+    if (t.defined()) return wrap(t);
+    Py_INCREF(Py_None);
+    return Owned(Py_None);
+}
+
+double number(PyObject *o)
+{
+    const double v = PyFloat_AsDouble(o);
+    if (v == -1.0 && PyErr_Occurred()) throw PyFail{};
+    return v;
+}
+
+void dims(const at::Tensor &t, int64_t n, const char *text)
+{
+    if (t.dim() != n) fail(PyExc_ValueError, text);
+}
+
+/* (comm, dev, logits, bias, topk, groups, kept groups, score, group score, renormalize, scale, ids are int64) -> (idx, weights) */
+PyObject *group_route(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 12);
+    const at::Tensor &logits = local(f, 2);
+    dims(logits, 2, "logits must be [tokens, experts]");
+    const int64_t T = logits.size(0), K = f.n(4);
+    if (K <= 0) fail(PyExc_ValueError, "num_topk must be positive");
+    const at::Tensor idx = f.empty({T, K}, f.n(11) ? at::kLong : at::kInt), w = f.empty({T, K}, at::kFloat);
+    const Info il(logits), ib = local_or_null(f, 3), ii(idx), iw(w);
+    if (ib.ti.data != nullptr && (ib.ti.dim != 1 || ib.ti.shape[0] != logits.size(1))) fail(PyExc_ValueError, "bias must be [experts]");
+    const int64_t groups = f.n(5), kept = f.n(6), score = f.n(7), by = f.n(8), renormalize = f.n(9);
+    const double scale = number(args[10]);
+    check("zbal_moe_group_route", unlocked([&] {
+              return L.group_route(*il, *ib, K, groups, kept, (zbal_score_t)score, (zbal_group_score_t)by, renormalize, scale, *ii, *iw,
+                                   f.comm, f.stream, 0);
+          }));
+    return tuple_of(wrap(idx), wrap(w));
+}
+
+/* (comm, dev, grad of the weights, logits, idx, score, renormalize, scale) -> grad of the logits */
+PyObject *group_route_backward(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 8);
+    const at::Tensor &grad = local(f, 2), &logits = local(f, 3), &idx = local(f, 4);
+    dims(logits, 2, "logits must be [tokens, experts]");
+    dims(idx, 2, "topk_idx must be [tokens, topk]");
+    if (grad.sizes() != idx.sizes()) fail(PyExc_ValueError, "grad must be [tokens, topk]");
+    const at::Tensor out = f.empty(logits.sizes(), logits.scalar_type());
+    const Info ig(grad), il(logits), ii(idx), io(out);
+    const int64_t score = f.n(5), renormalize = f.n(6);
+    const double scale = number(args[7]);
+    check("zbal_moe_group_route_backward", unlocked([&] {
+              return L.group_route_backward(*ig, *il, *ii, (zbal_score_t)score, renormalize, scale, *io, f.comm, f.stream, 0);
+          }));
+    return wrap(out).release();
+}
+
+/* the sizes of one of the experts' products */
+struct LinearShape {
+    int64_t rows, k, n, experts, cols;
+    zbal_activation_t act;
+    zbal_datatype_t type;
+    int64_t format;
+    LinearShape(const at::Tensor &x, const at::Tensor &w, int64_t activation, bool transposed)
+    {
+        dims(x, 2, "x must be [rows, k]");
+        if (w.dim() != 2 && w.dim() != 3) fail(PyExc_ValueError, "weight must be [experts, k, n], or [k, n] of one expert");
+        const int64_t d = w.dim();
+        rows = x.size(0);
+        k = w.size(transposed ? d - 1 : d - 2);
+        n = w.size(transposed ? d - 2 : d - 1);
+        experts = d == 3 ? w.size(0) : 1;
+        act = (zbal_activation_t)activation;
+        cols = act == ZBAL_ACTIVATION_SWIGLU ? n / 2 : n;
+        type = datatype(x.scalar_type());
+        format = transposed ? ZBAL_WEIGHT_FORMAT_NK : ZBAL_WEIGHT_FORMAT_ND;
+        if (x.size(1) != k) fail(PyExc_ValueError, "x and weight have different k");
+    }
+    at::Tensor workspace(const Frame &f, bool backward) const
+    {
+        const int64_t bytes = L.expert_linear_workspace(rows, k, n, experts, act, type, format, backward);
+        return bytes > 0 ? f.empty({bytes}, at::kByte) : at::Tensor();
+    }
+};
+Info info_or_null(const at::Tensor &t) { return t.defined() ? Info(t) : Info(); }
+
+/* a [experts, n] operand, or [n] of one expert */
+Info per_expert(const Frame &f, int i, const LinearShape &s, const char *text)
+{
+    if (f.args[i] == Py_None) return Info();
+    const at::Tensor &t = local(f, i);
+    if (!(t.dim() == 2 && t.size(0) == s.experts && t.size(1) == s.n) && !(t.dim() == 1 && s.experts == 1 && t.size(0) == s.n)) fail(PyExc_ValueError, text);
+    return Info(t);
+}
+Info counts_of(const Frame &f, int i, const LinearShape &s)
+{
+    if (f.args[i] == Py_None) return Info();
+    const at::Tensor &t = local(f, i);
+    if (t.numel() != s.experts) fail(PyExc_ValueError, "tokens_per_expert must be [experts]");
+    return Info(t);
+}
+
+/* (comm, dev, x, weight, counts, bias, activation, residual, output in 32 bits, transposed, preact wanted, out) -> (y, preact) */
+PyObject *expert_linear(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 12);
+    const at::Tensor &x = local(f, 2), &w = local(f, 3);
+    const LinearShape s(x, w, f.n(6), f.n(9) != 0);
+    const at::ScalarType yt = f.n(8) ? at::kFloat : x.scalar_type();
+    at::Tensor y, z;
+    if (args[11] == Py_None) {
+        y = f.empty({s.rows, s.cols}, yt);
+    } else {
+        y = local(f, 11);
+        if (y.scalar_type() != yt || y.dim() != 2 || y.size(0) != s.rows || y.size(1) != s.cols) fail(PyExc_ValueError, "out has another shape or type");
+    }
+    if (f.n(10)) z = f.empty({s.rows, s.n}, x.scalar_type());
+    const at::Tensor ws = s.workspace(f, false);
+    Info iw(w);
+    iw.ti.reserved[0] = (uint16_t)s.format;
+    const Info ix(x), ic = counts_of(f, 4, s), ib = per_expert(f, 5, s, "bias must be [experts, n]"), iy(y), iz = info_or_null(z), iws = info_or_null(ws);
+    Info ir;
+    if (args[7] != Py_None) {
+        const at::Tensor &r = local(f, 7);
+        if (r.sizes() != y.sizes()) fail(PyExc_ValueError, "residual must have the output's shape");
+        ir = Info(r);
+    }
+    check("zbal_moe_expert_linear", unlocked([&] {
+              return L.expert_linear(*ix, *iw, *ic, *ib, s.act, *ir, *iy, *iz, *iws, f.comm, f.stream, 0);
+          }));
+    return tuple_of(wrap(y), wrap_or_none(z));
+}
+
+/*
+ * (comm, dev, grad, x, weight, counts, activation, preact, transposed, bias wanted, weight gradients in 32 bits, x wanted, weight wanted) ->
+ * (grad of x, of weight, of bias, of preact)
+ */
+PyObject *expert_linear_backward(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 13);
+    const at::Tensor &grad = local(f, 2), &x = local(f, 3), &w = local(f, 4);
+    const LinearShape s(x, w, f.n(6), f.n(8) != 0);
+    if (grad.dim() != 2 || grad.size(0) != s.rows || grad.size(1) != s.cols) fail(PyExc_ValueError, "grad must have the output's shape");
+    const at::ScalarType wt = f.n(10) ? at::kFloat : x.scalar_type();
+    const bool bias = f.n(9) != 0;
+    at::Tensor gx, gw, gb, gz;
+    if (f.n(11)) gx = f.empty({s.rows, s.k}, x.scalar_type());
+    if (f.n(12)) gw = f.empty(w.sizes(), wt);
+    if (bias) gb = f.empty(w.dim() == 3 ? at::DimVector{s.experts, s.n} : at::DimVector{s.n}, wt);
+    if (s.act != ZBAL_ACTIVATION_NONE || grad.scalar_type() != x.scalar_type()) gz = f.empty({s.rows, s.n}, x.scalar_type());
+    const at::Tensor ws = s.workspace(f, true);
+    Info iw(w), iz;
+    iw.ti.reserved[0] = (uint16_t)s.format;
+    if (args[7] != Py_None) {
+        const at::Tensor &z = local(f, 7);
+        if (z.dim() != 2 || z.size(0) != s.rows || z.size(1) != s.n) fail(PyExc_ValueError, "preact must be [rows, n]");
+        iz = Info(z);
+    }
+    const Info ig(grad), ix(x), ic = counts_of(f, 5, s), igx = info_or_null(gx), igw = info_or_null(gw), igb = info_or_null(gb), igz = info_or_null(gz),
+               iws = info_or_null(ws);
+    check("zbal_moe_expert_linear_backward", unlocked([&] {
+              return L.expert_linear_backward(*ig, *ix, *iw, *ic, s.act, *iz, *igx, *igw, *igb, *igz, *iws, f.comm, f.stream, 0);
+          }));
+    return tuple_of(wrap_or_none(gx), wrap_or_none(gw), wrap_or_none(gb), wrap_or_none(gz));
+}
+
+/* (comm, dev, grad, x, put_offset, weights, ids, send_idx, experts) -> (grad of x, of the weights) */
+PyObject *combine_backward(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 9);
+    const at::Tensor &grad = local(f, 2), &x = local(f, 3), &w = local(f, 5);
+    dims(grad, 2, "grad must be [tokens, hidden]");
+    if (x.dim() != 2 || x.size(1) != grad.size(1)) fail(PyExc_ValueError, "x must be [rows, hidden]");
+    const at::Tensor ids = expert_ids(local(f, 6));
+    dims(ids, 2, "topk_idx must be [tokens, topk]");
+    if (w.sizes() != ids.sizes() || ids.size(0) != grad.size(0)) fail(PyExc_ValueError, "topk_weights and topk_idx must be [tokens, topk]");
+    const at::Tensor gx = f.empty(x.sizes(), x.scalar_type()), gw = f.empty(w.sizes(), at::kFloat);
+    const Info i0(grad), i1(x), i2(local(f, 4)), i3(w), i4(ids), i5(local(f, 7)), i6(gx), i7(gw);
+    const int64_t E = f.n(8);
+    check("zbal_combine_normal_backward", unlocked([&] {
+              return L.combine_backward(*i0, *i1, *i2, *i3, *i4, *i5, E, *i6, *i7, f.comm, f.stream, 0);
+          }));
+    return tuple_of(wrap(gx), wrap(gw));
+}
+
 /* (tensors,) -> whether every one of them is marked as pre-packed */
 PyObject *all_prepacked(PyObject *const *args, Py_ssize_t nargs)
 {
@@ -587,7 +808,12 @@ PyObject *bind(PyObject *const *args, Py_ssize_t nargs)
         !find(h, "zbal_dispatch_normal_notify_end", &L.notify_end) ||
         !find(h, "zbal_dispatch_normal", &L.dispatch) || !find(h, "zbal_combine_normal", &L.combine) ||
         !find(h, "zbal_dispatch_low_latency", &L.ll_dispatch) || !find(h, "zbal_combine_low_latency", &L.ll_combine) ||
-        !find(h, "zbal_fused_deep_moe", &L.fused) || !find(h, "zbal_fused_deep_moe_workspace_size", &L.fused_workspace))
+        !find(h, "zbal_fused_deep_moe", &L.fused) || !find(h, "zbal_fused_deep_moe_workspace_size", &L.fused_workspace) ||
+        !find(h, "zbal_moe_group_route", &L.group_route) || !find(h, "zbal_moe_group_route_backward", &L.group_route_backward) ||
+        !find(h, "zbal_moe_expert_linear", &L.expert_linear) ||
+        !find(h, "zbal_moe_expert_linear_backward", &L.expert_linear_backward) ||
+        !find(h, "zbal_moe_expert_linear_workspace_size", &L.expert_linear_workspace) ||
+        !find(h, "zbal_combine_normal_backward", &L.combine_backward))
         throw PyFail{};
     Py_INCREF(args[1]);
     Py_XSETREF(g_check, args[1]);
@@ -600,7 +826,9 @@ PyObject *bind(PyObject *const *args, Py_ssize_t nargs)
 #define ZB_METHOD(f) {#f, (PyCFunction)(void (*)(void))entry<f>, METH_FASTCALL, nullptr}
 PyMethodDef g_methods[] = {ZB_METHOD(bind),     ZB_METHOD(topk_route),  ZB_METHOD(layout),     ZB_METHOD(notify),
                            ZB_METHOD(dispatch), ZB_METHOD(dispatch_counts), ZB_METHOD(combine), ZB_METHOD(ll_dispatch),
-                           ZB_METHOD(ll_combine), ZB_METHOD(fused),     ZB_METHOD(all_prepacked), ZB_METHOD(current_stream),
+                           ZB_METHOD(ll_combine), ZB_METHOD(fused),     ZB_METHOD(group_route),
+                           ZB_METHOD(group_route_backward), ZB_METHOD(expert_linear), ZB_METHOD(expert_linear_backward),
+                           ZB_METHOD(combine_backward), ZB_METHOD(all_prepacked), ZB_METHOD(current_stream),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_zbal_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

@@ -75,6 +75,19 @@ def destroy_group(comm):
     capi.check("zbal_comm_destroy", capi.load().zbal_comm_destroy(comm, 0))
 
 
+def _code(table, what, name):
+    if name not in table:
+        raise ValueError("%s must be one of %s, got %r" % (what, ", ".join(sorted(table)), name))
+    return table[name]
+
+
+def _is_fp32(what, dtype, x):
+    """1 for torch.float32, 0 for None or x's own type"""
+    if dtype is not None and dtype != x.dtype and dtype != torch.float32:
+        raise ValueError("%s must be torch.float32 or the type of x" % what)
+    return int(dtype == torch.float32)
+
+
 class OperatorBuffer:
     """One-rank MoE layout / dispatch / combine / fused-MoE operators on worst-case-sized tensors."""
 
@@ -116,6 +129,37 @@ class OperatorBuffer:
     def topk_route(self, logits, num_topk, idx_dtype=torch.int64):
         """idx_dtype: torch.int64 (what get_dispatch_layout takes) or torch.int32 (what dispatch / fused_deep_moe take)"""
         return self.native.topk_route(self._comm, self._dev, logits, num_topk, idx_dtype == torch.int64)
+
+    def group_route(self, logits, num_topk, num_groups=1, topk_groups=1, score="sigmoid", bias=None, group_score="top2",
+                    renormalize=True, scale=1.0, idx_dtype=torch.int64):
+        """zbal_moe_group_route: returns (topk_idx, topk_weights)."""
+        if idx_dtype not in (torch.int64, torch.int32):
+            raise ValueError("idx_dtype must be torch.int64 or torch.int32")
+        return self.native.group_route(self._comm, self._dev, logits, bias, num_topk, num_groups, topk_groups,
+                                       _code(capi.SCORES, "score", score), _code(capi.GROUP_SCORES, "group_score", group_score),
+                                       int(bool(renormalize)), scale, int(idx_dtype == torch.int64))
+
+    def group_route_backward(self, grad_weights, logits, topk_idx, score="sigmoid", renormalize=True, scale=1.0):
+        """zbal_moe_group_route_backward: returns the logits' gradient."""
+        return self.native.group_route_backward(self._comm, self._dev, grad_weights, logits, topk_idx,
+                                                _code(capi.SCORES, "score", score), int(bool(renormalize)), scale)
+
+    # -- unquantised experts (extension) --------------------------------------------------------
+    def expert_linear(self, x, weight, tokens_per_expert=None, bias=None, activation="none", residual=None, out_dtype=None,
+                      transposed=False, return_preact=False, out=None):
+        """zbal_moe_expert_linear: returns (y, preact or None)."""
+        return self.native.expert_linear(self._comm, self._dev, x, weight, tokens_per_expert, bias,
+                                         _code(capi.ACTIVATIONS, "activation", activation), residual,
+                                         _is_fp32("out_dtype", out_dtype, x), int(bool(transposed)), int(bool(return_preact)), out)
+
+    def expert_linear_backward(self, grad, x, weight, tokens_per_expert=None, activation="none", preact=None, transposed=False,
+                               bias=False, weight_grad_dtype=None, need_x=True, need_weight=True):
+        """zbal_moe_expert_linear_backward: returns (grad_x, grad_weight, grad_bias, grad_preact), None for what was not asked
+        for, and for grad_preact where it is grad itself."""
+        return self.native.expert_linear_backward(
+            self._comm, self._dev, grad, x, weight, tokens_per_expert, _code(capi.ACTIVATIONS, "activation", activation), preact,
+            int(bool(transposed)), int(bool(bias)), _is_fp32("weight_grad_dtype", weight_grad_dtype, x), int(bool(need_x)),
+            int(bool(need_weight)))
 
     # -- normal mode -------------------------------------------------------------------------
     def get_dispatch_layout(self, topk_idx, num_experts):
@@ -163,6 +207,12 @@ class OperatorBuffer:
         """zbal_deepep.cpp:395-452."""
         return self.native.combine(self._comm, self._dev, x, handle["put_offset"], topk_weights, handle["expert_ids"],
                                    handle["send_token_idx"], handle["balance_matrix"], handle["num_experts"])
+
+    def combine_backward(self, grad, x, handle, topk_weights):
+        """zbal_combine_normal_backward: the gradients of combine(x, handle, topk_weights), as (grad_x, grad_topk_weights). Rows of
+        grad_x that no pick went to are not written."""
+        return self.native.combine_backward(self._comm, self._dev, grad, x, handle["put_offset"], topk_weights,
+                                            handle["expert_ids"], handle["send_token_idx"], handle["num_experts"])
 
     # -- low-latency mode ----------------------------------------------------------------------
     def low_latency_dispatch(self, x, topk_idx, num_max_dispatch_tokens_per_rank, num_experts, use_fp8=True,

@@ -2,7 +2,9 @@
  * The experts' products in half precision: rows sorted by expert times the experts' weights, with bias, activation and residual
  * in the epilogue, and the gradients of the rows, the weights, the bias and the pre-activation.
  */
-#include "zbal_expert_tile.h"
+#include <cmath>
+
+#include "zbal_expert_wide.h"
 
 namespace {
 
@@ -20,8 +22,8 @@ expert_gemm_any_kernel(XgemmParams p)
     constexpr int A_CHUNKS = TM * 8 / THREADS, B_CHUNKS = TN * 8 / THREADS;
     static_assert(A_CHUNKS * THREADS == TM * 8 || TM * 8 < THREADS, "every thread moves as many chunks");
     constexpr int AC = A_CHUNKS > 0 ? A_CHUNKS : 1;
-    __shared__ __attribute__((aligned(1024))) uint8_t lds_a[TM * 128];
-    __shared__ __attribute__((aligned(1024))) uint8_t lds_b[TN * 128];
+    __shared__ __attribute__((aligned(1024))) uint8_t lds[(TM + TN) * 128];
+    uint8_t *lds_a = lds, *lds_b = lds + TM * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
     typedef u32x4 __attribute__((aligned(2))) loose_t;
@@ -147,32 +149,10 @@ expert_gemm_any_kernel(XgemmParams p)
 
     /* a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile */
     const int q4 = (lane >> 4) * 4;
-#pragma unroll
-    for (int mt = 0; mt < MT; ++mt) {
-        const int row = m0 + wm * (MT * 16) + mt * 16 + (lane & 15);
-        if (row >= m_end) continue;
-#pragma unroll
-        for (int nt = 0; nt < NT; ++nt) {
-            if (p.n_half && nt >= NT / 2) break;
-            const int j = n0 + (p.n_half ? wn * (NT * 8) : wn * (NT * 16)) + nt * 16 + q4;
-            for (int i = 0; i < 4; ++i) {
-                if (j + i >= cols) break;
-                if (p.splits > 1) {
-                    float *to = p.partial + ((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + i;
-                    to[0] = acc[mt][nt][i];
-                    if (p.n_half) to[p.n_half] = acc[mt][(nt + NT / 2) % NT][i];
-                } else if constexpr (REDUCE) {
-                    x_store<DT>(p.out, p.out_f32, expert * p.out_stride + row * p.ldo + j + i, acc[mt][nt][i]);
-                } else {
-                    x_finish<DT>(p, expert, row, j + i, acc[mt][nt][i], acc[mt][(nt + NT / 2) % NT][i]);
-                }
-            }
-        }
-    }
     if constexpr (REDUCE) {
         auto put = [&](int j, int end, float v) __attribute__((always_inline)) {
             if (j >= end) return;
-            if (p.splits > 1) p.bias_partial[split * p.ldp + j] = v;
+            if (p.splits > 1) p.bias_partial[split * p.bias_ldp + j] = v;
             else x_store<DT>(p.bias_grad, p.out_f32, (int64_t)expert * end + j, v);
         };
         if (bias_b && (lane & 15) == 0)
@@ -183,35 +163,74 @@ expert_gemm_any_kernel(XgemmParams p)
 #pragma unroll
             for (int mt = 0; mt < MT; ++mt) put(m0 + wm * (MT * 16) + mt * 16 + lane, p.M, bias_acc[mt][0]);
     }
+    /*
+     * Through the LDS, a row sub-tile of every wave at a time: neighbouring lanes then have neighbouring columns, whose loads and stores are one
+     * access each, and several of them under way (1021 x 1001 x 1531, gelu, bias and residual: 63 us, from the sums' own lanes, one after the other, 96).
+     */
+    constexpr int LD = TN + 1, ROWS = WM * 16;
+    static_assert(ROWS * LD * 4 <= (TM + TN) * 128, "sums fit the operands' place");
+    float *sums = reinterpret_cast<float *>(lds);
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) {
+        __syncthreads();
+#pragma unroll
+        for (int nt = 0; nt < NT; ++nt) {
+            const int c = !p.n_half ? wn * (NT * 16) + nt * 16 : (nt < NT / 2 ? wn * (NT * 8) + nt * 16 : TN / 2 + wn * (NT * 8) + (nt - NT / 2) * 16);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) sums[(wm * 16 + (lane & 15)) * LD + c + q4 + i] = acc[mt][nt][i];
+        }
+        __syncthreads();
+#pragma unroll 4
+        for (int i = tid; i < ROWS * TN; i += THREADS) {
+            const int r = i / TN, c = i % TN, row = m0 + r / 16 * (MT * 16) + mt * 16 + r % 16;
+            const bool up = p.n_half && c >= TN / 2;
+            const int j = n0 + (up ? c - TN / 2 : c);
+            if (row >= m_end || j >= cols) continue;
+            const float z = sums[r * LD + c];
+            if (p.splits > 1) p.partial[((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + (up ? p.n_half : 0)] = z;
+            else if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, expert * p.out_stride + row * p.ldo + j, z);
+            else if (!up) x_finish<DT>(p, expert, row, j, z, p.n_half ? sums[r * LD + TN / 2 + c] : 0.0f);
+        }
+    }
 }
 
-/* the sums of a product split along k, in order, and what the epilogue does with them; one expert */
+/* the sums of a product split along k, in order, and what the epilogue does with them; one expert. Four columns a lane */
 template <int DT, bool REDUCE>
 __global__ void __launch_bounds__(256)
 expert_join_kernel(XgemmParams p)
 {
-    const int cols = p.n_half ? p.n_half : p.N;
+    const int cols = p.n_half ? p.n_half : p.N, quads = (cols + 3) / 4;
     const int rows = REDUCE ? p.M : x_rows_of(p, 0).end;
-    const int64_t plane = (int64_t)(REDUCE ? p.M : p.rows) * p.ldp;
-    const int j = blockIdx.x * blockDim.x + threadIdx.x;
-    if (j >= cols) {
-        if (!REDUCE || p.bias_side == 0) return;
-    }
-    for (int row = blockIdx.y; row < rows && j < cols; row += gridDim.y) {
+    const int64_t plane = (int64_t)(REDUCE ? p.M : p.rows) * p.ldp, total = (int64_t)rows * quads;
+    const bool whole = p.ldo % 4 == 0 && p.N % 4 == 0 && p.n_half % 4 == 0;
+    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
+        const int row = (int)(i / quads), j = (int)(i - (int64_t)row * quads) * 4;
         const float *from = p.partial + (int64_t)row * p.ldp + j;
-        float z = 0.0f, up = 0.0f;
-        for (int s = 0; s < p.splits; ++s) {
-            z += from[s * plane];
-            if (p.n_half) up += from[s * plane + p.n_half];
+        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f}, up = z;
+        if (whole) {
+            for (int s = 0; s < p.splits; ++s) {
+                z += *reinterpret_cast<const f32x4 *>(from + s * plane);
+                if (p.n_half) up += *reinterpret_cast<const f32x4 *>(from + s * plane + p.n_half);
+            }
+            if constexpr (REDUCE) x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, z);
+            else x_finish4<DT>(p, 0, row, j, z, up);
+        } else {
+            for (int c = 0; c < 4 && j + c < cols; ++c) {
+                float zc = 0.0f, uc = 0.0f;
+                for (int s = 0; s < p.splits; ++s) {
+                    zc += from[s * plane + c];
+                    if (p.n_half) uc += from[s * plane + p.n_half + c];
+                }
+                if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, row * p.ldo + j + c, zc);
+                else x_finish<DT>(p, 0, row, j + c, zc, uc);
+            }
         }
-        if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, row * p.ldo + j, z);
-        else x_finish<DT>(p, 0, row, j, z, up);
     }
     if constexpr (REDUCE) {
         const int n = p.bias_side == 1 ? p.N : (p.bias_side == 2 ? p.M : 0);
-        for (int i = j; blockIdx.y == 0 && i < n; i += gridDim.x * blockDim.x) {
+        for (int i = blockIdx.x * blockDim.x + threadIdx.x; i < n; i += gridDim.x * blockDim.x) {
             float z = 0.0f;
-            for (int s = 0; s < p.splits; ++s) z += p.bias_partial[s * p.ldp + i];
+            for (int s = 0; s < p.splits; ++s) z += p.bias_partial[s * p.bias_ldp + i];
             x_store<DT>(p.bias_grad, p.out_f32, i, z);
         }
     }
@@ -262,24 +281,148 @@ void launch_any(const XgemmParams &p, hipStream_t st)
     zb_launch(expert_gemm_any_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN>, dim3((unsigned)blocks, (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
 }
 
-template <int DT, bool REDUCE, bool B_TR> void launch_product(const XgemmParams &p, hipStream_t st)
+/* workgroups of a product in tiles of TM x TN: for rows sorted by expert as many as there can be tiles */
+template <bool REDUCE, int TM, int TN> unsigned tiles_of(const XgemmParams &p)
 {
-    if (!REDUCE && p.rows <= 32 * (int64_t)p.experts) launch_any<DT, REDUCE, B_TR, 16, 128, 1, 4>(p, st);
-    else launch_any<DT, REDUCE, B_TR, 128, 128, 2, 2>(p, st);
-    if (p.splits > 1) {
-        const int cols = p.n_half ? p.n_half : p.N, rows = REDUCE ? p.M : p.rows;
-        zb_launch(expert_join_kernel<DT, REDUCE>, dim3((cols + 255) / 256, rows < 4096 ? rows : 4096), dim3(256), 0, st, p);
+    const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN;
+    const int64_t n_tiles = (cols + tile_cols - 1) / tile_cols;
+    if (REDUCE) return (unsigned)((p.experts * ((p.M + TM - 1) / TM) * n_tiles + 7) / 8 * 8);
+    const int64_t most = p.rows / TM + p.experts;          /* every expert may end with a tile that is not full */
+    return (unsigned)(((most < p.rows ? most : p.rows) * n_tiles + 7) / 8 * 8);
+}
+
+template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN, int STAGES>
+void launch_direct(const XgemmParams &p, hipStream_t st)
+{
+    zb_launch(expert_gemm_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN, STAGES>, dim3(tiles_of<REDUCE, TM, TN>(p), (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
+}
+
+template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStream_t st)
+{
+    p.through_lds = !REDUCE && (p.bias || p.residual || p.preact || (p.act != ACT_NONE && p.act != ACT_SWIGLU));
+    unsigned blocks = tiles_of<REDUCE, 256, 256>(p);
+    if (!p.through_lds && blocks > XW_CUS) blocks = XW_CUS;
+    const dim3 grid(blocks), block(512);
+    if constexpr (REDUCE) {
+        if (p.bias_side == 1) zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 1>, grid, block, 0, st, p);
+        else if (p.bias_side == 2) zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 2>, grid, block, 0, st, p);
+        else zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 0>, grid, block, 0, st, p);
+    } else {
+        zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR>, grid, block, 0, st, p);
     }
 }
 
-template <bool REDUCE> void launch_types(const XgemmParams &p, int dtype, bool b_tr, hipStream_t st)
+/* every row of the operands and outputs starts at a multiple of eight elements */
+inline bool rows_are_aligned(const XgemmParams &p) { return p.lda % 8 == 0 && p.ldb % 8 == 0 && p.ldo % 8 == 0 && p.N % 8 == 0 && p.n_half % 8 == 0; }
+
+/* how a product is cut: the tiles, and the parts along k whose sums a second launch adds up */
+enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16 };
+struct Plan {
+    Cut cut;
+    int splits;
+    int64_t bytes;               /* of workspace */
+};
+
+/*
+ * The cut that takes least time by what a step of 64 k takes on a CU, `alone` with one tile there and `full` with as many as run side by side
+ * (us). Measured, best by this rule / the next: 32 experts of 7168 x 4096: 128 rows each wide 375 / 128 480, 32 rows 64 x 128 318 / 32 x 128 359;
+ * one matrix: 4096 x 7168 x 256 128 in four parts 31 / 64 x 128 in four 33 / 64 x 64 whole 40; 2048 x 4096 x 2048 128 43 / 64 x 128 52; 1024 x 2048 x
+ * 2048 64 x 64 17.7 / 128 20.2; 64 x 2048 x 7168 16 x 64 11.5 / 64 x 64 13.1. Weights' gradients end in large stores, which only the wide tiles overlap with
+ * products: 32 experts of 7168 x 4096, 128 rows each, wide 432 / 128 1009. Parts along k, for one expert, cost their sums twice through the memory, and a launch.
+ * Where the weights' stream is what takes the time, wide tiles read longer pieces of rows whose columns are consecutive (16 rows over 32 experts of 7168 x
+ * 4096: wide 139, 32 x 128 148, 16 x 64 162; k consecutive 145, 136, 137).
+ */
+Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
+{
+    struct Kind { Cut cut; int tm, tn, at_once; double alone, full; };
+    static const Kind kinds[] = {{CUT_WIDE, 256, 256, 1, 1.5, 1.5}, {CUT_128, 128, 128, 1, 0.57, 0.57}, {CUT_64_128, 64, 128, 2, 0.55, 0.75},
+                                 {CUT_64, 64, 64, 2, 0.4, 0.45}, {CUT_32, 32, 128, 2, 0.35, 0.5}, {CUT_16, 16, 64, 2, 0.2, 0.27}};
+    static const Kind any[] = {{CUT_ANY, 128, 128, 2, 1.2, 1.6}, {CUT_ANY_64, 64, 64, 4, 0.7, 1.0}, {CUT_ANY_16, 16, 128, 4, 0.6, 0.9}};
+    const bool aligned = rows_are_aligned(p);
+    const Kind *list = aligned ? kinds : any;
+    const int count = aligned ? 6 : 3;
+    const double steps = ((reduce ? (double)p.rows / p.experts : p.K) + XBK - 1) / XBK, per_expert = (double)p.rows / p.experts;
+    const double reached = p.rows < p.experts ? p.rows : p.experts;
+    const int cols = p.n_half ? p.n_half : p.N, rows = reduce ? p.M : p.rows;
+    Plan plan = {list[0].cut, 1, 0};
+    double best = 0.0;
+    for (int i = 0; i < count; ++i) {
+        const Kind &k = list[i];
+        if (reduce && k.tm < 64) continue;
+        const int tile_cols = p.n_half ? k.tn / 2 : k.tn;
+        const double n_tiles = (cols + tile_cols - 1) / tile_cols;
+        double m_tiles = reduce ? (double)p.experts * ((p.M + k.tm - 1) / k.tm) : (p.rows + k.tm - 1) / k.tm;
+        if (!reduce && p.experts > 1) {      /* every expert ends with half a tile, on average */
+            m_tiles = p.experts * (per_expert / k.tm + 0.5);
+            if (m_tiles < reached) m_tiles = reached;
+        }
+        const double tiles = m_tiles * n_tiles;
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            if (splits > 1 && (p.experts > 1 || k.cut == CUT_WIDE || steps / splits < 4 || tiles * splits > 512)) break;
+            const double each = tiles * splits, per_round = 256.0 * k.at_once;
+            double us = (each <= 256 ? k.alone : k.full * ceil(each / per_round)) * ceil(steps / splits);
+            if (k.cut == CUT_WIDE && !reduce && per_expert <= 128) us *= 0.6;      /* tiles without a second half */
+            /* an epilogue of stores in every round, which takes no time beside the next tile's steps in the wide kernel */
+            if (reduce) us += ceil(each / per_round) * (k.cut == CUT_WIDE ? 1.0 : 8.0);
+            if (splits > 1) us += 4.0 + (double)splits * rows * p.N * 8 / 5e6;
+            const double stream = !b_cols ? 5.3e6 : (k.tn == 256 ? 5.3e6 : (k.tn == 128 ? 5.0e6 : 4.5e6));       /* bytes a us */
+            const double memory = reached * p.b_stride * 2 / stream;
+            if (us < memory) us = memory;
+            if (best == 0.0 || us < best * 0.97) {
+                best = us;
+                plan.cut = k.cut;
+                plan.splits = splits;
+            }
+        }
+    }
+    if (plan.splits > 1) {
+        const int64_t ldp = (p.N + 3) / 4 * 4, bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
+        plan.bytes = plan.splits * (rows * ldp + (reduce ? bias_ldp : 0)) * 4;
+    }
+    return plan;
+}
+
+template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, void *workspace, int64_t workspace_bytes, hipStream_t st)
+{
+    Plan plan = plan_product(p, REDUCE, REDUCE || B_TR);
+    if (plan.bytes > workspace_bytes || !workspace) plan.splits = 1;
+    if (plan.splits > 1) {
+        p.splits = plan.splits;
+        p.ldp = (p.N + 3) / 4 * 4;
+        p.partial = (float *)workspace;
+        p.bias_partial = p.partial + (int64_t)p.splits * (REDUCE ? p.M : p.rows) * p.ldp;
+        p.bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
+    }
+    switch (plan.cut) {
+        case CUT_WIDE: launch_wide<DT, REDUCE, B_TR>(p, st); break;
+        case CUT_128: launch_direct<DT, REDUCE, B_TR, 128, 128, 2, 4, 4>(p, st); break;
+        case CUT_64_128: launch_direct<DT, REDUCE, B_TR, 64, 128, 2, 2, 3>(p, st); break;
+        case CUT_64: launch_direct<DT, REDUCE, B_TR, 64, 64, 2, 2, 4>(p, st); break;
+        case CUT_ANY: launch_any<DT, REDUCE, B_TR, 128, 128, 2, 2>(p, st); break;
+        case CUT_ANY_64: launch_any<DT, REDUCE, B_TR, 64, 64, 2, 2>(p, st); break;
+        default:
+            if constexpr (!REDUCE) {
+                if (plan.cut == CUT_32) launch_direct<DT, REDUCE, B_TR, 32, 128, 2, 2, 4>(p, st);
+                else if (plan.cut == CUT_16) launch_direct<DT, REDUCE, B_TR, 16, 64, 1, 2, 8>(p, st);
+                else launch_any<DT, REDUCE, B_TR, 16, 128, 1, 4>(p, st);
+            }
+    }
+    if (p.splits > 1) {
+        const int cols = p.n_half ? p.n_half : p.N, rows = REDUCE ? p.M : p.rows;
+        const int64_t quads = (int64_t)rows * ((cols + 3) / 4);
+        const unsigned blocks = (unsigned)((quads + 255) / 256 < 4096 ? (quads + 255) / 256 : 4096);
+        zb_launch(expert_join_kernel<DT, REDUCE>, dim3(blocks), dim3(256), 0, st, p);
+    }
+}
+
+template <bool REDUCE> void launch_types(const XgemmParams &p, int dtype, bool b_tr, void *ws, int64_t ws_bytes, hipStream_t st)
 {
     if (dtype == ZDT_BF16) {
-        if (b_tr) launch_product<ZDT_BF16, REDUCE, true>(p, st);
-        else if constexpr (!REDUCE) launch_product<ZDT_BF16, REDUCE, false>(p, st);
+        if (b_tr) launch_product<ZDT_BF16, REDUCE, true>(p, ws, ws_bytes, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_BF16, REDUCE, false>(p, ws, ws_bytes, st);
     } else {
-        if (b_tr) launch_product<ZDT_FP16, REDUCE, true>(p, st);
-        else if constexpr (!REDUCE) launch_product<ZDT_FP16, REDUCE, false>(p, st);
+        if (b_tr) launch_product<ZDT_FP16, REDUCE, true>(p, ws, ws_bytes, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_FP16, REDUCE, false>(p, ws, ws_bytes, st);
     }
 }
 
@@ -303,12 +446,57 @@ XgemmParams common_params(const zbalhip_expert_linear_t *d)
     return p;
 }
 
+/* the three products as tiles know them; tensors that the plan does not turn on are set where they are launched */
+XgemmParams forward_params(const zbalhip_expert_linear_t *d)
+{
+    XgemmParams p = common_params(d);
+    p.lda = d->k;
+    p.b = (const uint16_t *)d->weight;
+    p.ldb = d->weight_is_nk ? d->k : d->n;
+    p.b_stride = d->k * d->n;
+    p.K = (int)d->k;
+    p.N = (int)d->n;
+    p.act = d->activation;
+    p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
+    p.ldo = p.n_half ? p.n_half : p.N;
+    return p;
+}
+
+XgemmParams rows_gradient_params(const zbalhip_expert_linear_t *d)
+{
+    XgemmParams p = common_params(d);
+    p.lda = d->n;
+    p.b = (const uint16_t *)d->weight;
+    p.ldb = d->weight_is_nk ? d->k : d->n;
+    p.b_stride = d->k * d->n;
+    p.K = (int)d->n;
+    p.N = (int)d->k;
+    p.ldo = d->k;
+    return p;
+}
+
+XgemmParams weights_gradient_params(const zbalhip_expert_linear_t *d)
+{
+    XgemmParams p = common_params(d);
+    p.lda = d->weight_is_nk ? d->n : d->k;
+    p.ldb = d->weight_is_nk ? d->k : d->n;
+    p.M = (int)p.lda;
+    p.N = (int)p.ldb;
+    p.ldo = p.N;
+    p.out_stride = d->k * d->n;
+    return p;
+}
+
 } // namespace
 
 extern "C" int64_t zbalhip_expert_linear_workspace(const zbalhip_expert_linear_t *d, int32_t backward)
 {
-    (void)backward;
-    return linear_sizes_ok(d) ? 0 : -1;
+    if (!linear_sizes_ok(d)) return -1;
+    if (d->rows == 0) return 0;
+    if (!backward) return plan_product(forward_params(d), false, !d->weight_is_nk).bytes;
+    /* one after the other in the same memory */
+    const int64_t a = plan_product(rows_gradient_params(d), false, d->weight_is_nk != 0).bytes, b = plan_product(weights_gradient_params(d), true, true).bytes;
+    return a > b ? a : b;
 }
 
 extern "C" int32_t zbalhip_expert_linear(const zbalhip_expert_linear_t *d, const void *x, const void *bias, int32_t bias_is_f32,
@@ -318,26 +506,15 @@ extern "C" int32_t zbalhip_expert_linear(const zbalhip_expert_linear_t *d, const
     if (!linear_sizes_ok(d) || !d->weight || (d->experts > 1 && !d->counts)) return ZBALHIP_INVALID;
     if (d->rows == 0) return ZBALHIP_OK;
     if (!x || !y) return ZBALHIP_INVALID;
-    (void)workspace;
-    (void)workspace_bytes;
-    XgemmParams p = common_params(d);
+    XgemmParams p = forward_params(d);
     p.a = (const uint16_t *)x;
-    p.lda = d->k;
-    p.b = (const uint16_t *)d->weight;
-    p.ldb = d->weight_is_nk ? d->k : d->n;
-    p.b_stride = d->k * d->n;
-    p.K = (int)d->k;
-    p.N = (int)d->n;
-    p.act = d->activation;
-    p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
     p.out = y;
     p.out_f32 = y_is_f32;
-    p.ldo = p.n_half ? p.n_half : p.N;
     p.bias = bias;
     p.bias_f32 = bias_is_f32;
     p.residual = residual;
     p.preact = (uint16_t *)preact;
-    launch_types<false>(p, d->dtype, !d->weight_is_nk, (hipStream_t)stream);
+    launch_types<false>(p, d->dtype, !d->weight_is_nk, workspace, workspace_bytes, (hipStream_t)stream);
     return zbalhip_check_launch();
 }
 
@@ -351,8 +528,6 @@ extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t 
     if (d->rows > 0 && (!grad || (grad_weight && !x) || (d->activation != ACT_NONE && !preact) || (rounds && !grad_preact))) return ZBALHIP_INVALID;
     if (grad_bias && !grad_weight) return ZBALHIP_INVALID;
     if (!grad_x && !grad_weight && !(rounds && d->rows > 0)) return ZBALHIP_OK;
-    (void)workspace;
-    (void)workspace_bytes;
     hipStream_t st = (hipStream_t)stream;
     const uint16_t *dz = (const uint16_t *)grad;
     if (rounds && d->rows > 0) {
@@ -367,34 +542,20 @@ extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t 
         dz = (const uint16_t *)grad_preact;
     }
     if (grad_x && d->rows > 0) {
-        XgemmParams p = common_params(d);
+        XgemmParams p = rows_gradient_params(d);
         p.a = dz;
-        p.lda = d->n;
-        p.b = (const uint16_t *)d->weight;
-        p.ldb = d->weight_is_nk ? d->k : d->n;
-        p.b_stride = d->k * d->n;
-        p.K = (int)d->n;
-        p.N = (int)d->k;
         p.out = grad_x;
-        p.ldo = d->k;
-        launch_types<false>(p, d->dtype, d->weight_is_nk != 0, st);
+        launch_types<false>(p, d->dtype, d->weight_is_nk != 0, workspace, workspace_bytes, st);
     }
     if (grad_weight) {           /* also of experts without rows: zeros */
-        XgemmParams p = common_params(d);
-        const bool nk = d->weight_is_nk != 0;
-        p.a = nk ? dz : (const uint16_t *)x;
-        p.b = nk ? (const uint16_t *)x : dz;
-        p.lda = nk ? d->n : d->k;
-        p.ldb = nk ? d->k : d->n;
-        p.M = (int)p.lda;
-        p.N = (int)p.ldb;
+        XgemmParams p = weights_gradient_params(d);
+        p.a = d->weight_is_nk ? dz : (const uint16_t *)x;
+        p.b = d->weight_is_nk ? (const uint16_t *)x : dz;
         p.out = grad_weight;
         p.out_f32 = weight_grad_is_f32;
-        p.ldo = p.N;
-        p.out_stride = d->k * d->n;
         p.bias_grad = grad_bias;
-        p.bias_side = grad_bias ? (nk ? 2 : 1) : 0;
-        launch_types<true>(p, d->dtype, true, st);
+        p.bias_side = grad_bias ? (d->weight_is_nk ? 2 : 1) : 0;
+        launch_types<true>(p, d->dtype, true, workspace, workspace_bytes, st);
     }
     return zbalhip_check_launch();
 }

@@ -39,10 +39,11 @@ struct XgemmParams {
     uint16_t *preact;            /* [rows, N] */
     void *bias_grad;             /* REDUCE: [experts, bias_n], of out's type */
     int bias_side;               /* REDUCE: the operand whose columns it sums: 1 = b, 2 = a */
-    float *partial;              /* split along k: [splits][rows of C][ldp] sums instead of out; bias sums [splits][ldp] behind */
+    float *partial;              /* split along k: [splits][rows of C][ldp] sums instead of out, and [splits][bias_ldp] of the bias's */
     float *bias_partial;
-    int64_t ldp;
+    int64_t ldp, bias_ldp;
     int splits;
+    int through_lds;             /* the wide kernel's epilogue: more than a swiglu, with a workgroup per tile */
 };
 
 typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
@@ -251,6 +252,34 @@ template <int DT> __device__ __forceinline__ void x_finish(const XgemmParams &p,
     float y = p.n_half ? x_silu(z) * up : x_activate(p.act, z);
     if (p.residual) y += x_load<DT>(p.residual, p.out_f32, row * p.ldo + j);
     x_store<DT>(p.out, p.out_f32, row * p.ldo + j, y);
+}
+
+/* four values, where every row of outputs, bias and residual starts at a multiple of four and is one of four long */
+template <int DT> __device__ __forceinline__ f32x4 x_load4(const void *p, int f32, int64_t i)
+{
+    if (f32) return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+    const u32x2 h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i);
+    return f32x4{zb_half_to_f32<DT>(h[0] & 0xffffu), zb_half_to_f32<DT>(h[0] >> 16), zb_half_to_f32<DT>(h[1] & 0xffffu), zb_half_to_f32<DT>(h[1] >> 16)};
+}
+template <int DT> __device__ __forceinline__ void x_store4(void *p, int f32, int64_t i, const f32x4 &v)
+{
+    if (f32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
+    else *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + i) = u32x2{zb_pack2_half<DT>(v[0], v[1]), zb_pack2_half<DT>(v[2], v[3])};
+}
+template <int DT> __device__ __forceinline__ void x_finish4(const XgemmParams &p, int expert, int64_t row, int j, f32x4 z, f32x4 up)
+{
+    if (p.bias) {
+        z += x_load4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + j);
+        if (p.n_half) up += x_load4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + p.n_half + j);
+    }
+    if (p.preact) {
+        x_store4<DT>(p.preact, 0, row * p.N + j, z);
+        if (p.n_half) x_store4<DT>(p.preact, 0, row * p.N + p.n_half + j, up);
+    }
+    f32x4 y;
+    for (int i = 0; i < 4; ++i) y[i] = p.n_half ? x_silu(z[i]) * up[i] : x_activate(p.act, z[i]);
+    if (p.residual) y += x_load4<DT>(p.residual, p.out_f32, row * p.ldo + j);
+    x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, y);
 }
 
 } // namespace

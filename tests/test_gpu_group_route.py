@@ -130,6 +130,35 @@ def test_far_logits_keep_their_order(buf):
     check(buf, torch.stack([up, -5 * up, torch.roll(up, 7) + 60]).contiguous(), 8)
 
 
+def test_rows_of_infinity_and_of_the_lowest_value(buf):
+    logits = torch.randn((8, 256), generator=gen(8))
+    logits[0], logits[1, ::2], logits[2, :200] = INF, INF, -INF
+    logits[2, 200:] = INF
+    logits[3], logits[4, 1::2] = torch.finfo(torch.float32).min, torch.finfo(torch.float32).min
+    logits[5, 9:], logits[6, :250] = torch.finfo(torch.float32).min, -1e9
+    check(buf, logits, 8)
+    check(buf, logits, 8, groups=8, kept=4)
+    check(buf, logits, 8, groups=8, kept=4, group_score="max")
+    check(buf, logits[3:].contiguous(), 8, score="softmax")
+    bias = torch.zeros((256,))
+    bias[::2] = INF
+    check(buf, logits, 8, bias=bias)
+    check(buf, logits, 8, bias=torch.full((256,), INF), groups=8, kept=4)
+
+
+def test_logits_so_small_that_their_scores_are_equal(buf):
+    """ties of 64-bit scores go to the lower index, whatever the logits"""
+    logits = torch.zeros((4, 64))
+    logits[0, 40:] = 1e-30
+    logits[1, 20] = 1e-25
+    logits[2] = torch.arange(64) * 1e-35
+    logits[3, 8:] = 1e-24
+    for group_score in ("top2", "max"):
+        check(buf, logits, 8, groups=8, kept=3, group_score=group_score)
+        check(buf, logits, 8, groups=8, kept=3, group_score=group_score, score="softmax")
+    check(buf, logits, 20)
+
+
 def test_an_empty_batch(buf):
     idx, w = buf.group_route(torch.empty((0, 16), device="cuda"), 4)
     assert idx.shape == w.shape == (0, 4)

@@ -14,7 +14,7 @@ constexpr int XSLOTS = 64;       /* workgroups an XCD runs at a time (32 CUs), f
  * Any sizes: operands pass through registers, sixteen bytes at a time from wherever they start (two bytes' alignment), the last
  * elements of a row or column one by one.
  */
-template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN>
+template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN, bool SHORT>
 __global__ void __launch_bounds__(WM * WN * 64)
 expert_gemm_any_kernel(XgemmParams p)
 {
@@ -65,29 +65,47 @@ expert_gemm_any_kernel(XgemmParams p)
         *end = c < TN / 2 ? p.n_half : p.N;
         return c < TN / 2 ? n0 + c : p.n_half + n0 + c - TN / 2;
     };
-    auto eight = [&](const uint16_t *at, int valid) __attribute__((always_inline)) -> u32x4 {
-        u32x4 v = {0, 0, 0, 0};
-        if (valid >= 8) return *reinterpret_cast<const loose_t *>(at);
-        for (int i = 0; i < valid; ++i) v[i >> 1] |= (uint32_t)at[i] << ((i & 1) * 16);
-        return v;
-    };
-    auto load_a = [&](int c, int k0) __attribute__((always_inline)) -> u32x4 {
-        if constexpr (REDUCE) {
-            const int k = k0 + c / (TM / 8), m = m0 + c % (TM / 8) * 8;
-            return k < k_end ? eight(p.a + (int64_t)k * p.lda + m, m_end - m) : u32x4{0, 0, 0, 0};
+    /*
+     * Eight elements from column `col` of a row: a piece that ends past `end` is taken from its last eight and shifted, so that all loads are alike
+     * and under way together (one by one, the last columns' tiles took twice as long as the others: 1021 x 1001 x 1531 in 64 x 64, with gelu, bias and residual, 27 us, 41).
+     */
+    struct Piece { u32x4 v; int away; };         /* elements to shift out; eight: nothing is left */
+    auto eight = [&](const uint16_t *row, int col, int end, bool there) __attribute__((always_inline)) -> Piece {
+        if constexpr (SHORT) {
+            u32x4 v = {0, 0, 0, 0};
+            for (int i = 0; there && i < 8 && col + i < end; ++i) v[i >> 1] |= (uint32_t)row[col + i] << ((i & 1) * 16);
+            return {v, 0};
         } else {
-            const int row = m0 + (c >> 3), k = k0 + (c & 7) * 8;
-            return row < m_end ? eight(p.a + (int64_t)row * p.lda + k, k_end - k) : u32x4{0, 0, 0, 0};
+            const int from = col < end - 8 ? col : end - 8, away = col - from;
+            return {*reinterpret_cast<const loose_t *>(row + from), !there || away > 8 ? 8 : away};
         }
     };
-    auto load_b = [&](int c, int k0) __attribute__((always_inline)) -> u32x4 {
+    auto shifted = [&](const Piece &c) __attribute__((always_inline)) -> u32x4 {
+        if (c.away == 0) return c.v;
+        const int bits = (c.away & 3) * 16;
+        uint64_t lo = (uint64_t)c.v[1] << 32 | c.v[0], hi = (uint64_t)c.v[3] << 32 | c.v[2];
+        if (c.away >= 4) { lo = hi; hi = 0; }
+        if (c.away >= 8) lo = 0;
+        if (bits) { lo = lo >> bits | hi << (64 - bits); hi >>= bits; }
+        return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
+    };
+    auto load_a = [&](int c, int k0) __attribute__((always_inline)) -> Piece {
+        if constexpr (REDUCE) {
+            const int k = k0 + c / (TM / 8), m = m0 + c % (TM / 8) * 8;
+            return eight(p.a + (int64_t)(k < k_end ? k : k_end - 1) * p.lda, m, m_end, k < k_end);
+        } else {
+            const int row = m0 + (c >> 3), k = k0 + (c & 7) * 8;
+            return eight(p.a + (int64_t)(row < m_end ? row : m_end - 1) * p.lda, k, k_end, row < m_end);
+        }
+    };
+    auto load_b = [&](int c, int k0) __attribute__((always_inline)) -> Piece {
         int end;
         if constexpr (REDUCE || B_TR) {
             const int k = k0 + c / (TN / 8), n = b_col(c % (TN / 8) * 8, &end);
-            return k < k_end ? eight(b + (int64_t)k * p.ldb + n, end - n) : u32x4{0, 0, 0, 0};
+            return eight(b + (int64_t)(k < k_end ? k : k_end - 1) * p.ldb, n, end, k < k_end);
         } else {
             const int n = b_col(c >> 3, &end), k = k0 + (c & 7) * 8;
-            return n < end ? eight(b + (int64_t)n * p.ldb + k, k_end - k) : u32x4{0, 0, 0, 0};
+            return eight(b + (int64_t)(n < end ? n : end - 1) * p.ldb, k, k_end, n < end);
         }
     };
 
@@ -102,30 +120,32 @@ expert_gemm_any_kernel(XgemmParams p)
     const uint32_t one2 = DT == ZDT_BF16 ? 0x3f803f80u : 0x3c003c00u;
     const u32x4 ones = {one2, one2, one2, one2};
 
-    u32x4 ra[AC], rb[B_CHUNKS];
-    auto fetch = [&](int k0) __attribute__((always_inline)) {
+    /* two steps' pieces are under way while a third is multiplied, where registers leave room for it and for a second workgroup */
+    constexpr int AHEAD = TM * TN > 64 * 128 ? 1 : 2;
+    Piece ra[AHEAD][AC], rb[AHEAD][B_CHUNKS];
+    const bool a_mine = A_CHUNKS > 0 || tid < TM * 8;
+    auto fetch = [&](Piece(&pa)[AC], Piece(&pb)[B_CHUNKS], int k0) __attribute__((always_inline)) {
 #pragma unroll
         for (int i = 0; i < AC; ++i)
-            if (A_CHUNKS > 0 || tid < TM * 8) ra[i] = load_a(tid + i * THREADS, k0);
+            if (a_mine) pa[i] = load_a(tid + i * THREADS, k0);
 #pragma unroll
-        for (int i = 0; i < B_CHUNKS; ++i) rb[i] = load_b(tid + i * THREADS, k0);
+        for (int i = 0; i < B_CHUNKS; ++i) pb[i] = load_b(tid + i * THREADS, k0);
     };
-    if (k_begin < k_end) fetch(k_begin);
-    for (int k0 = k_begin; k0 < k_end; k0 += XBK) {
+    auto step = [&](Piece(&pa)[AC], Piece(&pb)[B_CHUNKS], int k0) __attribute__((always_inline)) {
         __syncthreads();
 #pragma unroll
         for (int i = 0; i < AC; ++i)
-            if (A_CHUNKS > 0 || tid < TM * 8) {
+            if (a_mine) {
                 const int c = tid + i * THREADS;
-                *reinterpret_cast<u32x4 *>(lds_a + (REDUCE ? tr_at<TM>(c / (TM / 8), c % (TM / 8)) : kc_at(c >> 3, c & 7))) = ra[i];
+                *reinterpret_cast<u32x4 *>(lds_a + (REDUCE ? tr_at<TM>(c / (TM / 8), c % (TM / 8)) : kc_at(c >> 3, c & 7))) = shifted(pa[i]);
             }
 #pragma unroll
         for (int i = 0; i < B_CHUNKS; ++i) {
             const int c = tid + i * THREADS;
-            *reinterpret_cast<u32x4 *>(lds_b + (REDUCE || B_TR ? tr_at<TN>(c / (TN / 8), c % (TN / 8)) : kc_at(c >> 3, c & 7))) = rb[i];
+            *reinterpret_cast<u32x4 *>(lds_b + (REDUCE || B_TR ? tr_at<TN>(c / (TN / 8), c % (TN / 8)) : kc_at(c >> 3, c & 7))) = shifted(pb[i]);
         }
         __syncthreads();
-        if (k0 + XBK < k_end) fetch(k0 + XBK);
+        fetch(pa, pb, k0 + AHEAD * XBK);          /* past the end: the last pieces again, and none of them used */
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             u32x4 fa[MT];
@@ -145,6 +165,14 @@ expert_gemm_any_kernel(XgemmParams p)
                 for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = x_mfma<DT>(fb, fa[mt], acc[mt][nt]);
             }
         }
+    };
+    if (k_begin < k_end) {
+#pragma unroll
+        for (int i = 0; i < AHEAD; ++i) fetch(ra[i], rb[i], k_begin + i * XBK);
+        for (int k0 = k_begin; k0 < k_end; k0 += AHEAD * XBK)
+#pragma unroll
+            for (int i = 0; i < AHEAD; ++i)
+                if (k0 + i * XBK < k_end) step(ra[i], rb[i], k0 + i * XBK);
     }
 
     /* a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile */
@@ -238,33 +266,71 @@ expert_join_kernel(XgemmParams p)
 
 /*
  * The pre-activation's gradient: dz = dy act'(z), for swiglu of both halves; with no activation the rounding of a gradient in 32 bits.
- * A stream of the three tensors.
+ * A stream of the three tensors, V elements to a lane: 16384 x 7168 out of 32 bits 137 us at eight (5.1 TB/s), 174 one by one; gelu 201, 242.
  */
-template <int DT>
+template <int DT, int V>
 __global__ void __launch_bounds__(256)
 expert_slope_kernel(XgemmParams p, const void *__restrict__ dy, int dy_f32, const uint16_t *__restrict__ z, uint16_t *__restrict__ dz)
 {
-    const int cols = p.n_half ? p.n_half : p.N;
-    int rows = p.rows;
-    if (p.counts) {
-        rows = x_rows_of(p, p.experts - 1).end;
-    }
-    const int64_t n = (int64_t)rows * cols, step = (int64_t)gridDim.x * blockDim.x;
-    for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < n; i += step) {
-        const float d = x_load<DT>(dy, dy_f32, i);
-        if (p.act == ACT_SWIGLU) {
-            const int64_t row = i / cols, at = row * p.N + (i - row * cols);
-            const float g = zb_half_to_f32<DT>(z[at]), u = zb_half_to_f32<DT>(z[at + cols]);
-            dz[at] = (uint16_t)zb_f32_to_half<DT>(d * u * x_slope(ACT_SILU, g));
-            dz[at + cols] = (uint16_t)zb_f32_to_half<DT>(d * x_silu(g));
+    typedef uint16_t halves __attribute__((ext_vector_type(V)));
+    typedef float floats __attribute__((ext_vector_type(V), aligned(V * 4 < 16 ? 4 : 16)));
+    const int cols = (p.n_half ? p.n_half : p.N) / V, rows = p.counts ? x_rows_of(p, p.experts - 1).end : p.rows;
+    const int64_t n = (int64_t)rows * cols, first = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
+    const int step = gridDim.x * blockDim.x, step_rows = step / cols, step_cols = step - step_rows * cols;
+    int64_t row = first / cols;
+    int col = (int)(first - row * cols);
+    for (int64_t i = first; i < n; i += step) {
+        float d[V];
+        if (dy_f32) {
+            const floats v = reinterpret_cast<const floats *>(dy)[i];
+#pragma unroll
+            for (int k = 0; k < V; ++k) d[k] = v[k];
         } else {
-            const float s = p.act == ACT_NONE ? 1.0f : x_slope(p.act, zb_half_to_f32<DT>(z[i]));
-            dz[i] = (uint16_t)zb_f32_to_half<DT>(d * s);
+            const halves v = reinterpret_cast<const halves *>(dy)[i];
+#pragma unroll
+            for (int k = 0; k < V; ++k) d[k] = zb_half_to_f32<DT>(v[k]);
         }
+        if (p.act == ACT_SWIGLU) {
+            const int64_t at = row * 2 * cols + col;
+            const halves gs = reinterpret_cast<const halves *>(z)[at], us = reinterpret_cast<const halves *>(z)[at + cols];
+            halves dg, du;
+#pragma unroll
+            for (int k = 0; k < V; ++k) {
+                const float g = zb_half_to_f32<DT>(gs[k]), u = zb_half_to_f32<DT>(us[k]);
+                dg[k] = (uint16_t)zb_f32_to_half<DT>(d[k] * u * x_slope(ACT_SILU, g));
+                du[k] = (uint16_t)zb_f32_to_half<DT>(d[k] * x_silu(g));
+            }
+            reinterpret_cast<halves *>(dz)[at] = dg;
+            reinterpret_cast<halves *>(dz)[at + cols] = du;
+        } else {
+            halves v;
+            if (p.act == ACT_NONE) {
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] = (uint16_t)zb_f32_to_half<DT>(d[k]);
+            } else {
+                const halves zs = reinterpret_cast<const halves *>(z)[i];
+#pragma unroll
+                for (int k = 0; k < V; ++k) v[k] = (uint16_t)zb_f32_to_half<DT>(d[k] * x_slope(p.act, zb_half_to_f32<DT>(zs[k])));
+            }
+            reinterpret_cast<halves *>(dz)[i] = v;
+        }
+        row += step_rows;
+        col += step_cols;
+        if (col >= cols) { col -= cols; ++row; }
     }
 }
 
-template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN>
+template <int DT> void launch_slope(const XgemmParams &p, const void *dy, int dy_f32, const uint16_t *z, uint16_t *dz, hipStream_t st)
+{
+    const int cols = p.n_half ? p.n_half : p.N;
+    const bool wide = cols % 8 == 0;             /* the tensors themselves are aligned */
+    const int64_t groups = ((int64_t)p.rows * cols / (wide ? 8 : 1) + 255) / 256;
+    const dim3 grid((unsigned)(groups < 4096 ? groups : 4096));
+    if (wide) zb_launch(expert_slope_kernel<DT, 8>, grid, dim3(256), 0, st, p, dy, dy_f32, z, dz);
+    else zb_launch(expert_slope_kernel<DT, 1>, grid, dim3(256), 0, st, p, dy, dy_f32, z, dz);
+}
+
+template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN, bool SHORT = false>
 void launch_any(const XgemmParams &p, hipStream_t st)
 {
     const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN;
@@ -278,7 +344,7 @@ void launch_any(const XgemmParams &p, hipStream_t st)
         blocks = (most < p.rows ? most : p.rows) * n_tiles;
         blocks = (blocks + 7) / 8 * 8;
     }
-    zb_launch(expert_gemm_any_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN>, dim3((unsigned)blocks, (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
+    zb_launch(expert_gemm_any_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN, SHORT>, dim3((unsigned)blocks, (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
 }
 
 /* workgroups of a product in tiles of TM x TN: for rows sorted by expert as many as there can be tiles */
@@ -316,7 +382,7 @@ template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStr
 inline bool rows_are_aligned(const XgemmParams &p) { return p.lda % 8 == 0 && p.ldb % 8 == 0 && p.ldo % 8 == 0 && p.N % 8 == 0 && p.n_half % 8 == 0; }
 
 /* how a product is cut: the tiles, and the parts along k whose sums a second launch adds up */
-enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16 };
+enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT };
 struct Plan {
     Cut cut;
     int splits;
@@ -337,7 +403,8 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
     struct Kind { Cut cut; int tm, tn, at_once; double alone, full; };
     static const Kind kinds[] = {{CUT_WIDE, 256, 256, 1, 1.5, 1.5}, {CUT_128, 128, 128, 1, 0.57, 0.57}, {CUT_64_128, 64, 128, 2, 0.55, 0.75},
                                  {CUT_64, 64, 64, 2, 0.4, 0.45}, {CUT_32, 32, 128, 2, 0.35, 0.5}, {CUT_16, 16, 64, 2, 0.2, 0.27}};
-    static const Kind any[] = {{CUT_ANY, 128, 128, 2, 1.2, 1.6}, {CUT_ANY_64, 64, 64, 4, 0.7, 1.0}, {CUT_ANY_16, 16, 128, 4, 0.6, 0.9}};
+    static const Kind any[] = {{CUT_ANY, 128, 128, 2, 1.8, 2.2}, {CUT_ANY_64, 64, 64, 4, 0.75, 1.6}, {CUT_ANY_16, 16, 128, 4, 0.8, 1.8}};
+    if ((reduce ? p.M : p.K) < 8 || (p.n_half ? p.n_half : p.N) < 8) return {CUT_SHORT, 1, 0};
     const bool aligned = rows_are_aligned(p);
     const Kind *list = aligned ? kinds : any;
     const int count = aligned ? 6 : 3;
@@ -360,7 +427,8 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
         for (int splits = 1; splits <= 8; splits *= 2) {
             if (splits > 1 && (p.experts > 1 || k.cut == CUT_WIDE || steps / splits < 4 || tiles * splits > 512)) break;
             const double each = tiles * splits, per_round = 256.0 * k.at_once;
-            double us = (each <= 256 ? k.alone : k.full * ceil(each / per_round)) * ceil(steps / splits);
+            const double beside = each < per_round ? ceil(each / 256.0) - 1.0 : k.at_once - 1.0;       /* that share a CU with one */
+            double us = (k.at_once == 1 ? k.full : k.alone + (k.full - k.alone) * fmax(beside, 0.0) / (k.at_once - 1)) * ceil(each / per_round) * ceil(steps / splits);
             if (k.cut == CUT_WIDE && !reduce && per_expert <= 128) us *= 0.6;      /* tiles without a second half */
             /* an epilogue of stores in every round, which takes no time beside the next tile's steps in the wide kernel */
             if (reduce) us += ceil(each / per_round) * (k.cut == CUT_WIDE ? 1.0 : 8.0);
@@ -399,6 +467,7 @@ template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, voi
         case CUT_64_128: launch_direct<DT, REDUCE, B_TR, 64, 128, 2, 2, 3>(p, st); break;
         case CUT_64: launch_direct<DT, REDUCE, B_TR, 64, 64, 2, 2, 4>(p, st); break;
         case CUT_ANY: launch_any<DT, REDUCE, B_TR, 128, 128, 2, 2>(p, st); break;
+        case CUT_SHORT: launch_any<DT, REDUCE, B_TR, 64, 64, 2, 2, true>(p, st); break;
         case CUT_ANY_64: launch_any<DT, REDUCE, B_TR, 64, 64, 2, 2>(p, st); break;
         default:
             if constexpr (!REDUCE) {
@@ -535,10 +604,8 @@ extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t 
         p.N = (int)d->n;
         p.act = d->activation;
         p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
-        int64_t blocks = (d->rows * (p.n_half ? p.n_half : p.N) + 1023) / 1024;
-        blocks = blocks < 2048 ? blocks : 2048;
-        if (d->dtype == ZDT_BF16) zb_launch(expert_slope_kernel<ZDT_BF16>, dim3((unsigned)blocks), dim3(256), 0, st, p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact);
-        else zb_launch(expert_slope_kernel<ZDT_FP16>, dim3((unsigned)blocks), dim3(256), 0, st, p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact);
+        if (d->dtype == ZDT_BF16) launch_slope<ZDT_BF16>(p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact, st);
+        else launch_slope<ZDT_FP16>(p, grad, grad_is_f32, (const uint16_t *)preact, (uint16_t *)grad_preact, st);
         dz = (const uint16_t *)grad_preact;
     }
     if (grad_x && d->rows > 0) {

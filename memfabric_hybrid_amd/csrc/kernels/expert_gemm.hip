@@ -4,11 +4,10 @@
  */
 #include <cmath>
 
+#include "zbal_expert_rows.h"
 #include "zbal_expert_wide.h"
 
 namespace {
-
-constexpr int XSLOTS = 64;       /* workgroups an XCD runs at a time (32 CUs), for the tile order */
 
 /*
  * Any sizes: operands pass through registers, sixteen bytes at a time from wherever they start (two bytes' alignment), the last
@@ -347,20 +346,37 @@ void launch_any(const XgemmParams &p, hipStream_t st)
     zb_launch(expert_gemm_any_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN, SHORT>, dim3((unsigned)blocks, (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
 }
 
-/* workgroups of a product in tiles of TM x TN: for rows sorted by expert as many as there can be tiles */
+/* workgroups of a product of rows sorted by expert: as many as there can be tiles */
+template <int TM> unsigned tiles_of_cols(const XgemmParams &p, int tile_cols)
+{
+    const int cols = p.n_half ? p.n_half : p.N;
+    const int64_t n_tiles = (cols + tile_cols - 1) / tile_cols, most = p.rows / TM + p.experts;    /* every expert may end with a tile that is not full */
+    return (unsigned)(((most < p.rows ? most : p.rows) * n_tiles + 7) / 8 * 8);
+}
+
 template <bool REDUCE, int TM, int TN> unsigned tiles_of(const XgemmParams &p)
 {
-    const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN;
-    const int64_t n_tiles = (cols + tile_cols - 1) / tile_cols;
-    if (REDUCE) return (unsigned)((p.experts * ((p.M + TM - 1) / TM) * n_tiles + 7) / 8 * 8);
-    const int64_t most = p.rows / TM + p.experts;          /* every expert may end with a tile that is not full */
-    return (unsigned)(((most < p.rows ? most : p.rows) * n_tiles + 7) / 8 * 8);
+    if (REDUCE) return (unsigned)(((int64_t)p.experts * ((p.M + TM - 1) / TM) * ((p.N + TN - 1) / TN) + 7) / 8 * 8);
+    return tiles_of_cols<TM>(p, p.n_half ? TN / 2 : TN);
 }
 
 template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN, int STAGES>
 void launch_direct(const XgemmParams &p, hipStream_t st)
 {
     zb_launch(expert_gemm_kernel<DT, REDUCE, B_TR, TM, TN, WM, WN, STAGES>, dim3(tiles_of<REDUCE, TM, TN>(p), (unsigned)p.splits), dim3(WM * WN * 64), 0, st, p);
+}
+
+template <int DT> void launch_rows(const XgemmParams &p, hipStream_t st)
+{
+    /* eight waves where four have more than one batch of loads */
+    const dim3 grid(tiles_of_cols<16>(p, 16)), four(256), eight(512);
+    if (p.n_half) {
+        if (p.K > 1024) zb_launch(expert_gemm_rows_kernel<DT, 2, 8>, grid, eight, 0, st, p);
+        else zb_launch(expert_gemm_rows_kernel<DT, 2, 4>, grid, four, 0, st, p);
+    } else {
+        if (p.K > 2048) zb_launch(expert_gemm_rows_kernel<DT, 1, 8>, grid, eight, 0, st, p);
+        else zb_launch(expert_gemm_rows_kernel<DT, 1, 4>, grid, four, 0, st, p);
+    }
 }
 
 template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStream_t st)
@@ -382,7 +398,7 @@ template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStr
 inline bool rows_are_aligned(const XgemmParams &p) { return p.lda % 8 == 0 && p.ldb % 8 == 0 && p.ldo % 8 == 0 && p.N % 8 == 0 && p.n_half % 8 == 0; }
 
 /* how a product is cut: the tiles, and the parts along k whose sums a second launch adds up */
-enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT };
+enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT, CUT_ROWS };
 struct Plan {
     Cut cut;
     int splits;
@@ -402,12 +418,13 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
 {
     struct Kind { Cut cut; int tm, tn, at_once; double alone, full; };
     static const Kind kinds[] = {{CUT_WIDE, 256, 256, 1, 1.5, 1.5}, {CUT_128, 128, 128, 1, 0.57, 0.57}, {CUT_64_128, 64, 128, 2, 0.55, 0.75},
-                                 {CUT_64, 64, 64, 2, 0.4, 0.45}, {CUT_32, 32, 128, 2, 0.35, 0.5}, {CUT_16, 16, 64, 2, 0.2, 0.27}};
+                                 {CUT_64, 64, 64, 2, 0.4, 0.45}, {CUT_32, 32, 128, 2, 0.35, 0.5}, {CUT_16, 16, 64, 2, 0.2, 0.27},
+                                 {CUT_ROWS, 16, 16, 4, 0.1, 0.15}};
     static const Kind any[] = {{CUT_ANY, 128, 128, 2, 1.8, 2.2}, {CUT_ANY_64, 64, 64, 4, 0.75, 1.6}, {CUT_ANY_16, 16, 128, 4, 0.8, 1.8}};
     if ((reduce ? p.M : p.K) < 8 || (p.n_half ? p.n_half : p.N) < 8) return {CUT_SHORT, 1, 0};
     const bool aligned = rows_are_aligned(p);
     const Kind *list = aligned ? kinds : any;
-    const int count = aligned ? 6 : 3;
+    const int count = !aligned ? 3 : (b_cols ? 6 : 7);
     const double steps = ((reduce ? (double)p.rows / p.experts : p.K) + XBK - 1) / XBK, per_expert = (double)p.rows / p.experts;
     const double reached = p.rows < p.experts ? p.rows : p.experts;
     const int cols = p.n_half ? p.n_half : p.N, rows = reduce ? p.M : p.rows;
@@ -416,7 +433,7 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
     for (int i = 0; i < count; ++i) {
         const Kind &k = list[i];
         if (reduce && k.tm < 64) continue;
-        const int tile_cols = p.n_half ? k.tn / 2 : k.tn;
+        const int tile_cols = p.n_half && k.cut != CUT_ROWS ? k.tn / 2 : k.tn;
         const double n_tiles = (cols + tile_cols - 1) / tile_cols;
         double m_tiles = reduce ? (double)p.experts * ((p.M + k.tm - 1) / k.tm) : (p.rows + k.tm - 1) / k.tm;
         if (!reduce && p.experts > 1) {      /* every expert ends with half a tile, on average */
@@ -425,7 +442,7 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
         }
         const double tiles = m_tiles * n_tiles;
         for (int splits = 1; splits <= 8; splits *= 2) {
-            if (splits > 1 && (p.experts > 1 || k.cut == CUT_WIDE || steps / splits < 4 || tiles * splits > 512)) break;
+            if (splits > 1 && (p.experts > 1 || k.cut == CUT_WIDE || k.cut == CUT_ROWS || steps / splits < 4 || tiles * splits > 512)) break;
             const double each = tiles * splits, per_round = 256.0 * k.at_once;
             const double beside = each < per_round ? ceil(each / 256.0) - 1.0 : k.at_once - 1.0;       /* that share a CU with one */
             double us = (k.at_once == 1 ? k.full : k.alone + (k.full - k.alone) * fmax(beside, 0.0) / (k.at_once - 1)) * ceil(each / per_round) * ceil(steps / splits);
@@ -469,6 +486,9 @@ template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, voi
         case CUT_ANY: launch_any<DT, REDUCE, B_TR, 128, 128, 2, 2>(p, st); break;
         case CUT_SHORT: launch_any<DT, REDUCE, B_TR, 64, 64, 2, 2, true>(p, st); break;
         case CUT_ANY_64: launch_any<DT, REDUCE, B_TR, 64, 64, 2, 2>(p, st); break;
+        case CUT_ROWS:
+            if constexpr (!REDUCE && !B_TR) launch_rows<DT>(p, st);
+            break;
         default:
             if constexpr (!REDUCE) {
                 if (plan.cut == CUT_32) launch_direct<DT, REDUCE, B_TR, 32, 128, 2, 2, 4>(p, st);

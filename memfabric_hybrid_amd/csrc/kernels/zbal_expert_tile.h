@@ -19,6 +19,7 @@
 namespace {
 
 constexpr int XBK = 64;          /* k per step */
+constexpr int XSLOTS = 64;       /* workgroups an XCD runs at a time (32 CUs), for the tile order */
 
 enum { ACT_NONE = 0, ACT_RELU, ACT_SILU, ACT_GELU, ACT_GELU_TANH, ACT_SWIGLU };
 
@@ -154,6 +155,19 @@ template <int TM> __device__ __forceinline__ XTile x_locate(const XgemmParams &p
 {
     const int lane = threadIdx.x & 63;
     auto tiles_of = [&](uint32_t before, uint32_t incl) { const XSpan s = x_span(p, before, incl); return (uint32_t)(s.end - s.begin + TM - 1) / TM; };
+    /* tile r of an expert's */
+    auto place = [&](int expert, int begin, int end, int mt, int r) __attribute__((always_inline)) -> XTile {
+        int group = slots / mt;
+        group = group < 1 ? 1 : (group > 8 ? 8 : group);
+        const int per = mt * group, g = r / per, in = r - g * per, from = begin + in % mt * TM;
+        return {expert, from, end - from > TM ? from + TM : end, g * group + in / mt};
+    };
+    if (p.experts == 1) {
+        const XSpan s = x_rows_of(p, 0);
+        const int mt = (s.end - s.begin + TM - 1) / TM, total = mt * n_tiles, chunk = (total + 7) / 8, logical = (id & 7) * chunk + (id >> 3);
+        if ((id >> 3) >= chunk || logical >= total) return {-1, 0, 0, 0};
+        return place(0, s.begin, s.end, mt, logical);
+    }
     uint32_t run = 0, tiles = 0;
     for (int base = 0; base < p.experts; base += 64) {
         const uint32_t c = base + lane < p.experts ? x_count(p, base + lane) : 0;
@@ -162,8 +176,7 @@ template <int TM> __device__ __forceinline__ XTile x_locate(const XgemmParams &p
         run = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
     const int total = (int)tiles * n_tiles, chunk = (total + 7) / 8, logical = (id & 7) * chunk + (id >> 3);
-    XTile t = {-1, 0, 0, 0};
-    if ((id >> 3) >= chunk || logical >= total) return t;
+    if ((id >> 3) >= chunk || logical >= total) return {-1, 0, 0, 0};
     const int q = logical / n_tiles;                         /* a row tile of the expert wanted */
     run = 0;
     uint32_t first = 0;
@@ -178,20 +191,12 @@ template <int TM> __device__ __forceinline__ XTile x_locate(const XgemmParams &p
             const int first_e = __builtin_amdgcn_readlane((int)mt_incl, l) - mt_e;
             const XSpan s = x_span(p, incl - c, incl);
             const int begin = __builtin_amdgcn_readlane(s.begin, l), end = __builtin_amdgcn_readlane(s.end, l);
-            const int r = logical - first_e * n_tiles;
-            int group = slots / mt_e;
-            group = group < 1 ? 1 : (group > 8 ? 8 : group);
-            const int per = mt_e * group, g = r / per, in = r - g * per;
-            t.expert = base + l;
-            t.row_begin = begin + in % mt_e * TM;
-            t.row_end = end - t.row_begin > TM ? t.row_begin + TM : end;
-            t.n_tile = g * group + in / mt_e;
-            return t;
+            return place(base + l, begin, end, mt_e, logical - first_e * n_tiles);
         }
         first = (uint32_t)__builtin_amdgcn_readlane((int)mt_incl, 63);
         run = (uint32_t)__builtin_amdgcn_readlane((int)incl, 63);
     }
-    return t;
+    return {-1, 0, 0, 0};
 }
 
 /* ---- activations --------------------------------------------------------------------------------------------------- */

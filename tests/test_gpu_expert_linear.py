@@ -131,6 +131,20 @@ def test_grouped(buf, rows, E, K, N, act, transposed):
     forward_case(buf, rows, E, K, N, torch.float16, act, transposed=transposed, residual=True)
 
 
+# sizes that are cut into every kind of tiles and parts, for many workgroups a CU; the last rows, columns and k of each are ragged
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("rows,E,K,N", [(8200, 1, 136, 4104), (4033, 64, 200, 4104), (1280, 20, 136, 2056), (1200, 40, 72, 1928), (900, 3, 264, 1160),
+                                        (4100, 1, 2056, 264), (70, 1, 2120, 520), (2100, 1, 4097, 250), (1030, 2, 266, 2050), (200, 60, 130, 1026), (5000, 3, 131, 1029),
+                                        (1, 1, 4104, 2056), (1, 1, 1104, 4104), (17, 2, 2056, 4104), (5, 3, 1032, 72)])
+def test_every_cut(buf, rows, E, K, N, transposed):
+    counts = "all" if E == 1 else None
+    forward_case(buf, rows, E, K, N, torch.bfloat16, transposed=transposed, counts=counts, out_dtype=torch.float32)
+    forward_case(buf, rows, E, K, N, torch.float16, "silu", bias=torch.float16, residual=True, preact=True, transposed=transposed, counts=counts, seed=1)
+    if N % 2 == 0:
+        forward_case(buf, rows, E, K, N, torch.bfloat16, "swiglu", transposed=transposed, counts=counts, seed=2)
+        forward_case(buf, rows, E, K, N, torch.float16, "swiglu", bias=torch.float32, residual=True, preact=True, transposed=transposed, counts=counts, seed=3)
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 0, 0], [0, 0, 0, 50], [50, 0, 0, 0], [10, 10, 10, 10], [-5, 20, -(1 << 31), 10], [30, 1 << 30, 7, (1 << 31) - 1],
                                     [1, 47, 1, 1], [20, 20, 20, 20]])
 @pytest.mark.parametrize("N", [128, 130])
@@ -214,6 +228,16 @@ def test_gradients(buf, rows, E, K, N, transposed):
     backward_case(buf, rows, E, K, N, torch.float16, transposed=transposed, wgrad=torch.float32)
 
 
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("rows,E,K,N", [(2049, 1, 1544, 1536), (1030, 1, 1216, 3336), (1030, 1, 3336, 1216), (8201, 1, 256, 264), (8200, 1, 250, 129), (3000, 3, 1040, 1288), (2500, 3, 1031, 1290),
+                                        (2049, 20, 520, 776), (129, 1, 2056, 4104)])
+def test_gradients_of_every_cut(buf, rows, E, K, N, transposed):
+    counts = "all" if E == 1 else None
+    backward_case(buf, rows, E, K, N, torch.bfloat16, transposed=transposed, counts=counts)
+    backward_case(buf, rows, E, K, N, torch.float16, "silu", transposed=transposed, counts=counts, wgrad=torch.float32, grad_dtype=torch.float32)
+    backward_case(buf, rows, E, K, N, torch.bfloat16, transposed=transposed, counts=counts, bias=False, seed=1)
+
+
 @pytest.mark.parametrize("act", ACTIVATIONS)
 @pytest.mark.parametrize("rows,E,K,N", [(7, 1, 64, 40), (130, 3, 200, 66), (600, 4, 256, 512)])
 def test_gradients_of_activations(buf, rows, E, K, N, act):
@@ -264,7 +288,8 @@ def test_gradients_against_differences(buf):
 
 # ---- calls ---------------------------------------------------------------------------------------------------------------
 
-@pytest.mark.parametrize("rows,E,K,N", [(4, 1, 2048, 512), (40, 8, 256, 512), (2000, 4, 512, 520), (500, 1, 4096, 128)])
+@pytest.mark.parametrize("rows,E,K,N", [(4, 1, 2048, 512), (40, 8, 256, 512), (2000, 4, 512, 520), (500, 1, 4096, 128), (8200, 1, 256, 264),
+                                        (1000, 1, 1001, 333), (9000, 8, 136, 2048)])
 def test_the_same_every_time_and_captured(buf, rows, E, K, N):
     g, x, w, counts = make(rows, E, K, N, torch.bfloat16, 5)
     ct = torch.tensor(counts, dtype=torch.int32, device="cuda")

@@ -135,7 +135,7 @@ def test_grouped(buf, rows, E, K, N, act, transposed):
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("rows,E,K,N", [(8200, 1, 136, 4104), (4033, 64, 200, 4104), (1280, 20, 136, 2056), (1200, 40, 72, 1928), (900, 3, 264, 1160),
                                         (4100, 1, 2056, 264), (70, 1, 2120, 520), (2100, 1, 4097, 250), (1030, 2, 266, 2050), (200, 60, 130, 1026), (5000, 3, 131, 1029),
-                                        (1, 1, 4104, 2056), (1, 1, 1104, 4104), (17, 2, 2056, 4104), (5, 3, 1032, 72)])
+                                        (1, 1, 4104, 2056), (1, 1, 1104, 4104), (17, 2, 2056, 4104), (5, 3, 1032, 72), (3, 5, 1048, 80)])
 def test_every_cut(buf, rows, E, K, N, transposed):
     counts = "all" if E == 1 else None
     forward_case(buf, rows, E, K, N, torch.bfloat16, transposed=transposed, counts=counts, out_dtype=torch.float32)
@@ -230,7 +230,7 @@ def test_gradients(buf, rows, E, K, N, transposed):
 
 @pytest.mark.parametrize("transposed", [False, True])
 @pytest.mark.parametrize("rows,E,K,N", [(2049, 1, 1544, 1536), (1030, 1, 1216, 3336), (1030, 1, 3336, 1216), (8201, 1, 256, 264), (8200, 1, 250, 129), (3000, 3, 1040, 1288), (2500, 3, 1031, 1290),
-                                        (2049, 20, 520, 776), (129, 1, 2056, 4104)])
+                                        (2049, 20, 520, 776), (129, 1, 2056, 4104), (4941, 8, 8, 5640)])
 def test_gradients_of_every_cut(buf, rows, E, K, N, transposed):
     counts = "all" if E == 1 else None
     backward_case(buf, rows, E, K, N, torch.bfloat16, transposed=transposed, counts=counts)

@@ -417,6 +417,8 @@ typedef struct {
     const float *bias;
     int64_t tokens, experts, topk, groups, kept_groups;
 } zbalhip_group_route_t;
+/* of a call that has a wave, or a workgroup, for a token: a launch is less than 2^32 lanes */
+#define ZBALHIP_ROUTE_MAX_TOKENS ((1 << 24) - 1)
 ZBALHIP_API int32_t zbalhip_group_route(const zbalhip_group_route_t *route, void *topk_idx, int32_t idx_is_i64, float *topk_w, void *stream);
 ZBALHIP_API int32_t zbalhip_group_route_backward(const zbalhip_group_route_t *route, const float *grad_w, const void *topk_idx,
                                      int32_t idx_is_i64, void *grad_logits, void *stream);

@@ -95,7 +95,7 @@ extern "C" int32_t zbalhip_combine_backward(const void *grad, const void *y, int
                                             void *stream)
 {
     if (dtype != ZDT_BF16 && dtype != ZDT_FP16) return ZBALHIP_INVALID;
-    if (tokens < 0 || tokens > 0x7fffffff || hidden <= 0 || hidden % 8 != 0 || hidden > 0x7fffffff || topk <= 0 || topk > kMaxTopk ||
+    if (tokens < 0 || tokens > ZBALHIP_ROUTE_MAX_TOKENS || hidden <= 0 || hidden % 8 != 0 || hidden > 0x7fffffff || topk <= 0 || topk > kMaxTopk ||
         experts <= 0 || experts > 0x7fffffff || y_rows < 0)
         return ZBALHIP_INVALID;
     if (tokens == 0) return ZBALHIP_OK;

@@ -529,7 +529,7 @@ template <int LANES> void launch_backward(const RouteBackParams &p, bool vec, hi
 
 extern "C" int32_t zbalhip_group_route(const zbalhip_group_route_t *d, void *topk_idx, int32_t idx_is_i64, float *topk_w, void *stream)
 {
-    if (!d || d->tokens < 0 || d->tokens > 0x7fffffff || d->experts <= 0 || d->experts > kMaxExperts || d->topk <= 0 || d->topk > kMaxTopk ||
+    if (!d || d->tokens < 0 || d->tokens > ZBALHIP_ROUTE_MAX_TOKENS || d->experts <= 0 || d->experts > kMaxExperts || d->topk <= 0 || d->topk > kMaxTopk ||
         d->topk > d->experts || d->groups <= 0 || d->groups > kMaxGroups || d->experts % d->groups != 0 || d->kept_groups <= 0 ||
         d->kept_groups > d->groups || d->topk > d->kept_groups * (d->experts / d->groups) || (d->score & ~1) || (d->group_score & ~1))
         return ZBALHIP_INVALID;
@@ -554,7 +554,7 @@ extern "C" int32_t zbalhip_group_route(const zbalhip_group_route_t *d, void *top
 extern "C" int32_t zbalhip_group_route_backward(const zbalhip_group_route_t *d, const float *grad_w, const void *topk_idx,
                                                 int32_t idx_is_i64, void *grad_logits, void *stream)
 {
-    if (!d || d->tokens < 0 || d->tokens > 0x7fffffff || d->experts <= 0 || d->experts > kMaxExperts || d->topk <= 0 || d->topk > kMaxTopk ||
+    if (!d || d->tokens < 0 || d->tokens > ZBALHIP_ROUTE_MAX_TOKENS || d->experts <= 0 || d->experts > kMaxExperts || d->topk <= 0 || d->topk > kMaxTopk ||
         (d->score & ~1))
         return ZBALHIP_INVALID;
     if (d->dtype != ZDT_FP32 && d->dtype != ZDT_BF16 && d->dtype != ZDT_FP16) return ZBALHIP_INVALID;

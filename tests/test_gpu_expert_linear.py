@@ -256,6 +256,17 @@ def test_gradient_counts(buf, counts, K, N):
             assert (gw[e] == 0).all() and (gb[e] == 0).all()
 
 
+def test_the_most_experts(buf):
+    """tiles of a kind that holds every expert's place"""
+    for transposed in (False, True):
+        forward_case(buf, 20000, 1024, 264, 256, torch.bfloat16, transposed=transposed)
+        backward_case(buf, 20000, 1024, 264, 256, torch.bfloat16, transposed=transposed)
+    counts = [0] * 1024
+    counts[1023] = 300
+    forward_case(buf, 300, 1024, 264, 256, torch.float16, "silu", bias=torch.float32, counts=counts)
+    backward_case(buf, 300, 1024, 264, 256, torch.float16, "silu", counts=counts)
+
+
 def test_no_rows(buf):
     w = torch.randn((2, 64, 128), device="cuda").to(torch.bfloat16)
     x, ct = torch.empty((0, 64), device="cuda", dtype=torch.bfloat16), torch.zeros((2,), dtype=torch.int32, device="cuda")

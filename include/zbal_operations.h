@@ -246,7 +246,8 @@ int32_t zbal_moe_weight_prepack(const zbal_tensor_info_t *src, const zbal_tensor
  * ([E] fp32, may be null). Of groupNum groups of consecutive experts the topkGroupNum best are kept, and the topkNum largest
  * choices in those are the picks, in falling order, ties to the lower index. weight = scale * s, over the sum of the picks' s if
  * renormalize (0 where that is 0). An expert is no pick if its logit is minus infinity or its choice is that or no number; slots that are left
- * get the id -1 and the weight 0. topkIndex, topkWeight: as in zbal_moe_topk_route. Up to 1024 experts, 64 groups, 32 picks.
+ * get the id -1 and the weight 0. topkIndex, topkWeight: as in zbal_moe_topk_route. Up to 1024 experts, 64 groups, 32 picks; fewer than
+ * 2^24 tokens.
  */
 int32_t zbal_moe_group_route(const zbal_tensor_info_t *logits, const zbal_tensor_info_t *bias, int64_t topkNum,
                              int64_t groupNum, int64_t topkGroupNum, zbal_score_t score, zbal_group_score_t groupScore,
@@ -300,7 +301,7 @@ int64_t zbal_moe_expert_linear_workspace_size(int64_t rows, int64_t k, int64_t n
 /*
  * extension: the gradient of zbal_combine_normal on a group of one rank. grad [T, H], srcTokens [rows, H] and the others as the combine took
  * them -> gradTokens [rows, H]: the row of a pick gets its weight times its token's gradient (rows of no pick are left as they are),
- * gradWeight [T, K] fp32: the product of the two rows, 0 for a pick that went nowhere.
+ * gradWeight [T, K] fp32: the product of the two rows, 0 for a pick that went nowhere. Fewer than 2^24 tokens.
  */
 int32_t zbal_combine_normal_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *srcTokens,
                                      const zbal_tensor_info_t *srcTokensPerEp, const zbal_tensor_info_t *topKWeight,

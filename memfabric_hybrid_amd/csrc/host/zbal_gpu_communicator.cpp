@@ -916,6 +916,7 @@ public:
         const char *op = "GroupRoute";
         ZBAL_VALIDATE_RETURN(logits->dim == 2, op << " failed as logits must be [tokens, experts]", Z_INVALID_PARAM);
         const int64_t T = logits->shape[0], E = logits->shape[1];
+        ZBAL_VALIDATE_RETURN(T <= ZBALHIP_ROUTE_MAX_TOKENS, op << " failed as tokens " << T << " exceed " << ZBALHIP_ROUTE_MAX_TOKENS, Z_INVALID_PARAM);
         ZBAL_VALIDATE_RETURN(E > 0 && E <= 1024 && groupNum <= 64 && E % groupNum == 0,
                              op << " failed as " << E << " experts do not make " << groupNum << " groups (up to 1024, up to 64)", Z_INVALID_PARAM);
         ZBAL_VALIDATE_RETURN(topkNum <= 32 && topkNum <= topkGroupNum * (E / groupNum),
@@ -939,6 +940,7 @@ public:
         const char *op = "GroupRouteBackward";
         ZBAL_VALIDATE_RETURN(logits->dim == 2, op << " failed as logits must be [tokens, experts]", Z_INVALID_PARAM);
         const int64_t T = logits->shape[0], E = logits->shape[1];
+        ZBAL_VALIDATE_RETURN(T <= ZBALHIP_ROUTE_MAX_TOKENS, op << " failed as tokens " << T << " exceed " << ZBALHIP_ROUTE_MAX_TOKENS, Z_INVALID_PARAM);
         ZBAL_VALIDATE_RETURN(topkIndex->dim == 2 && topkIndex->shape[0] == T, op << " failed as topkIndex must be [tokens, topk]", Z_INVALID_PARAM);
         const int64_t K = topkIndex->shape[1];
         ZBAL_VALIDATE_RETURN(E > 0 && E <= 1024 && K > 0 && K <= 32, op << " failed as experts " << E << " / topk " << K << " are out of range",
@@ -1089,6 +1091,7 @@ public:
         ZBAL_VALIDATE_RETURN(info_.groupSize == 1, op << " failed as it runs on a group of one rank", Z_INVALID_PARAM);
         int64_t T = 0, H = 0;
         if (!TokensShape(op, grad, &T, &H)) return Z_INVALID_PARAM;
+        ZBAL_VALIDATE_RETURN(T <= ZBALHIP_ROUTE_MAX_TOKENS, op << " failed as tokens " << T << " exceed " << ZBALHIP_ROUTE_MAX_TOKENS, Z_INVALID_PARAM);
         ZBAL_VALIDATE_RETURN(topkIndex->dim == 2 && topkIndex->shape[0] == T, op << " failed as topkIndex must be [tokens, topk]", Z_INVALID_PARAM);
         const int64_t K = topkIndex->shape[1];
         ZBAL_VALIDATE_RETURN(K > 0 && K <= 32, op << " failed as topk " << K << " is out of range", Z_INVALID_PARAM);

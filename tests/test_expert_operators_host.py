@@ -34,7 +34,7 @@ def route(**kw):
     return capi.GroupRoute(**d)
 
 
-@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(tokens=1 << 31), dict(experts=0), dict(experts=1032), dict(topk=0), dict(topk=33), dict(groups=0),
+@pytest.mark.parametrize("kw", [dict(tokens=-1), dict(tokens=1 << 31), dict(tokens=1 << 24), dict(experts=0), dict(experts=1032), dict(topk=0), dict(topk=33), dict(groups=0),
                                 dict(groups=5), dict(groups=128, experts=1024), dict(kept_groups=0), dict(kept_groups=9), dict(topk=9, kept_groups=1),
                                 dict(score=2), dict(score=-1), dict(group_score=2), dict(dtype=capi.DT_INT32), dict(logits=None)])
 def test_route_refusals(lib, kw):
@@ -102,7 +102,7 @@ def test_workspace_sizes(lib):
         assert f(16, 64, 63, 1, 5, capi.DT_BF16, capi.WEIGHT_FORMAT_ND, backward) == -1
 
 
-@pytest.mark.parametrize("kw", [dict(dtype=capi.DT_FP32), dict(tokens=-1), dict(hidden=0), dict(hidden=20), dict(topk=0), dict(topk=33), dict(experts=0), dict(rows=-1),
+@pytest.mark.parametrize("kw", [dict(dtype=capi.DT_FP32), dict(tokens=-1), dict(tokens=1 << 24), dict(hidden=0), dict(hidden=20), dict(topk=0), dict(topk=33), dict(experts=0), dict(rows=-1),
                                 dict(grad=None), dict(y=None), dict(out=None)])
 def test_combine_refusals(lib, kw):
     d = dict(grad=4096, y=4096, rows=8, dtype=capi.DT_BF16, tokens=4, hidden=64, topk=2, experts=8, out=4096)

@@ -204,13 +204,30 @@ template <int TM> __device__ __forceinline__ XTile x_locate(const XgemmParams &p
 __device__ __forceinline__ float x_sigmoid(float z) { return 1.0f / (1.0f + __expf(-z)); }
 __device__ __forceinline__ float x_silu(float z) { return z / (1.0f + __expf(-z)); }
 
+/*
+ * The normal distribution's integral up to z, and exp(-z^2 / 2), which both gelu and its slope are made of: erfc(x) = P(t) exp(-x^2), t = 1 / (1 + 0.3275911 x),
+ * x = |z| / sqrt 2, to 1.5e-7 (Abramowitz and Stegun, 7.1.26), so to 1.3 steps of 2^-24 here, 4.6 with
+ * the roundings of the terms (checked from -12 to 12). The library's erf and exp cost the gradient's stream of
+ * 16384 x 7168 201 us instead of 192 (183 at a copy's rate).
+ */
+struct XNormal { float integral, bell; };
+__device__ __forceinline__ XNormal x_normal(float z)
+{
+    const float t = 1.0f / (1.0f + 0.231641888f * fabsf(z)), bell = __expf(-0.5f * z * z);
+    const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
+    const float tail = 0.5f * poly * bell;
+    return {z < 0.0f ? tail : 1.0f - tail, bell};
+}
+/* 0.5 (1 + tanh u) is the sigmoid of 2 u */
+__device__ __forceinline__ float x_gelu_gate(float z) { return x_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z)); }
+
 __device__ __forceinline__ float x_activate(int act, float z)
 {
     switch (act) {
         case ACT_RELU: return z > 0.0f ? z : (z == z ? 0.0f : z);
         case ACT_SILU: return x_silu(z);
-        case ACT_GELU: return 0.5f * z * (1.0f + erff(z * 0.70710678118654752f));
-        case ACT_GELU_TANH: return 0.5f * z * (1.0f + tanhf(0.79788456080286536f * (z + 0.044715f * z * z * z)));
+        case ACT_GELU: return z * x_normal(z).integral;
+        case ACT_GELU_TANH: return z * x_gelu_gate(z);
         default: return z;
     }
 }
@@ -224,10 +241,13 @@ __device__ __forceinline__ float x_slope(int act, float z)
             const float s = x_sigmoid(z);
             return s * (1.0f + z * (1.0f - s));
         }
-        case ACT_GELU: return 0.5f * (1.0f + erff(z * 0.70710678118654752f)) + z * 0.39894228040143268f * expf(-0.5f * z * z);
+        case ACT_GELU: {
+            const XNormal n = x_normal(z);
+            return n.integral + z * 0.39894228040143268f * n.bell;
+        }
         case ACT_GELU_TANH: {
-            const float c = 0.79788456080286536f, t = tanhf(c * (z + 0.044715f * z * z * z));
-            return 0.5f * (1.0f + t) + 0.5f * z * (1.0f - t * t) * c * (1.0f + 0.134145f * z * z);
+            const float s = x_gelu_gate(z), w = s * (1.0f - s);
+            return w == 0.0f ? s : s + z * w * 1.5957691216057308f * (1.0f + 0.134145f * z * z);        /* far out z^2 is infinite */
         }
         default: return 1.0f;
     }

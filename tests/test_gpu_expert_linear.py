@@ -246,6 +246,19 @@ def test_gradients_of_activations(buf, rows, E, K, N, act):
     backward_case(buf, rows, E, K, N, torch.bfloat16, act, grad_dtype=torch.float32, bias=False)
 
 
+@pytest.mark.parametrize("act", ["silu", "gelu", "gelu_tanh"])
+def test_slopes_far_out(buf, act):
+    """nothing becomes infinite or no number where the activation has long been straight"""
+    z = torch.tensor([[-3e38, -1e30, -1e20, -300.0, -40.0, -12.0, 0.0, -0.0, 12.0, 40.0, 300.0, 1e20, 1e30, 3e38, 1e-30, -1e-30]], device="cuda").to(torch.bfloat16)
+    x, w = torch.zeros((1, 8), device="cuda", dtype=torch.bfloat16), torch.zeros((8, 16), device="cuda", dtype=torch.bfloat16)
+    gz = buf.expert_linear_backward(torch.ones_like(z), x, w, activation=act, preact=z)[3]
+    want = torch.tensor([[0.0] * 6 + [0.5] * 2 + [1.0] * 6 + [0.5] * 2], device="cuda")
+    assert (gz.float() - want).abs().max() < 2.0 ** -9 + 13 * 7e-6        # a rounding; silu's slope at -12 is -11 exp(-12)
+    y = buf.expert_linear(x, w, bias=z[0].float(), activation=act)
+    exact = act64(z.double(), act)
+    assert ((y.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 8 * U * z.double().abs().clamp(max=12)).all()
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 0], [0, 0, 90], [90, 0, 0], [20, 30, 10], [-4, 70, 1 << 30]])
 @pytest.mark.parametrize("K,N", [(128, 128), (66, 130)])
 def test_gradient_counts(buf, counts, K, N):

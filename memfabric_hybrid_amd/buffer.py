@@ -416,10 +416,10 @@ class Buffer:
         """Extension: the experts' product y = act(x W + bias) + residual on rows as an unquantised dispatch leaves them. x [rows, k]
         bf16 or fp16, sorted by expert; weight [experts, k, n] of x's type ([experts, n, k] if transposed; one expert's may
         leave out the first dimension); tokens_per_expert [experts] int32 or int64 on the device: what get_dispatch_layout and
-        low_latency_dispatch return (one expert: None means all rows). Rows past their sum are neither read nor written. bias
-        [experts, n] of x's type or fp32. activation: none, relu, silu, gelu, gelu_tanh or swiglu (silu of the first n / 2
-        columns times the others, y is [rows, n / 2]). residual of y's shape and type. y is of x's type or, with out_dtype,
-        torch.float32; out: a tensor to write it to. Sums are held in 32 bits, every output is rounded once.
+        low_latency_dispatch return, as counts, not as running sums (one expert: None means all rows). Rows past their sum are
+        neither read nor written. bias [experts, n] of x's type or fp32. activation: none, relu, silu, gelu, gelu_tanh or swiglu
+        (silu of the first n / 2 columns times the others, y is [rows, n / 2]). residual of y's shape and type. y is of x's type
+        or, with out_dtype, torch.float32; out: a tensor to write it to. Sums are held in 32 bits, every output is rounded once.
         Returns y, or (y, x W + bias of x's type) with return_preact."""
         y, preact = self.runtime.expert_linear(x, weight, tokens_per_expert, bias, activation, residual, out_dtype, transposed,
                                                return_preact, out)

@@ -8,7 +8,7 @@
  * groups, and in them a few candidates more than there are picks, by choices of 32 bits (without a bias by the logits, whose order is that of the
  * scores), and ranks the candidates, one to a lane, by their choices in 64 bits, of whose scores the weights are made. A row whose groups are
  * closer than the rounding of 32 bits (one in some thousands) is worked out in 64 bits from the start. What bounds it is the number of
- * instructions: 8192 tokens, 256 experts in eight groups, 13.1 us; all rows in 64 bits 19.6; picks by rounds of arg-max in 32 bits 21.8.
+ * instructions: 8192 tokens, 256 experts in eight groups, 12.9 us; all rows in 64 bits 19.6; picks by rounds of arg-max in 32 bits 21.8.
  */
 #include "zbal_device.h"
 #include "zbal_hip_kernels.h"
@@ -27,15 +27,12 @@ __device__ __forceinline__ float logit_at(const void *p, int dtype, int64_t i)
     return dtype == ZDT_BF16 ? zb_bf16_to_f32(h) : zb_fp16_to_f32(h);
 }
 
-template <int CTRL> __device__ __forceinline__ float swapped(float v)
-{
-    return __int_as_float(__builtin_amdgcn_update_dpp(0, __float_as_int(v), CTRL, 0xf, 0xf, true));
-}
+template <int CTRL> __device__ __forceinline__ int swapped(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, 0xf, 0xf, true); }
+template <int CTRL> __device__ __forceinline__ float swapped(float v) { return __int_as_float(swapped<CTRL>(__float_as_int(v))); }
 template <int CTRL> __device__ __forceinline__ double swapped(double v)
 {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
-    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)u, CTRL, 0xf, 0xf, true);
-    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(u >> 32), CTRL, 0xf, 0xf, true);
+    const uint32_t lo = (uint32_t)swapped<CTRL>((int)(uint32_t)u), hi = (uint32_t)swapped<CTRL>((int)(uint32_t)(u >> 32));
     return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 /* over each run of LANES lanes, to all of them: neighbours, pairs, the halves of eight and of sixteen mirrored, then the rest */
@@ -50,26 +47,12 @@ template <int LANES, typename V, typename F> __device__ __forceinline__ V over_l
     return v;
 }
 
-__device__ __forceinline__ double shfl_xor_f64(double v, int mask) { return __shfl_xor(v, mask, 64); }
 __device__ __forceinline__ double lane_f64(double v, int lane)
 {
     const uint64_t u = __builtin_bit_cast(uint64_t, v);
     const uint64_t lo = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)u, lane), hi = (uint32_t)__builtin_amdgcn_readlane((int)(uint32_t)(u >> 32), lane);
     return __builtin_bit_cast(double, hi << 32 | lo);
 }
-__device__ __forceinline__ double wave_max_f64(double v)
-{
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v = fmax(v, shfl_xor_f64(v, off));
-    return v;
-}
-__device__ __forceinline__ double wave_sum_f64(double v)
-{
-#pragma unroll
-    for (int off = 32; off > 0; off >>= 1) v += shfl_xor_f64(v, off);
-    return v;
-}
-
 struct RouteParams {
     const void *logits;
     int dtype, tokens, experts, topk, groups, kept, score, by_max, renormalize;
@@ -153,7 +136,7 @@ template <int SLOTS> struct RouteRow {
                 s[i] = mine(i) ? exp((double)l[i] - (double)top) : 0.0;
                 part += s[i];
             }
-            const double sum = wave_sum_f64(part);
+            const double sum = over_lanes<64>(part, [](double a, double b) { return a + b; });
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) s[i] /= sum;
         } else {
@@ -175,7 +158,7 @@ template <int SLOTS> struct RouteRow {
                 b1 = fmax(b1, c[i]);
             }
             for (int off = 1; off < 1 << p.log2_lanes; off <<= 1) {
-                const double o1 = shfl_xor_f64(b1, off), o2 = shfl_xor_f64(b2, off);
+                const double o1 = __shfl_xor(b1, off, 64), o2 = __shfl_xor(b2, off, 64);
                 b2 = fmax(fmin(b1, o1), fmax(b2, o2));
                 b1 = fmax(b1, o1);
             }
@@ -190,19 +173,14 @@ template <int SLOTS> struct RouteRow {
             double best = c[0];
 #pragma unroll
             for (int i = 1; i < SLOTS; ++i) best = fmax(best, c[i]);
-            best = wave_max_f64(best);
+            best = over_lanes<64>(best, [](double a, double b) { return fmax(a, b); });
             if (best == none) break;
             int e = 0x7fffffff;
             double es = 0.0;
 #pragma unroll
             for (int i = SLOTS - 1; i >= 0; --i)
                 if (c[i] == best) { e = expert_of(i); es = s[i]; }
-            int lowest = e;
-#pragma unroll
-            for (int off = 32; off > 0; off >>= 1) {
-                const int o = __shfl_xor(lowest, off, 64);
-                lowest = o < lowest ? o : lowest;
-            }
+            const int lowest = over_lanes<64>(e, [](int a, int b) { return a < b ? a : b; });
             const int owner = __ffsll((long long)__ballot(e == lowest)) - 1;
             es = lane_f64(es, owner);
 #pragma unroll
@@ -244,7 +222,7 @@ template <int SLOTS> struct RouteRow {
                 double d = 0.0;
 #pragma unroll
                 for (int i = 0; i < SLOTS; ++i) d += mine(i) ? exp((double)l[i] - (double)top) : 0.0;
-                sum = wave_sum_f64(d);
+                sum = over_lanes<64>(d, [](double a, double b) { return a + b; });
             }
         } else {
 #pragma unroll
@@ -298,15 +276,16 @@ template <int SLOTS> struct RouteRow {
         low = -zb_wave_reduce_dpp<true>(-low);
         if (high == __builtin_inff()) return false;    /* nothing to halve */
         uint64_t has[SLOTS];
-        auto reach = [&](float v) __attribute__((always_inline)) {
+        auto reach = [&](float v) __attribute__((always_inline)) {       /* v is finite, or no number */
             int n = 0;
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) {
-                has[i] = __ballot(key[i] >= v && key[i] > none);
+                has[i] = __ballot(key[i] >= v);
                 n += __popcll(has[i]);
             }
             return n;
         };
+        if (high == none) low = 0.0f;                  /* nothing to pick */
         int count = reach(low);
         const int enough = p.topk + 4;
         for (int i = 0; i < 40 && count > enough; ++i) {
@@ -318,7 +297,7 @@ template <int SLOTS> struct RouteRow {
             else high = mid;
         }
         /* and what rounding may have left below it */
-        count = reach(low - kStep * fmaxf(1.0f, fabsf(low)));
+        count = reach(fmaxf(low - kStep * fmaxf(1.0f, fabsf(low)), -3.402823466e38f));
         if (count > 64) return false;
         int before = 0;
 #pragma unroll

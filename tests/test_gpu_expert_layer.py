@@ -116,3 +116,25 @@ def test_layer_captured(buf):
         want = step(src)
         torch.cuda.synchronize()
         assert all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("T", [1, 2, 40])
+def test_experts_behind_the_low_latency_exchange(buf, T):
+    """serving: rows packed by expert and int64 counts, nothing quantised"""
+    H, E, I, K = 512, 16, 256, 4
+    p, g = parameters(H, E, I, torch.bfloat16, T)
+    x = torch.randn((T, H), device="cuda", generator=g).to(torch.bfloat16)
+    idx, w = buf.group_route(buf.expert_linear(x, p["gate"], out_dtype=torch.float32), K, 4, 2)
+    recv, counts, handle, _, _ = buf.low_latency_dispatch(x, idx, 64, E, use_fp8=False)
+    assert counts.dtype == torch.int64
+    h = buf.expert_linear(recv, p["w1"], counts, activation="swiglu")
+    out, _, _ = buf.low_latency_combine(buf.expert_linear(h, p["w2"], counts), idx, w, handle)
+    F = torch.nn.functional
+    want = torch.zeros((T, H), dtype=torch.float64, device="cuda")
+    for t in range(T):
+        for k in range(K):
+            e = int(idx[t, k])
+            gate, up = (x[t].double() @ p["w1"][e].double()).chunk(2)
+            want[t] += w[t, k].double() * ((F.silu(gate) * up) @ p["w2"][e].double())
+    # three roundings to bf16, of h, of a pick's row and of the sum; those of h meet I terms of w2's size I^-1/2
+    assert (out.double() - want).norm() <= 3 * 2.0 ** -8 * want.norm()

@@ -192,7 +192,7 @@ expert_gemm_any_kernel(XgemmParams p)
     }
     /*
      * Through the LDS, a row sub-tile of every wave at a time: neighbouring lanes then have neighbouring columns, whose loads and stores are one
-     * access each, and several of them under way (1021 x 1001 x 1531, gelu, bias and residual: 63 us, from the sums' own lanes, one after the other, 96).
+     * access each, and several of them under way (1021 x 1001 x 1531, gelu, bias and residual, from the sums' own lanes, one after the other: 33 us more).
      */
     constexpr int LD = TN + 1, ROWS = WM * 16;
     static_assert(ROWS * LD * 4 <= (TM + TN) * 128, "sums fit the operands' place");

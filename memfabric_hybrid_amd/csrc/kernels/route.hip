@@ -194,14 +194,16 @@ template <int SLOTS> struct RouteRow {
     /*
      * By 32 bits as far as they decide; false, with nothing written, where they do not.
      *
-     * How far choices of 32 bits may be off: an exponential and a quotient of one or two steps each, the rounding of the exponential's argument (which the
-     * slope of the sigmoid keeps under a quarter of a step of one; softmax: 2^-24 |l - max| of a score, less than that of the largest), a sum of up to
-     * 1024 terms in a tree of some twenty additions, and the bias's addition: under 16 steps of 2^-24 of the larger of one and the choice,
-     * twice that for a sum of two. kStep leaves a factor of two.
+     * How far choices of 32 bits may be off, in steps of 2^-24. A sigmoid: 2 |l| of its exponential for the rounding of the argument, which its slope makes 0.45, the
+     * exponential's own 2 a quarter of that, sum and quotient 3: under 4. A softmax: 3 |l - max| of the score, which is at most exp(l - max), so 1.1; its
+     * exponential, quotient and product 6: under 7.1, with the sum in 64 bits (without a bias the sum's error is a common factor of all choices, and changes no order).
+     * The choice's own rounding: 1 of its size. So 8.1 of the larger of one and the choice. Two choices in question are 16.2 apart at most, and 1 for what
+     * the limit itself is rounded by: kStep is 64. A group's sum is off by what its two choices are, whose sizes a bias may make far larger than the sum, and
+     * the rounding of the sum and of its bounds, 2 of the two sizes: 10.1 of each size, where kOff is 16.
      */
     __device__ bool quick(Candidate *candidates)
     {
-        constexpr float kStep = 0x1p-18f;
+        constexpr float kStep = 0x1p-18f, kOff = 0x1p-20f;
         const float none = -__builtin_inff();
         const bool by_logit = p.bias == nullptr;       /* the order of the logits is that of the scores */
         float key[SLOTS], c[SLOTS], b[SLOTS], top = 0.0f;
@@ -214,16 +216,19 @@ template <int SLOTS> struct RouteRow {
                 c[i] = mine(i) ? __builtin_amdgcn_exp2f((l[i] - top) * 1.44269504f) : 0.0f;
                 part += c[i];
             }
-            const float over = __builtin_amdgcn_rcpf(zb_wave_reduce_dpp<false>(part));
-#pragma unroll
-            for (int i = 0; i < SLOTS; ++i) c[i] *= over;
             /* over the sum of the picks' scores, the sum of all cancels */
             if (!by_logit || !p.renormalize) {
                 double d = 0.0;
 #pragma unroll
                 for (int i = 0; i < SLOTS; ++i) d += mine(i) ? exp((double)l[i] - (double)top) : 0.0;
                 sum = over_lanes<64>(d, [](double a, double b) { return a + b; });
+                part = (float)sum;
+            } else {
+                part = zb_wave_reduce_dpp<false>(part);
             }
+            const float over = __builtin_amdgcn_rcpf(part);
+#pragma unroll
+            for (int i = 0; i < SLOTS; ++i) c[i] *= over;
         } else {
 #pragma unroll
             for (int i = 0; i < SLOTS; ++i) c[i] = __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(l[i] * -1.44269504f));
@@ -253,14 +258,17 @@ template <int SLOTS> struct RouteRow {
             if (p.log2_lanes > 2) join(swapped<0x141>(b1), swapped<0x141>(b2));      /* the halves of eight and of sixteen lanes, mirrored */
             if (p.log2_lanes > 3) join(swapped<0x140>(b1), swapped<0x140>(b2));
             if (p.log2_lanes > 4) join(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
-            const float score = p.by_max || b2 == none ? b1 : b1 + b2;
+            const bool two = !p.by_max && b2 > none, exact_keys = p.by_max && by_logit;
+            const float score = two ? b1 + b2 : b1;
             const bool keep = rank_of_group(score) < p.kept && group < p.groups;
-            /* the last group kept against the best of the others */
-            const float least = -zb_wave_reduce_dpp<true>(keep ? -score : none), most = zb_wave_reduce_dpp<true>(keep || group >= p.groups ? none : score);
-            const float gap = least - most, size = fmaxf(1.0f, fmaxf(fabsf(least), fabsf(most)));
+            /* the least that a group kept can be against the most that one of the others can be; logits are what they are */
+            float off = b1 > none && !exact_keys ? kOff * fmaxf(1.0f, fabsf(b1)) : 0.0f;
+            if (two) off += kOff * fmaxf(1.0f, fabsf(b2));
+            const float least = -zb_wave_reduce_dpp<true>(keep ? off - score : none), most = zb_wave_reduce_dpp<true>(keep || group >= p.groups ? none : score + off);
+            const float gap = least - most, apart = exact_keys ? kStep * fmaxf(1.0f, fmaxf(fabsf(least), fabsf(most))) : 0.0f;
             /* equal logits are a tie, for the lower index, if the next ones above have scores of 64 bits above theirs */
-            const bool tie = p.by_max && by_logit && gap == 0.0f && fabsf(least) > 0x1p-10f && least < 20.0f && least - top > -600.0f;
-            if (most > none && !(gap > kStep * size) && !tie) return false;
+            const bool tie = exact_keys && gap == 0.0f && fabsf(least) > 0x1p-10f && least < 20.0f && least - top > -600.0f;
+            if (most > none && !(gap > apart) && !tie) return false;
             if (!keep)
 #pragma unroll
                 for (int i = 0; i < SLOTS; ++i) key[i] = none;

@@ -159,6 +159,38 @@ def test_logits_so_small_that_their_scores_are_equal(buf):
     check(buf, logits, 20)
 
 
+def picks64(logits, topk, groups, kept, score, bias, group_score):
+    """plain()'s picks for many rows at once, with stable sorts"""
+    c = scores(logits, score) + bias.double()
+    c = torch.where((logits > -INF) & (c > -INF), c, -INF)
+    T, E = logits.shape
+    v = c.view(T, groups, E // groups).sort(dim=-1, descending=True).values
+    of = v[..., 0]
+    if group_score == "top2" and E > groups:
+        of = of + torch.where(v[..., 1] > -INF, v[..., 1], 0.0)
+    keep = torch.zeros((T, groups), dtype=torch.bool).scatter_(1, of.sort(dim=-1, descending=True, stable=True).indices[:, :kept], True)
+    c = torch.where(keep.repeat_interleave(E // groups, dim=1), c, -INF)
+    value, idx = c.sort(dim=-1, descending=True, stable=True)
+    return torch.where(value[:, :topk] > -INF, idx[:, :topk], -1)
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("size", [1e2, 1e4, 1e6])
+def test_biases_that_cancel_in_a_group(buf, score, size):
+    """a group's sum is near one, its two choices are rounded where the bias is: the picks are those of 64 bits all the same"""
+    g = gen(int(size))
+    for E, groups, kept, K in ((4, 2, 1, 2), (64, 8, 3, 4)):
+        T = 1 << 17 if E == 4 else 1 << 14
+        logits = torch.randn((T, E), generator=g)
+        bias = torch.tensor([size, -size]).repeat(E // 2)
+        if E > 4:                                                # one pair in a group is far above its others
+            bias = torch.where(torch.arange(E) % 8 < 2, bias, -3 * size)
+        for group_score in ("top2", "max"):
+            idx = buf.group_route(logits.cuda(), K, groups, kept, score, bias.cuda(), group_score)[0].cpu()
+            want = picks64(logits, K, groups, kept, score, bias, group_score)
+            assert torch.equal(idx, want), (E, group_score, (idx != want).any(-1).sum().item())
+
+
 def test_an_empty_batch(buf):
     idx, w = buf.group_route(torch.empty((0, 16), device="cuda"), 4)
     assert idx.shape == w.shape == (0, 4)

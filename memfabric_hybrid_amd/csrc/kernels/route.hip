@@ -259,7 +259,8 @@ template <int SLOTS> struct RouteRow {
             if (p.log2_lanes > 3) join(swapped<0x140>(b1), swapped<0x140>(b2));
             if (p.log2_lanes > 4) join(__shfl_xor(b1, 16, 64), __shfl_xor(b2, 16, 64));
             const bool two = !p.by_max && b2 > none, exact_keys = p.by_max && by_logit;
-            const float score = two ? b1 + b2 : b1;
+            /* a sum past the lowest number is still more than a group that has no experts */
+            const float score = two ? fmaxf(b1 + b2, -3.402823466e38f) : b1;
             const bool keep = rank_of_group(score) < p.kept && group < p.groups;
             /* the least that a group kept can be against the most that one of the others can be; logits are what they are */
             float off = b1 > none && !exact_keys ? kOff * fmaxf(1.0f, fabsf(b1)) : 0.0f;

@@ -191,6 +191,17 @@ def test_biases_that_cancel_in_a_group(buf, score, size):
             assert torch.equal(idx, want), (E, group_score, (idx != want).any(-1).sum().item())
 
 
+def test_biases_of_the_lowest_value(buf):
+    """two of them are minus infinity in 32 bits; a group of theirs still comes before one that is ruled out"""
+    low = torch.finfo(torch.float32).min
+    logits = torch.randn((40, 8), generator=gen(21))
+    logits[:20, :2] = -INF
+    for b in ([0, 0, low, low, low, low, 0, 0], [0, 0, low, low, -3.3e38, -3.3e38, 0, 0], [0, 0, 3e38, 3e38, 3.3e38, 3.3e38, 0, 0], [low] * 8):
+        for kept in (1, 2, 3):
+            for group_score in ("top2", "max"):
+                check(buf, logits, 2 * kept, groups=4, kept=kept, bias=torch.tensor(b), group_score=group_score)
+
+
 def test_an_empty_batch(buf):
     idx, w = buf.group_route(torch.empty((0, 16), device="cuda"), 4)
     assert idx.shape == w.shape == (0, 4)

@@ -408,7 +408,7 @@ ZBALHIP_API int32_t zbalhip_gemm_prepare(void);
  * slots without a pick get the id -1 and the weight 0. weight = scale * s, over the sum of the picks' s if renormalize (0 where that sum is
  * 0). topk_idx [T,K] as in zbalhip_topk_route, topk_w [T,K] fp32. E <= 1024, K <= 32, groups <= 64, K <= experts of the kept groups.
  * The gradient takes logits, score, renormalize, scale and the picks (ids outside [0,E) are none; equal ones add up): grad_w [T,K] fp32 ->
- * grad_logits [T,E] of the logits' type. The bias has none.
+ * grad_logits [T,E] of the logits' type, zeros for a row without picks. The bias has none.
  */
 typedef struct {
     const void *logits;

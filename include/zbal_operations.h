@@ -256,7 +256,7 @@ int32_t zbal_moe_group_route(const zbal_tensor_info_t *logits, const zbal_tensor
 
 /*
  * extension: its gradient. gradWeight [T, K] fp32, topkIndex as the router left it -> gradLogits [T, E] of the logits' type. Ids outside
- * [0, E) are no picks. The bias, which only decides, has no gradient.
+ * [0, E) are no picks; a row without picks gets zeros, whatever its logits. The bias, which only decides, has no gradient.
  */
 int32_t zbal_moe_group_route_backward(const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *logits,
                                       const zbal_tensor_info_t *topkIndex, zbal_score_t score, int64_t renormalize,

@@ -405,7 +405,8 @@ class Buffer:
     def group_route_backward(self, grad_weights: torch.Tensor, logits: torch.Tensor, topk_idx: torch.Tensor,
                              score: str = "sigmoid", renormalize: bool = True, scale: float = 1.0) -> torch.Tensor:
         """Extension: the logits' gradient from that of group_route's weights, with the picks as they were made (the picking itself
-        and the bias have none). Ids outside [0, experts) are no picks."""
+        and the bias have none). Ids outside [0, experts) are no picks; a row without picks has a gradient of zeros, whatever its
+        logits."""
         return self.runtime.group_route_backward(grad_weights, logits, topk_idx, score, renormalize, scale)
 
     # ---- unquantised experts ----------------------------------------------------------------------------

@@ -380,7 +380,8 @@ __device__ __forceinline__ float exp_of(float t)
  * Lane k of a token's LANES has its k-th pick: d_k = dL/ds_k is scale g_k, or, where the weights are over their sum S, scale / S (g_k -
  * sum_j g_j s_j / S). An expert's D is the sum over its picks (the first of them adds up in order, should an expert be there twice).
  * sigmoid: dl = D s (1 - s), nothing where there is no pick. softmax: dl = s (D - sum D s): with weights over their sum, sum D s is zero and
- * nothing but the picks has a gradient either; else every logit has one.
+ * nothing but the picks has a gradient either; else every logit has one. A row that has no pick has a gradient of zeros whatever its logits, and so has
+ * one whose logits are all minus infinity, where a softmax is no number.
  *
  * The picks' part is in 64 bits and the same number of instructions for one token as for four, so a wave has as many tokens as their picks and
  * a sixteenth of their logits leave room for; the logits are read once, four at a time, and stay in registers. 16384 tokens, 128 experts, softmax over
@@ -445,17 +446,24 @@ group_route_backward_kernel(RouteBackParams p)
 #pragma unroll
         for (int i = 0; i < kBackLogits; ++i) mx = fmaxf(mx, x[i]);
         mx = over_lanes<LANES>(mx, larger);
+        const bool none_picked = over_lanes<LANES>(e, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; }) < 0;
         float part = 0.0f;
+        if (none_picked || mx == none) {
 #pragma unroll
-        for (int i = 0; i < kBackLogits; ++i) {
-            x[i] = exp_of(x[i] - mx);
-            part += x[i];
+            for (int i = 0; i < kBackLogits; ++i) x[i] = 0.0f;
+            part = 1.0f / LANES;
+        } else {
+#pragma unroll
+            for (int i = 0; i < kBackLogits; ++i) {
+                x[i] = exp_of(x[i] - mx);
+                part += x[i];
+            }
         }
         sum = over_lanes<LANES>((double)part, plus);
     } else if (p.score == SCORE_SOFTMAX) {
         mx = over_lanes<LANES>(l, larger);                   /* the other logits cancel */
     }
-    if (e >= 0) s = p.score == SCORE_SOFTMAX ? exp((double)l - (double)mx) / sum : 1.0 / (1.0 + exp(-(double)l));
+    if (e >= 0) s = p.score == SCORE_SIGMOID ? 1.0 / (1.0 + exp(-(double)l)) : (l == none ? 0.0 : exp((double)l - (double)mx) / sum);
     double d = g;
     if (p.renormalize) {
         const double total = over_lanes<LANES>(s, plus), gs = over_lanes<LANES>(g * s, plus);

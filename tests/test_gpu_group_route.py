@@ -246,6 +246,65 @@ def test_gradient(buf, E, K, score, renormalize):
         assert ((got.double() - want).abs() <= half * want.abs() + slack * (1 + half) + tiny).all()
 
 
+def formula_backward(grad, logits, idx, score, renormalize, scale):
+    """The gradient's formula in 64 bits, and the size of the terms that cancel in it. Scores that are no numbers, of a row that is ruled out as
+    a whole, are none: such a row has no picks, and no gradient."""
+    s = scores(logits, score).nan_to_num(0.0)
+    there = (idx >= 0) & (idx < logits.shape[1])
+    at = torch.where(there, idx, 0)
+    p = torch.gather(s, 1, at) * there
+    d = torch.where(there, grad.double(), 0.0) * scale
+    mag = d.abs()
+    if renormalize:
+        total = p.sum(-1, keepdim=True)
+        over = torch.where(total > 0, 1 / torch.where(total > 0, total, 1.0), 0.0)
+        mag = there * (mag + (mag * p).sum(-1, keepdim=True) * over) * over
+        d = there * (d - (d * p).sum(-1, keepdim=True) * over) * over
+    D, M = torch.zeros_like(s).scatter_add_(1, at, d), torch.zeros_like(s).scatter_add_(1, at, mag)
+    if score == "sigmoid":
+        return D * s * (1 - s), M * s
+    if renormalize:                                              # the sum is zero
+        return D * s, M * s
+    return s * (D - (D * s).sum(-1, keepdim=True)), s * (M + (M * s).sum(-1, keepdim=True))
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renormalize", [True, False])
+@pytest.mark.parametrize("E,K", [(7, 3), (64, 8), (65, 17), (256, 8), (1000, 32)])
+def test_gradient_of_masked_rows(buf, E, K, score, renormalize):
+    """logits of minus infinity: some, all but one, a whole row; picks that the router left out, and ones that are ruled out"""
+    g = gen(E + K)
+    T = 24
+    for dtype in (torch.float32, torch.bfloat16):
+        logits = (torch.randn((T, E), generator=g) * 1.5).to(dtype)
+        for t in range(T):
+            logits[t, torch.randperm(E, generator=g)[: (0, 1, K, E // 2, E)[t % 5]:]] = -INF
+        logits[5] = -INF
+        idx = buf.group_route(logits.cuda(), K, score=score, renormalize=renormalize)[0].cpu()
+        assert (idx[5] == -1).all()
+        idx[8::2] = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(8, T, 2)])
+        masked = (logits[23] == -INF).nonzero().flatten()
+        if masked.numel():                                       # nothing but ruled-out picks
+            idx[23] = masked[torch.arange(K) % masked.numel()]
+        grad = torch.randn((T, K), generator=g)
+        got = buf.group_route_backward(grad.cuda(), logits.cuda(), idx.cuda(), score, renormalize, 2.5).cpu()
+        want, mag = formula_backward(grad, logits, idx, score, renormalize, 2.5)
+        half, tiny = torch.finfo(dtype).eps / 2, 1e-44
+        assert ((got.double() - want).abs() <= half * want.abs() + (8 + E / 16) * 2.0 ** -24 * (1 + half) * mag + tiny).all()
+        assert (got[5] == 0).all()
+
+
+@pytest.mark.parametrize("score", ["sigmoid", "softmax"])
+@pytest.mark.parametrize("renormalize", [True, False])
+def test_gradient_of_rows_without_picks(buf, score, renormalize):
+    """whatever their logits: the weights are zeros there, and do not change"""
+    logits = torch.randn((6, 96), generator=gen(4))
+    logits[0], logits[1, 5], logits[2, 7], logits[3], logits[4, ::2] = -INF, math.nan, INF, math.nan, INF
+    idx = torch.full((6, 4), -1)
+    got = buf.group_route_backward(torch.ones((6, 4)).cuda(), logits.cuda(), idx.cuda(), score, renormalize, 1.0)
+    assert (got == 0).all()
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_gradient_against_differences(buf, score):
     """the forward call's own weights, at fixed picks"""

@@ -369,11 +369,20 @@ __device__ __forceinline__ void put_logit(void *p, int dtype, int64_t i, float v
     else static_cast<uint16_t *>(p)[i] = (uint16_t)(dtype == ZDT_BF16 ? zb_f32_to_bf16(v) : zb_f32_to_fp16(v));
 }
 
-/* exp(t), t <= 0, in two steps of 2^-24: the exponent's rounding goes back in */
-__device__ __forceinline__ float exp_of(float t)
+/* 2^y, y <= 0, to 2^-32: the whole part is the exponent, the rest, up to a half, goes through the polynomial that meets 2^f in the eight Chebyshev nodes. No number: 0 */
+__device__ __forceinline__ double exp2_of(double y)
 {
-    const float hi = t * 1.44269504f, lo = fmaf(t, 1.44269504f, -hi) + t * 1.92596299e-8f, v = __builtin_amdgcn_exp2f(hi);
-    return t < -104.0f ? 0.0f : fmaf(v, lo * 0.693147181f, v);
+    y = fmax(y, -1400.0);
+    const double n = __builtin_rint(y), f = y - n;
+    double v = 1.5303699001378845e-05;
+    v = __builtin_fma(v, f, 0.00015469729140704658);
+    v = __builtin_fma(v, f, 0.0013333478480888061);
+    v = __builtin_fma(v, f, 0.009618025613598036);
+    v = __builtin_fma(v, f, 0.055504109063177154);
+    v = __builtin_fma(v, f, 0.24022651213495422);
+    v = __builtin_fma(v, f, 0.6931471805568341);
+    v = __builtin_fma(v, f, 0.9999999999595622);
+    return __builtin_amdgcn_ldexp(v, (int)n);
 }
 
 /*
@@ -383,11 +392,14 @@ __device__ __forceinline__ float exp_of(float t)
  * nothing but the picks has a gradient either; else every logit has one. A row that has no pick has a gradient of zeros whatever its logits, and so has
  * one whose logits are all minus infinity, where a softmax is no number.
  *
- * The picks' part is in 64 bits and the same number of instructions for one token as for four, so a wave has as many tokens as their picks and
- * a sixteenth of their logits leave room for; the logits are read once, four at a time, and stay in registers. 16384 tokens, 128 experts, softmax over
- * all: 6.4 us, one token to a wave 16.7; 8192 tokens, 256 experts, sigmoid: 4.3 and 7.9.
+ * All of it is in 64 bits, rounded once (exponentials, their sum and the last product in 32: 0.2 us less where a row has 128 experts, 1.6 of 10.1 for 4096 tokens of
+ * 1024, and twice the error). The picks' part is the same number of instructions for one token as for four, so a wave has as many tokens as
+ * their picks and a sixteenth of their logits leave room for; the logits are read once, four at a time, and stay in registers. 16384 tokens, 128 experts,
+ * softmax over all: 6.5 us, one token to a wave 16.7; 8192 tokens, 256 experts, sigmoid: 4.2 and 7.9.
  */
 constexpr int kBackLogits = 16;                  /* of a lane */
+constexpr double kLog2e = 1.4426950408889634;
+constexpr int kUnpicked = 0x7fc05eed;            /* a place of the row that no pick has written: a NaN that arithmetic does not make */
 
 template <int LANES, bool VEC>
 __global__ void __launch_bounds__(256)
@@ -405,13 +417,14 @@ group_route_backward_kernel(RouteBackParams p)
     auto plus = [](auto a, auto b) __attribute__((always_inline)) { return a + b; };
     auto larger = [](float a, float b) __attribute__((always_inline)) { return fmaxf(a, b); };
 
+    const float unpicked = dense ? __int_as_float(kUnpicked) : 0.0f;
     float x[kBackLogits], mx = none;
 #pragma unroll
     for (int c = 0; c < kBackLogits / V; ++c) {
         const int at = (c * LANES + sub) * V;
         if (at >= p.experts) continue;
-        if constexpr (VEC) *reinterpret_cast<f32x4 *>(row + at) = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        else row[at] = 0.0f;
+        if constexpr (VEC) *reinterpret_cast<f32x4 *>(row + at) = f32x4{unpicked, unpicked, unpicked, unpicked};
+        else row[at] = unpicked;
     }
     int e = -1;
     double g = 0.0, s = 0.0;
@@ -424,7 +437,7 @@ group_route_backward_kernel(RouteBackParams p)
         g = (double)p.grad[(int64_t)t * p.topk + sub] * p.scale;
         l = logit_at(p.logits, p.dtype, base + e);
     }
-    double sum = 1.0;
+    double sum = 1.0, ex[kBackLogits];
     if (dense) {
 #pragma unroll
         for (int c = 0; c < kBackLogits / V; ++c) {
@@ -447,19 +460,27 @@ group_route_backward_kernel(RouteBackParams p)
         for (int i = 0; i < kBackLogits; ++i) mx = fmaxf(mx, x[i]);
         mx = over_lanes<LANES>(mx, larger);
         const bool none_picked = over_lanes<LANES>(e, [](int a, int b) __attribute__((always_inline)) { return a > b ? a : b; }) < 0;
-        float part = 0.0f;
+        double part = 0.0;
         if (none_picked || mx == none) {
 #pragma unroll
-            for (int i = 0; i < kBackLogits; ++i) x[i] = 0.0f;
-            part = 1.0f / LANES;
+            for (int i = 0; i < kBackLogits; ++i) ex[i] = 0.0;
+            part = 1.0 / LANES;
         } else {
 #pragma unroll
-            for (int i = 0; i < kBackLogits; ++i) {
-                x[i] = exp_of(x[i] - mx);
-                part += x[i];
+            for (int c = 0; c < kBackLogits / V; ++c) {
+                if (c * LANES * V >= p.experts) continue;            /* nobody's */
+#pragma unroll
+                for (int i = c * V; i < c * V + V; ++i) {
+                    ex[i] = exp2_of(__builtin_fma((double)x[i], kLog2e, (double)mx * -kLog2e));
+                    part += ex[i];
+                }
             }
+            bool nan = false;
+#pragma unroll
+            for (int i = 0; i < kBackLogits; i += 2) nan = nan || __builtin_isunordered(x[i], x[i + 1]);
+            if (nan) part = __builtin_nan("");
         }
-        sum = over_lanes<LANES>((double)part, plus);
+        sum = over_lanes<LANES>(part, plus);
     } else if (p.score == SCORE_SOFTMAX) {
         mx = over_lanes<LANES>(l, larger);                   /* the other logits cancel */
     }
@@ -469,7 +490,7 @@ group_route_backward_kernel(RouteBackParams p)
         const double total = over_lanes<LANES>(s, plus), gs = over_lanes<LANES>(g * s, plus);
         d = e >= 0 && total > 0.0 ? (g - gs / total) / total : 0.0;
     }
-    const float c = dense ? (float)over_lanes<LANES>(d * s, plus) : 0.0f, over = (float)(1.0 / sum);
+    const double c = dense ? over_lanes<LANES>(d * s, plus) : 0.0, rest = -c / sum;
 
     /* an expert that is there twice: its place in the row holds one lane's number only */
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -488,7 +509,7 @@ group_route_backward_kernel(RouteBackParams p)
         }
     }
     if (p.score == SCORE_SIGMOID) all *= s * (1.0 - s);
-    else if (!dense) all *= s;
+    else all = dense ? s * (all - c) : all * s;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
     if (first) row[e] = (float)all;
     __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
@@ -501,7 +522,7 @@ group_route_backward_kernel(RouteBackParams p)
         else v[0] = row[at];
         if (dense)
 #pragma unroll
-            for (int j = 0; j < V; ++j) v[j] = x[k * V + j] * ((v[j] - c) * over);
+            for (int j = 0; j < V; ++j) v[j] = __float_as_int(v[j]) == kUnpicked ? (float)(ex[k * V + j] * rest) : v[j];
         if constexpr (!VEC) put_logit(p.out, p.dtype, base + at, v[0]);
         else if (p.dtype == ZDT_FP32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p.out) + base + at) = v;
         else {

@@ -305,6 +305,21 @@ def test_gradient_of_rows_without_picks(buf, score, renormalize):
     assert (got == 0).all()
 
 
+@pytest.mark.parametrize("E,K", [(64, 8), (65, 17), (128, 8), (1024, 32)])
+@pytest.mark.parametrize("scale", [1.0, 2.5])
+def test_dense_gradient_is_rounded_once(buf, E, K, scale):
+    """softmax scores as weights: everything in front of the last rounding is in 64 bits"""
+    g = gen(E)
+    logits = torch.randn((200, E), generator=g) * 3
+    idx = torch.stack([torch.randperm(E, generator=g)[:K] for _ in range(200)])
+    idx[3, 1], idx[4, 0] = idx[3, 0], -1
+    grad = torch.randn((200, K), generator=g)
+    got = buf.group_route_backward(grad.cuda(), logits.cuda(), idx.cuda(), "softmax", False, scale).cpu().double()
+    want, mag = formula_backward(grad, logits, idx, "softmax", False, scale)
+    # exponentials that are good to 2^-31, on both sides of a difference
+    assert ((got - want).abs() <= 2.0 ** -24 * want.abs() + 2.0 ** -28 * mag + 1e-44).all()
+
+
 @pytest.mark.parametrize("score", ["sigmoid", "softmax"])
 def test_gradient_against_differences(buf, score):
     """the forward call's own weights, at fixed picks"""

@@ -205,18 +205,34 @@ __device__ __forceinline__ float x_sigmoid(float z) { return 1.0f / (1.0f + __ex
 __device__ __forceinline__ float x_silu(float z) { return z / (1.0f + __expf(-z)); }
 
 /*
- * The normal distribution's integral up to z, and exp(-z^2 / 2), which both gelu and its slope are made of: erfc(x) = P(t) exp(-x^2), t = 1 / (1 + 0.3275911 x),
- * x = |z| / sqrt 2, to 1.5e-7 (Abramowitz and Stegun, 7.1.26), so to 1.3 steps of 2^-24 here, 4.6 with
- * the roundings of the terms (checked from -12 to 12). The library's erf and exp cost the gradient's stream of
- * 16384 x 7168 201 us instead of 192 (183 at a copy's rate).
+ * The normal distribution's integral up to z and exp(-z^2 / 2), which gelu and its slope are made of. With x = |z| the tail is R(x) exp(-x^2 / 2), and
+ * R(x) (1 + 0.31 x) hardly changes: a polynomial of the ninth degree in w = 0.31 x / (1 + 0.31 x) that meets it in the ten Chebyshev nodes of x = 0 .. 16 is good to
+ * 2^-26. The square's rounding and its product's with log2 e go back into the exponential, so that the tail, and gelu far below zero, keep their relative precision:
+ * within 7 steps of 2^-24 from -12 to 12, where 1 + erf is off by a step of one (1.6e3 steps of gelu(-3.5)). gelu's rms error for normally distributed z is 0.38
+ * steps. The library's erfc and exp are as good, and cost 4096 x 2048 x 4096 with gelu 94 us instead of 81, the gradient's stream of 16384 x 7168 217 instead of 196.
  */
 struct XNormal { float integral, bell; };
 __device__ __forceinline__ XNormal x_normal(float z)
 {
-    const float t = 1.0f / (1.0f + 0.231641888f * fabsf(z)), bell = __expf(-0.5f * z * z);
-    const float poly = ((((1.061405429f * t - 1.453152027f) * t + 1.421413741f) * t - 0.284496736f) * t + 0.254829592f) * t;
-    const float tail = 0.5f * poly * bell;
-    return {z < 0.0f ? tail : 1.0f - tail, bell};
+    const float x = fminf(fabsf(z), 16.0f), d = __builtin_fmaf(x, 0.31f, 1.0f);
+    float r = __builtin_amdgcn_rcpf(d);
+    r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
+    const float w = x * 0.31f * r;
+    float v = 0.0197242107f;
+    v = __builtin_fmaf(v, w, -0.0798610598f);
+    v = __builtin_fmaf(v, w, 0.0995214731f);
+    v = __builtin_fmaf(v, w, -0.0151915457f);
+    v = __builtin_fmaf(v, w, 0.00912341755f);
+    v = __builtin_fmaf(v, w, -0.130728304f);
+    v = __builtin_fmaf(v, w, -0.0196085535f);
+    v = __builtin_fmaf(v, w, 0.527600467f);
+    v = __builtin_fmaf(v, w, -0.786909699f);
+    v = __builtin_fmaf(v, w, 0.5f);
+    v *= r;
+    const float h = x * x, low = __builtin_fmaf(x, x, -h), a = h * -0.721347511f;
+    const float rest = __builtin_fmaf(low, -0.721347511f, __builtin_fmaf(h, -9.62981517e-09f, __builtin_fmaf(h, -0.721347511f, -a)));
+    const float e = __builtin_amdgcn_exp2f(a), bell = __builtin_fmaf(e, rest * 0.693147181f, e);
+    return {z < 0.0f ? v * bell : __builtin_fmaf(-v, bell, 1.0f), bell};
 }
 /* 0.5 (1 + tanh u) is the sigmoid of 2 u */
 __device__ __forceinline__ float x_gelu_gate(float z) { return x_sigmoid(1.5957691216057308f * (z + 0.044715f * z * z * z)); }
@@ -243,7 +259,7 @@ __device__ __forceinline__ float x_slope(int act, float z)
         }
         case ACT_GELU: {
             const XNormal n = x_normal(z);
-            return n.integral + z * 0.39894228040143268f * n.bell;
+            return __builtin_fmaf(z * 0.39894228040143268f, n.bell, n.integral);
         }
         case ACT_GELU_TANH: {
             const float s = x_gelu_gate(z), w = s * (1.0f - s);

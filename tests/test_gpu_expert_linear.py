@@ -259,6 +259,37 @@ def test_slopes_far_out(buf, act):
     assert ((y.double() - exact).abs() <= 2.0 ** -8 * exact.abs() + 8 * U * z.double().abs().clamp(max=12)).all()
 
 
+def test_gelu_keeps_its_precision(buf):
+    """Outputs of 32 bits, in steps of 2^-24 of themselves: the tail's polynomial 0.2 by its fit, 5 by its roundings; reciprocal and product 2; the bell's
+    exponential 2, its argument's rest and their sum 2; product, difference and the product with z 3."""
+    z = torch.linspace(-12.5, 12.5, 100001, device="cuda").view(1, -1)[:, :65536].contiguous()
+    z = torch.cat([z, -z])
+    x, w = torch.zeros((1, 8), device="cuda", dtype=torch.float16), torch.zeros((8, 65536), device="cuda", dtype=torch.float16)
+    for row in z:
+        y = buf.expert_linear(x, w, bias=row, activation="gelu", out_dtype=torch.float32)[0].double()
+        r = row.double()
+        want = 0.5 * r * torch.special.erfc(r * -(0.5 ** 0.5))
+        assert ((y - want).abs() <= 16 * U * want.abs() + 1e-37).all()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+def test_gelus_slope_keeps_its_precision(buf, dtype):
+    """every value of the type from 2^-8 to 8, either sign: one rounding, and terms of 32 bits as large as the integral and the bell are there"""
+    z = torch.arange(1 << 15, dtype=torch.int32).to(torch.int16).view(dtype)
+    z = z[(z >= 2.0 ** -8) & (z <= 8)]
+    z = torch.cat([-z, z]).view(1, -1).cuda()
+    z = z[:, :z.shape[1] // 8 * 8].contiguous()
+    N = z.shape[1]
+    x, w = torch.zeros((1, 8), device="cuda", dtype=dtype), torch.zeros((8, N), device="cuda", dtype=dtype)
+    gz = buf.expert_linear_backward(torch.ones_like(z), x, w, activation="gelu", preact=z)[3].double()
+    r = z.double()
+    integral, bell = 0.5 * torch.special.erfc(r * -(0.5 ** 0.5)), r.abs() * torch.exp(-0.5 * r * r) * 0.3989422804014327
+    want = integral + torch.sign(r) * bell
+    err = U * (14 * integral + 8 * bell + want.abs())
+    half = torch.exp2(torch.frexp(want.abs() + err).exponent.double()) * half_step(dtype) / 2             # of a step where the result lies
+    assert ((gz - want).abs() <= half + err + (2.0 ** -25 if dtype == torch.float16 else 1e-37)).all()
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 0], [0, 0, 90], [90, 0, 0], [20, 30, 10], [-4, 70, 1 << 30]])
 @pytest.mark.parametrize("K,N", [(128, 128), (66, 130)])
 def test_gradient_counts(buf, counts, K, N):

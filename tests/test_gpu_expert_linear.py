@@ -1,5 +1,6 @@
 """The experts' products and their gradients against plain forms in 64 bits: one row to many, sizes that no tile, chunk or register divides, both
 weight orders, every activation and part of the epilogue, experts without rows, counts that are wrong, rows that are nobody's."""
+import ctypes
 
 import pytest
 import torch
@@ -288,6 +289,36 @@ def test_gelus_slope_keeps_its_precision(buf, dtype):
     err = U * (14 * integral + 8 * bell + want.abs())
     half = torch.exp2(torch.frexp(want.abs() + err).exponent.double()) * half_step(dtype) / 2             # of a step where the result lies
     assert ((gz - want).abs() <= half + err + (2.0 ** -25 if dtype == torch.float16 else 1e-37)).all()
+
+
+@pytest.mark.parametrize("transposed", [False, True])
+@pytest.mark.parametrize("rows,E,K,N", [(9, 2, 64, 128), (1, 1, 7, 5), (70, 1, 2120, 520), (1200, 40, 72, 1928), (4033, 64, 200, 4104), (900, 3, 264, 1160), (1030, 2, 266, 2050), (17, 2, 2056, 4104),
+                                        (1, 1, 4104, 2056), (4100, 1, 2056, 264), (8200, 1, 136, 4104)])
+def test_every_preactivation_is_written_and_no_other(buf, rows, E, K, N, transposed):
+    """through the kernels' own entry, into tensors that hold NaN: the rows of experts become numbers within the sums' rounding, the rows of nobody stay"""
+    for act, name in ((2, "silu"), (5, "swiglu")):
+        if name == "swiglu" and N % 2:
+            continue
+        g, x, w, counts = make(rows, E, K, N, torch.float16, 9, transposed)
+        if rows > 1:                                             # the last rows are nobody's
+            last = max(range(E), key=lambda e: counts[e])
+            counts[last] -= 1
+        cols = N // 2 if name == "swiglu" else N
+        nan = float("nan")
+        y, z = torch.full((rows, cols), nan, device="cuda", dtype=torch.float16), torch.full((rows, N), nan, device="cuda", dtype=torch.float16)
+        ct = torch.tensor(counts, dtype=torch.int32, device="cuda")
+        d = capi.ExpertLinear(w.data_ptr(), int(transposed), capi.DT_FP16, ct.data_ptr(), 0, act, rows, K, N, E)
+        lib = capi.load()
+        size = lib.zbalhip_expert_linear_workspace(ctypes.byref(d), 0)
+        ws = torch.empty((max(size, 16),), dtype=torch.uint8, device="cuda")
+        code = lib.zbalhip_expert_linear(ctypes.byref(d), x.data_ptr(), None, 0, None, y.data_ptr(), 0, z.data_ptr(), ws.data_ptr(), size,
+                                         torch.cuda.current_stream().cuda_stream)
+        assert code == 0
+        want, mag = products(x, w, counts, transposed)
+        n = want.shape[0]
+        err = (K + 2) * U * mag
+        assert ((z[:n].double() - want).abs() <= half_step(torch.float16) * (want.abs() + err) + err + 2.0 ** -25).all()
+        assert torch.isfinite(y[:n]).all() and torch.isnan(y[n:]).all() and torch.isnan(z[n:]).all()
 
 
 @pytest.mark.parametrize("counts", [[0, 0, 0], [0, 0, 90], [90, 0, 0], [20, 30, 10], [-4, 70, 1 << 30]])

@@ -265,7 +265,8 @@ expert_join_kernel(XgemmParams p)
 
 /*
  * The pre-activation's gradient: dz = dy act'(z), for swiglu of both halves; with no activation the rounding of a gradient in 32 bits.
- * A stream of the three tensors, V elements to a lane: 16384 x 7168 out of 32 bits 137 us at eight (5.1 TB/s), 174 one by one; gelu, which reads z besides, 192, 225.
+ * A stream of the three tensors, V elements to a lane: 16384 x 7168 out of 32 bits 137 us at eight (5.1 TB/s), 174 one by one; gelu, which reads z besides, 196
+ * (one by one 225, where eight took 192).
  */
 template <int DT, int V>
 __global__ void __launch_bounds__(256)

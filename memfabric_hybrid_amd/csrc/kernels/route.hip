@@ -8,7 +8,7 @@
  * groups, and in them a few candidates more than there are picks, by choices of 32 bits (without a bias by the logits, whose order is that of the
  * scores), and ranks the candidates, one to a lane, by their choices in 64 bits, of whose scores the weights are made. A row whose groups are
  * closer than the rounding of 32 bits (one in some thousands) is worked out in 64 bits from the start. What bounds it is the number of
- * instructions: 8192 tokens, 256 experts in eight groups, 12.9 us; all rows in 64 bits 19.6; picks by rounds of arg-max in 32 bits 21.8.
+ * instructions: 8192 tokens, 256 experts in eight groups, 13.4 us; all rows in 64 bits 19.6; picks by rounds of arg-max in 32 bits 21.8.
  */
 #include "zbal_device.h"
 #include "zbal_hip_kernels.h"
@@ -395,7 +395,7 @@ __device__ __forceinline__ double exp2_of(double y)
  * All of it is in 64 bits, rounded once (exponentials, their sum and the last product in 32: 0.2 us less where a row has 128 experts, 1.6 of 10.1 for 4096 tokens of
  * 1024, and twice the error). The picks' part is the same number of instructions for one token as for four, so a wave has as many tokens as
  * their picks and a sixteenth of their logits leave room for; the logits are read once, four at a time, and stay in registers. 16384 tokens, 128 experts,
- * softmax over all: 6.5 us, one token to a wave 16.7; 8192 tokens, 256 experts, sigmoid: 4.2 and 7.9.
+ * softmax over all: 6.9 us, one token to a wave 16.7; 8192 tokens, 256 experts, sigmoid: 4.2 and 7.9.
  */
 constexpr int kBackLogits = 16;                  /* of a lane */
 constexpr double kLog2e = 1.4426950408889634;

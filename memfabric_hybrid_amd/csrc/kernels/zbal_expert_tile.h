@@ -218,16 +218,16 @@ __device__ __forceinline__ XNormal x_normal(float z)
     float r = __builtin_amdgcn_rcpf(d);
     r = __builtin_fmaf(r, __builtin_fmaf(-d, r, 1.0f), r);
     const float w = x * 0.31f * r;
-    float v = 0.0197242107f;
-    v = __builtin_fmaf(v, w, -0.0798610598f);
-    v = __builtin_fmaf(v, w, 0.0995214731f);
-    v = __builtin_fmaf(v, w, -0.0151915457f);
-    v = __builtin_fmaf(v, w, 0.00912341755f);
-    v = __builtin_fmaf(v, w, -0.130728304f);
-    v = __builtin_fmaf(v, w, -0.0196085535f);
-    v = __builtin_fmaf(v, w, 0.527600467f);
-    v = __builtin_fmaf(v, w, -0.786909699f);
-    v = __builtin_fmaf(v, w, 0.5f);
+    float v = 0x1.432956p-6f;
+    v = __builtin_fmaf(v, w, -0x1.471c64p-4f);
+    v = __builtin_fmaf(v, w, 0x1.97a3d4p-4f);
+    v = __builtin_fmaf(v, w, -0x1.f1cbecp-7f);
+    v = __builtin_fmaf(v, w, 0x1.2af4c6p-7f);
+    v = __builtin_fmaf(v, w, -0x1.0bbb48p-3f);
+    v = __builtin_fmaf(v, w, -0x1.41443cp-6f);
+    v = __builtin_fmaf(v, w, 0x1.0e21a6p-1f);
+    v = __builtin_fmaf(v, w, -0x1.92e5d4p-1f);
+    v = __builtin_fmaf(v, w, 0x1.0p-1f);
     v *= r;
     const float h = x * x, low = __builtin_fmaf(x, x, -h), a = h * -0.721347511f;
     const float rest = __builtin_fmaf(low, -0.721347511f, __builtin_fmaf(h, -9.62981517e-09f, __builtin_fmaf(h, -0.721347511f, -a)));

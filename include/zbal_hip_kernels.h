@@ -464,6 +464,60 @@ ZBALHIP_API int32_t zbalhip_combine_backward(const void *grad, const void *y, in
                                  int64_t tokens, int64_t hidden, int64_t topk, int64_t experts, void *grad_y, float *grad_w,
                                  void *stream);
 
+/*
+ * The root-mean-square norm (no reference counterpart). x [T, H] (dtype bf16, fp16 or fp32), residual of its shape and type (may be null),
+ * weight [H] of x's type or fp32 (null: ones).
+ *   h = x + residual, y = h weight / sqrt(mean(h^2) + eps), both in 32 bits; each output is rounded once from them.
+ * y and total (= h), both [T, H] of x's type, and q [T, H] with scales [T] may be null, not all three: scale = the row's largest |y| / 127, q = y / scale,
+ * rounded to nearest even. A row of zeros has the scale 0, another one 2^-126 at least, one with an infinity or a NaN the scale NaN (and any q).
+ * The gradient: x is h (total, where there was a residual); residual is not read. grad [T, H] (of y) and grad_total (of total, may be null) of x's type ->
+ * grad_x, that of x and of the residual, and grad_weight [H] (may be null) of x's type or fp32, a sum over the rows always in the same order; zeros
+ * without rows. workspace: zbalhip_rms_norm_backward_workspace bytes (-1: the sizes are not allowed) where grad_weight is asked for, 16-byte aligned, undefined
+ * before and after. T <= ZBALHIP_EXPERT_MAX_ROWS, H <= ZBALHIP_EXPERT_MAX_WIDTH, 0 < eps < infinity. total may lie on residual or x, grad_x on grad or
+ * grad_total, exactly.
+ */
+typedef struct {
+    const void *x, *residual, *weight;
+    int32_t dtype, weight_is_f32;
+    int64_t tokens, hidden;
+    float eps;
+} zbalhip_rms_norm_t;
+ZBALHIP_API int32_t zbalhip_rms_norm(const zbalhip_rms_norm_t *norm, void *y, void *total, int8_t *q, float *scales, void *stream);
+ZBALHIP_API int64_t zbalhip_rms_norm_backward_workspace(const zbalhip_rms_norm_t *norm);
+ZBALHIP_API int32_t zbalhip_rms_norm_backward(const zbalhip_rms_norm_t *norm, const void *grad, const void *grad_total, void *grad_x, void *grad_weight,
+                                  int32_t weight_grad_is_f32, void *workspace, int64_t workspace_bytes, void *stream);
+
+/*
+ * Rows in int8 behind an activation (no reference counterpart): y = act(x) in 32 bits, q and scales of y as the norm's. x [rows, width] (dtype bf16, fp16 or
+ * fp32); activation as the experts' products have it (swiglu: y is [rows, width / 2]). counts as theirs: rows past the last expert's are neither read
+ * nor written; null: all rows. rows <= ZBALHIP_EXPERT_MAX_ROWS, width <= ZBALHIP_EXPERT_MAX_WIDTH, experts <= 1024.
+ */
+typedef struct {
+    const void *counts;
+    int32_t counts_are_i64, dtype, activation;
+    int64_t rows, width, experts;
+} zbalhip_quantize_rows_t;
+ZBALHIP_API int32_t zbalhip_quantize_rows(const zbalhip_quantize_rows_t *rows, const void *x, int8_t *q, float *scales, void *stream);
+
+/*
+ * The experts' products in int8 (no reference counterpart): zbalhip_expert_linear on int8 rows and weights with a scale for each row and for each
+ * expert's column.
+ *   z = (x W) * weight_scale * x_scale + bias, y = act(z) + residual; x W is exact, in 32-bit integers; y is rounded once.
+ * x int8 [rows, K], x_scales fp32 [rows], weight int8 [E, N, K], weight_scales [E, N] fp32 or bf16; counts, activation, rows past the last expert's, sizes and
+ * workspace as there. y (and residual, of its shape and type) y_dtype bf16, fp16 or fp32; bias [E, N] fp32, or of y's type where that has 16 bits, or
+ * bf16 beside an fp32 y: bias and residual may be null.
+ */
+typedef struct {
+    const void *weight, *weight_scales;
+    int32_t weight_scales_are_f32, counts_are_i64;
+    const void *counts;
+    int32_t activation, y_dtype;
+    int64_t rows, k, n, experts;
+} zbalhip_expert_linear_int8_t;
+ZBALHIP_API int64_t zbalhip_expert_linear_int8_workspace(const zbalhip_expert_linear_int8_t *linear);
+ZBALHIP_API int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t *linear, const void *x, const float *x_scales, const void *bias,
+                                   int32_t bias_is_f32, const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
+
 #ifdef __cplusplus
 }
 #endif

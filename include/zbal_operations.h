@@ -310,6 +310,58 @@ int32_t zbal_combine_normal_backward(const zbal_tensor_info_t *grad, const zbal_
                                      const zbal_tensor_info_t *gradWeight, zbal_comm_t comm, aclrtStream stream,
                                      int64_t flags);
 
+/*
+ * extension: the root-mean-square norm. h = x + residual, y = h weight / sqrt(mean(h^2) + eps). x [T, H] bf16, fp16 or fp32; residual of its shape and
+ * type and weight [H] of its type or fp32 may be null. y and total (= h) [T, H] of x's type, and quantized int8 [T, H] with scales fp32
+ * [T] (the row's largest |y| / 127) may be null, not all three; each is rounded once from 32 bits. A row of zeros has the scale 0, one with an infinity or a
+ * NaN the scale NaN. total may be the residual's or x's memory.
+ */
+int32_t zbal_moe_rms_norm(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, const zbal_tensor_info_t *residual,
+                          double eps, const zbal_tensor_info_t *y, const zbal_tensor_info_t *total,
+                          const zbal_tensor_info_t *quantized, const zbal_tensor_info_t *scales, zbal_comm_t comm,
+                          aclrtStream stream, int64_t flags);
+
+/*
+ * extension: its gradient. x: the h that was normalised (total, where there was a residual); grad of y and gradTotal of total (may be null), of x's shape and
+ * type -> gradX, that of x and of the residual, and gradWeight [H] (may be null) of x's type or fp32, summed in 32 bits and always in the same
+ * order. workspace: zbal_moe_rms_norm_workspace_size bytes where gradWeight is asked for; it may not be shared with a call that can run at the
+ * same time.
+ */
+int32_t zbal_moe_rms_norm_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x,
+                                   const zbal_tensor_info_t *weight, const zbal_tensor_info_t *gradTotal, double eps,
+                                   const zbal_tensor_info_t *gradX, const zbal_tensor_info_t *gradWeight,
+                                   const zbal_tensor_info_t *workspace, zbal_comm_t comm, aclrtStream stream, int64_t flags);
+
+/* extension: bytes of workspace for zbal_moe_rms_norm_backward. -1 on sizes that are not allowed. */
+int64_t zbal_moe_rms_norm_workspace_size(int64_t tokens, int64_t hidden);
+
+/*
+ * extension: an activation of rows, in int8 with a scale for each row (as above): what the second of two int8 products reads. x [rows, width] bf16, fp16
+ * or fp32 -> quantized [rows, width] (swiglu: [rows, width / 2]), scales fp32 [rows]. tokensPerExpert as zbal_moe_expert_linear takes it, or null:
+ * rows past their sum are neither read nor written.
+ */
+int32_t zbal_moe_quantize_rows(const zbal_tensor_info_t *x, const zbal_tensor_info_t *tokensPerExpert,
+                               zbal_activation_t activation, const zbal_tensor_info_t *quantized,
+                               const zbal_tensor_info_t *scales, zbal_comm_t comm, aclrtStream stream, int64_t flags);
+
+/*
+ * extension: the experts' products on rows as zbal_dispatch_normal leaves them with QUANT_BF16_2_INT8. z = (x W) weightScales xScales + bias, y =
+ * act(z) + residual; x W in integers, exactly. x int8 [rows, K] with xScales fp32 [rows]; weight int8 [E, N, K] (ZBAL_WEIGHT_FORMAT_NK in
+ * reserved[0]) with weightScales [E, N] fp32 or bf16; with one expert the leading dimension may be left out. tokensPerExpert, activation and workspace as
+ * zbal_moe_expert_linear has them. y bf16, fp16 or fp32, residual of its shape and type, bias [E, N] fp32 or of y's type (beside an fp32 y: fp32 or
+ * bf16): these two may be null. Rows past the last expert's are neither read nor written.
+ */
+int32_t zbal_moe_expert_linear_int8(const zbal_tensor_info_t *x, const zbal_tensor_info_t *xScales,
+                                    const zbal_tensor_info_t *weight, const zbal_tensor_info_t *weightScales,
+                                    const zbal_tensor_info_t *tokensPerExpert, const zbal_tensor_info_t *bias,
+                                    zbal_activation_t activation, const zbal_tensor_info_t *residual,
+                                    const zbal_tensor_info_t *y, const zbal_tensor_info_t *workspace, zbal_comm_t comm,
+                                    aclrtStream stream, int64_t flags);
+
+/* extension: bytes of its workspace, often 0. -1 on sizes that are not allowed. */
+int64_t zbal_moe_expert_linear_int8_workspace_size(int64_t rows, int64_t k, int64_t n, int64_t expertNum,
+                                                   zbal_activation_t activation);
+
 #ifdef __cplusplus
 }
 #endif

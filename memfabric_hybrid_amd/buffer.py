@@ -440,6 +440,47 @@ class Buffer:
         return self.runtime.expert_linear_backward(grad, x, weight, tokens_per_expert, activation, preact, transposed, bias,
                                                    weight_grad_dtype, need_x, need_weight)
 
+    # ---- around the int8 exchange -------------------------------------------------------------------------
+    def rms_norm(self, x: torch.Tensor, weight: Optional[torch.Tensor] = None, residual: Optional[torch.Tensor] = None,
+                 eps: float = 1e-6, quantize: bool = False, need_norm: bool = True) -> Tuple[Optional[torch.Tensor], ...]:
+        """Extension: the root-mean-square norm, y = h weight / sqrt(mean(h^2) + eps) with h = x + residual. x [tokens, hidden] bf16,
+        fp16 or fp32, residual of its shape and type; weight [hidden] of its type or fp32 (None: ones). total is h, the next
+        residual (where there was one). quantize: y in int8 besides, q [tokens, hidden] with scales [tokens] fp32, the row's
+        largest magnitude / 127, as an int8 dispatch leaves rows; need_norm=False leaves out y itself. Everything is computed
+        in 32 bits and rounded once, q from the unrounded y. A row of zeros has the scale 0, one with an infinity or a NaN the
+        scale NaN. Returns (y, q, scales, total): None for what was not asked for."""
+        return self.runtime.rms_norm(x, weight, residual, eps, quantize, need_norm)
+
+    def rms_norm_backward(self, grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor] = None,
+                          grad_total: Optional[torch.Tensor] = None, eps: float = 1e-6,
+                          weight_grad_dtype: Optional[torch.dtype] = None, need_weight: bool = True
+                          ) -> Tuple[torch.Tensor, Optional[torch.Tensor]]:
+        """Extension: rms_norm's gradients from that of y and, where the residual stream goes on, of total (grad, grad_total: of x's
+        shape and type). x is what was normalised: the total that the forward call returned, or its x without a residual.
+        grad_x is the gradient of the forward call's x and of its residual both; grad_weight [hidden] is of x's type or, with
+        weight_grad_dtype, torch.float32. Returns (grad_x, grad_weight or None)."""
+        return self.runtime.rms_norm_backward(grad, x, weight, grad_total, eps, weight_grad_dtype, need_weight)
+
+    def quantize_rows(self, x: torch.Tensor, tokens_per_expert: Optional[torch.Tensor] = None, activation: str = "none"
+                      ) -> Tuple[torch.Tensor, torch.Tensor]:
+        """Extension: an activation of rows, in int8: what the second of two int8 products reads. x [rows, width] bf16, fp16 or fp32;
+        activation as expert_linear has it (swiglu: [rows, width / 2]). tokens_per_expert as expert_linear takes it: rows past
+        their sum are neither read nor written. Returns (q int8, scales [rows] fp32), as rms_norm's."""
+        return self.runtime.quantize_rows(x, tokens_per_expert, activation)
+
+    def expert_linear_int8(self, x: torch.Tensor, x_scales: torch.Tensor, weight: torch.Tensor, weight_scales: torch.Tensor,
+                           tokens_per_expert: Optional[torch.Tensor] = None, bias: Optional[torch.Tensor] = None,
+                           activation: str = "none", residual: Optional[torch.Tensor] = None,
+                           out_dtype: torch.dtype = torch.bfloat16, out: Optional[torch.Tensor] = None) -> torch.Tensor:
+        """Extension: the experts' product y = act(x W * weight_scales * x_scales + bias) + residual on rows as an int8 dispatch,
+        rms_norm or quantize_rows leave them. x int8 [rows, k] with x_scales [rows] fp32; weight int8 [experts, n, k], every
+        output channel's k consecutive, with weight_scales [experts, n] fp32 or bf16 (one expert's may leave out the first
+        dimension). tokens_per_expert, activation and out as expert_linear has them. bias [experts, n] fp32 or of y's type (for an
+        fp32 y: fp32 or bf16), residual of y's shape and type; y is of out_dtype: bf16, fp16 or fp32. x W is exact; y is
+        rounded once from 32 bits. Returns y."""
+        return self.runtime.expert_linear_int8(x, x_scales, weight, weight_scales, tokens_per_expert, bias, activation, residual,
+                                               out_dtype, out)
+
     def fused_deep_moe(self, x: torch.Tensor, topk_idx: torch.Tensor, gmm1_permuted_weight: torch.Tensor,
                        gmm1_permuted_weight_scale: torch.Tensor, gmm2_weight: torch.Tensor,
                        gmm2_weight_scale: torch.Tensor, topk_weights: torch.Tensor, num_experts: int,

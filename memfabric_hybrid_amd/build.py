@@ -24,7 +24,7 @@ LIB = os.path.join(LIB_DIR, "libzbal.so")
 TORCH_LIB = os.path.join(LIB_DIR, "_zbal_torch.so")
 ROCM = os.environ.get("ROCM_PATH", "/opt/rocm")
 
-KERNELS = ["layout", "dispatch", "combine", "reduce", "prepack", "gemm", "route", "expert_gemm", "combine_backward"]
+KERNELS = ["layout", "dispatch", "combine", "reduce", "prepack", "gemm", "route", "expert_gemm", "combine_backward", "norm"]
 HOST = ["zbal_runtime", "zbal_registry", "zbal_gpu_communicator", "zbal_c_api", "zbal_amd_operators"]
 
 HIP_FLAGS = [

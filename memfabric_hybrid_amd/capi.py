@@ -105,6 +105,26 @@ class ExpertLinear(ctypes.Structure):
                 ("n", ctypes.c_int64), ("experts", ctypes.c_int64)]
 
 
+class RmsNorm(ctypes.Structure):
+    """zbalhip_rms_norm_t"""
+    _fields_ = [("x", ctypes.c_void_p), ("residual", ctypes.c_void_p), ("weight", ctypes.c_void_p), ("dtype", ctypes.c_int32),
+                ("weight_is_f32", ctypes.c_int32), ("tokens", ctypes.c_int64), ("hidden", ctypes.c_int64), ("eps", ctypes.c_float)]
+
+
+class QuantizeRows(ctypes.Structure):
+    """zbalhip_quantize_rows_t"""
+    _fields_ = [("counts", ctypes.c_void_p), ("counts_are_i64", ctypes.c_int32), ("dtype", ctypes.c_int32), ("activation", ctypes.c_int32),
+                ("rows", ctypes.c_int64), ("width", ctypes.c_int64), ("experts", ctypes.c_int64)]
+
+
+class ExpertLinearInt8(ctypes.Structure):
+    """zbalhip_expert_linear_int8_t"""
+    _fields_ = [("weight", ctypes.c_void_p), ("weight_scales", ctypes.c_void_p), ("weight_scales_are_f32", ctypes.c_int32),
+                ("counts_are_i64", ctypes.c_int32), ("counts", ctypes.c_void_p), ("activation", ctypes.c_int32),
+                ("y_dtype", ctypes.c_int32), ("rows", ctypes.c_int64), ("k", ctypes.c_int64), ("n", ctypes.c_int64),
+                ("experts", ctypes.c_int64)]
+
+
 _TI = ctypes.POINTER(TensorInfo)
 _i64, _i32, _vp, _u16, _u32, _u64 = (ctypes.c_int64, ctypes.c_int32, ctypes.c_void_p, ctypes.c_uint16,
                                      ctypes.c_uint32, ctypes.c_uint64)
@@ -163,6 +183,12 @@ SIGNATURES = {
     "zbal_moe_expert_linear_backward": (_i32, [_TI, _TI, _TI, _TI, _i32, _TI, _TI, _TI, _TI, _TI, _TI, _vp, _vp, _i64]),
     "zbal_moe_expert_linear_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i32, _i32, _i64, _i64]),
     "zbal_combine_normal_backward": (_i32, [_TI, _TI, _TI, _TI, _TI, _TI, _i64, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_rms_norm": (_i32, [_TI, _TI, _TI, ctypes.c_double, _TI, _TI, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_rms_norm_backward": (_i32, [_TI, _TI, _TI, _TI, ctypes.c_double, _TI, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_rms_norm_workspace_size": (_i64, [_i64, _i64]),
+    "zbal_moe_quantize_rows": (_i32, [_TI, _TI, _i32, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_expert_linear_int8": (_i32, [_TI, _TI, _TI, _TI, _TI, _TI, _i32, _TI, _TI, _TI, _vp, _vp, _i64]),
+    "zbal_moe_expert_linear_int8_workspace_size": (_i64, [_i64, _i64, _i64, _i64, _i32]),
     "zbal_moe_weight_prepack": (_i32, [_TI, _TI, _vp, _vp, _i64]),
     # zbal_hip_kernels.h
     "zbalhip_topk_route": (_i32, [_vp, _i64, _i64, _i64, _vp, _i32, _vp, _vp]),
@@ -206,6 +232,12 @@ SIGNATURES = {
     "zbalhip_expert_linear_backward": (_i32, [ctypes.POINTER(ExpertLinear), _vp, _i32, _vp, _vp, _vp, _vp, _vp, _i32, _vp, _vp, _i64,
                                               _vp]),
     "zbalhip_combine_backward": (_i32, [_vp, _vp, _i64, _i32, _vp, _vp, _vp, _i32, _vp, _i64, _i64, _i64, _i64, _vp, _vp, _vp]),
+    "zbalhip_rms_norm": (_i32, [ctypes.POINTER(RmsNorm), _vp, _vp, _vp, _vp, _vp]),
+    "zbalhip_rms_norm_backward_workspace": (_i64, [ctypes.POINTER(RmsNorm)]),
+    "zbalhip_rms_norm_backward": (_i32, [ctypes.POINTER(RmsNorm), _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
+    "zbalhip_quantize_rows": (_i32, [ctypes.POINTER(QuantizeRows), _vp, _vp, _vp, _vp]),
+    "zbalhip_expert_linear_int8_workspace": (_i64, [ctypes.POINTER(ExpertLinearInt8)]),
+    "zbalhip_expert_linear_int8": (_i32, [ctypes.POINTER(ExpertLinearInt8), _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
 }
 
 _lib = None

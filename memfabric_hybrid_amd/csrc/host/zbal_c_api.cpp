@@ -498,3 +498,55 @@ ZBAL_API int32_t zbal_combine_normal_backward(const zbal_tensor_info_t *grad, co
     if (!c) return Z_INVALID_PARAM;
     return c->CombineNormalBackward(grad, srcTokens, srcTokensPerEp, topKWeight, topkIndex, sendTokensIndex, expertNum, gradTokens, gradWeight, stream);
 }
+
+ZBAL_API int32_t zbal_moe_rms_norm(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, const zbal_tensor_info_t *residual, double eps,
+                                   const zbal_tensor_info_t *y, const zbal_tensor_info_t *total, const zbal_tensor_info_t *quantized,
+                                   const zbal_tensor_info_t *scales, zbal_comm_t comm, aclrtStream stream, int64_t)
+{
+    if (!Present("RmsNorm", {{"x", x}})) return Z_INVALID_PARAM;
+    CommunicatorPtr c = Resolve("RmsNorm", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->RmsNorm(x, weight, residual, eps, y, total, quantized, scales, stream);
+}
+
+ZBAL_API int32_t zbal_moe_rms_norm_backward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                            const zbal_tensor_info_t *gradTotal, double eps, const zbal_tensor_info_t *gradX,
+                                            const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *workspace, zbal_comm_t comm,
+                                            aclrtStream stream, int64_t)
+{
+    if (!Present("RmsNormBackward", {{"grad", grad}, {"x", x}, {"gradX", gradX}})) return Z_INVALID_PARAM;
+    CommunicatorPtr c = Resolve("RmsNormBackward", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->RmsNormBackward(grad, x, weight, gradTotal, eps, gradX, gradWeight, workspace, stream);
+}
+
+ZBAL_API int64_t zbal_moe_rms_norm_workspace_size(int64_t tokens, int64_t hidden) { return RmsNormWorkspaceBytes(tokens, hidden); }
+
+ZBAL_API int32_t zbal_moe_quantize_rows(const zbal_tensor_info_t *x, const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation,
+                                        const zbal_tensor_info_t *quantized, const zbal_tensor_info_t *scales, zbal_comm_t comm,
+                                        aclrtStream stream, int64_t)
+{
+    if (!Present("QuantizeRows", {{"x", x}, {"quantized", quantized}, {"scales", scales}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(activation >= 0 && activation < ZBAL_ACTIVATION_BUTT, "QuantizeRows failed as activation " << activation << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("QuantizeRows", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->QuantizeRows(x, tokensPerExpert, activation, quantized, scales, stream);
+}
+
+ZBAL_API int32_t zbal_moe_expert_linear_int8(const zbal_tensor_info_t *x, const zbal_tensor_info_t *xScales, const zbal_tensor_info_t *weight,
+                                             const zbal_tensor_info_t *weightScales, const zbal_tensor_info_t *tokensPerExpert,
+                                             const zbal_tensor_info_t *bias, zbal_activation_t activation, const zbal_tensor_info_t *residual,
+                                             const zbal_tensor_info_t *y, const zbal_tensor_info_t *workspace, zbal_comm_t comm,
+                                             aclrtStream stream, int64_t)
+{
+    if (!Present("ExpertLinearInt8", {{"x", x}, {"xScales", xScales}, {"weight", weight}, {"weightScales", weightScales}, {"y", y}})) return Z_INVALID_PARAM;
+    ZBAL_VALIDATE_RETURN(activation >= 0 && activation < ZBAL_ACTIVATION_BUTT, "ExpertLinearInt8 failed as activation " << activation << " is invalid", Z_INVALID_PARAM);
+    CommunicatorPtr c = Resolve("ExpertLinearInt8", comm);
+    if (!c) return Z_INVALID_PARAM;
+    return c->ExpertLinearInt8(x, xScales, weight, weightScales, tokensPerExpert, bias, activation, residual, y, workspace, stream);
+}
+
+ZBAL_API int64_t zbal_moe_expert_linear_int8_workspace_size(int64_t rows, int64_t k, int64_t n, int64_t expertNum, zbal_activation_t activation)
+{
+    return ExpertLinearInt8WorkspaceBytes(rows, k, n, expertNum, activation);
+}

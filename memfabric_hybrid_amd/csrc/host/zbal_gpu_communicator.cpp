@@ -14,6 +14,7 @@
  * owns all experts.
  */
 #include <algorithm>
+#include <cmath>
 #include <cstdlib>
 #include <cstring>
 #include <ctime>
@@ -955,7 +956,14 @@ public:
                                                          topkIndex->dataType == ZBAL_DATA_TYPE_INT64, gradLogits->data, stream));
     }
 
-    /* the operands that both directions of the experts' products share */
+    static bool HalfPrecision(const char *op, const zbal_tensor_info_t *x)
+    {
+        ZBAL_VALIDATE_RETURN(x->dataType == ZBAL_DATA_TYPE_BFP16 || x->dataType == ZBAL_DATA_TYPE_FP16,
+                             op << " failed as x has type " << DtName(x->dataType) << ", expected bf16 or fp16", false);
+        return true;
+    }
+
+    /* the operands that the experts' products share, in both directions and in int8 */
     bool ExpertLinearOperands(const char *op, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
                               const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation, zbalhip_expert_linear_t *d)
     {
@@ -977,8 +985,6 @@ public:
                              op << " failed as rows " << d->rows << ", k " << d->k << " and n " << d->n << " are out of range", false);
         ZBAL_VALIDATE_RETURN(x->shape[1] == d->k, op << " failed as x has " << x->shape[1] << " columns, weight takes " << d->k, false);
         ZBAL_VALIDATE_RETURN(activation != ZBAL_ACTIVATION_SWIGLU || d->n % 2 == 0, op << " failed as swiglu needs an even n, got " << d->n, false);
-        ZBAL_VALIDATE_RETURN(x->dataType == ZBAL_DATA_TYPE_BFP16 || x->dataType == ZBAL_DATA_TYPE_FP16,
-                             op << " failed as x has type " << DtName(x->dataType) << ", expected bf16 or fp16", false);
         if (d->rows > 0 && !CheckTensor(op, "x", x, x->dataType, x->dataType, d->rows * d->k)) return false;
         if (!CheckTensor(op, "weight", weight, x->dataType, x->dataType, d->experts * d->k * d->n)) return false;
         d->weight = weight->data;
@@ -1024,7 +1030,7 @@ public:
     {
         const char *op = "ExpertLinear";
         zbalhip_expert_linear_t d = {};
-        if (!ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
+        if (!HalfPrecision(op, x) || !ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
         if (d.rows == 0) return Z_OK;
         const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.n / 2 : d.n;
         ZB_CHECK(op, "y", y, x->dataType, ZBAL_DATA_TYPE_FP32, d.rows * cols);
@@ -1050,7 +1056,7 @@ public:
     {
         const char *op = "ExpertLinearBackward";
         zbalhip_expert_linear_t d = {};
-        if (!ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
+        if (!HalfPrecision(op, x) || !ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &d)) return Z_INVALID_PARAM;
         const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.n / 2 : d.n;
         const bool rounds = activation != ZBAL_ACTIVATION_NONE || grad->dataType != x->dataType;
         if (d.rows > 0) {
@@ -1115,6 +1121,143 @@ public:
                                                      (float *)gradWeight->data, stream));
     }
 
+    /* what both directions of the norm share */
+    bool NormOperands(const char *op, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, double eps, zbalhip_rms_norm_t *d)
+    {
+        ZBAL_VALIDATE_RETURN(x->dim == 2, op << " failed as x must be [tokens, hidden]", false);
+        d->tokens = x->shape[0];
+        d->hidden = x->shape[1];
+        d->dtype = x->dataType;
+        d->eps = (float)eps;
+        ZBAL_VALIDATE_RETURN(d->hidden > 0 && d->hidden <= ZBALHIP_EXPERT_MAX_WIDTH && d->tokens <= ZBALHIP_EXPERT_MAX_ROWS,
+                             op << " failed as tokens " << d->tokens << " and hidden " << d->hidden << " are out of range", false);
+        ZBAL_VALIDATE_RETURN(d->eps > 0.0f && std::isfinite(d->eps), op << " failed as eps " << eps << " is not a positive number of 32 bits", false);
+        if (d->tokens > 0 && !CheckRouteLogits(op, "x", x, d->tokens * d->hidden)) return false;
+        if (Given(weight)) {
+            if (!CheckTensor(op, "weight", weight, x->dataType, ZBAL_DATA_TYPE_FP32, d->hidden)) return false;
+            d->weight = weight->data;
+            d->weight_is_f32 = weight->dataType == ZBAL_DATA_TYPE_FP32;
+        }
+        d->x = x->data;
+        return true;
+    }
+
+    int32_t RmsNorm(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, const zbal_tensor_info_t *residual, double eps,
+                    const zbal_tensor_info_t *y, const zbal_tensor_info_t *total, const zbal_tensor_info_t *quantized,
+                    const zbal_tensor_info_t *scales, aclrtStream stream) override
+    {
+        const char *op = "RmsNorm";
+        zbalhip_rms_norm_t d = {};
+        if (!NormOperands(op, x, weight, eps, &d)) return Z_INVALID_PARAM;
+        if (d.tokens == 0) return Z_OK;
+        const int64_t n = d.tokens * d.hidden;
+        if (Given(residual)) ZB_CHECK(op, "residual", residual, x->dataType, x->dataType, n);
+        if (Given(y)) ZB_CHECK(op, "y", y, x->dataType, x->dataType, n);
+        if (Given(total)) ZB_CHECK(op, "total", total, x->dataType, x->dataType, n);
+        if (Given(quantized)) {
+            ZB_CHECK(op, "quantized", quantized, ZBAL_DATA_TYPE_INT8, ZBAL_DATA_TYPE_INT8, n);
+            ZBAL_VALIDATE_RETURN(scales != nullptr, op << " failed as scales is null", Z_INVALID_PARAM);
+            ZB_CHECK(op, "scales", scales, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, d.tokens);
+        }
+        ZBAL_VALIDATE_RETURN(Given(y) || Given(total) || Given(quantized), op << " failed as no output is asked for", Z_INVALID_PARAM);
+        d.residual = Given(residual) ? residual->data : nullptr;
+        /* the sum in place is all right: every element is read by the lane that writes it */
+        const bool on_x = Given(total) && total->data == x->data, on_residual = Given(total) && Given(residual) && total->data == residual->data;
+        if (!Apart(op, {{"y", y}, {"quantized", quantized}, {"scales", Given(quantized) ? scales : nullptr}},
+                   {{"x", x}, {"weight", weight}, {"residual", residual}, {"total", total}}) ||
+            !Apart(op, {{"total", total}}, {{"x", on_x ? nullptr : x}, {"residual", on_residual ? nullptr : residual}, {"weight", weight}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_rms_norm(&d, Given(y) ? y->data : nullptr, Given(total) ? total->data : nullptr,
+                                             Given(quantized) ? (int8_t *)quantized->data : nullptr, Given(quantized) ? (float *)scales->data : nullptr, stream));
+    }
+
+    int32_t RmsNormBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                            const zbal_tensor_info_t *gradTotal, double eps, const zbal_tensor_info_t *gradX,
+                            const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *workspace, aclrtStream stream) override
+    {
+        const char *op = "RmsNormBackward";
+        zbalhip_rms_norm_t d = {};
+        if (!NormOperands(op, x, weight, eps, &d)) return Z_INVALID_PARAM;
+        const int64_t n = d.tokens * d.hidden;
+        if (d.tokens > 0) {
+            ZB_CHECK(op, "grad", grad, x->dataType, x->dataType, n);
+            ZB_CHECK(op, "gradX", gradX, x->dataType, x->dataType, n);
+            if (Given(gradTotal)) ZB_CHECK(op, "gradTotal", gradTotal, x->dataType, x->dataType, n);
+        }
+        if (Given(gradWeight)) ZB_CHECK(op, "gradWeight", gradWeight, x->dataType, ZBAL_DATA_TYPE_FP32, d.hidden);
+        if (Given(workspace)) ZB_CHECK(op, "workspace", workspace, workspace->dataType, workspace->dataType, 0);
+        const int64_t bytes = Given(workspace) ? Numel(workspace) * (int64_t)ElemSize(workspace->dataType) : 0;
+        ZBAL_VALIDATE_RETURN(!Given(gradWeight) || d.tokens == 0 || bytes >= zbalhip_rms_norm_backward_workspace(&d),
+                             op << " failed as workspace holds " << bytes << " bytes, needs " << zbalhip_rms_norm_backward_workspace(&d), Z_INVALID_PARAM);
+        if (d.tokens == 0 && !Given(gradWeight)) return Z_OK;
+        if (!Apart(op, {{"gradX", gradX}, {"gradWeight", gradWeight}, {"workspace", workspace}}, {{"grad", grad}, {"x", x}, {"weight", weight}, {"gradTotal", gradTotal}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_rms_norm_backward(&d, grad->data, Given(gradTotal) ? gradTotal->data : nullptr, gradX->data,
+                                                      Given(gradWeight) ? gradWeight->data : nullptr, Given(gradWeight) && gradWeight->dataType == ZBAL_DATA_TYPE_FP32,
+                                                      Given(workspace) ? workspace->data : nullptr, bytes, stream));
+    }
+
+    int32_t QuantizeRows(const zbal_tensor_info_t *x, const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation,
+                         const zbal_tensor_info_t *quantized, const zbal_tensor_info_t *scales, aclrtStream stream) override
+    {
+        const char *op = "QuantizeRows";
+        ZBAL_VALIDATE_RETURN(x->dim == 2, op << " failed as x must be [rows, width]", Z_INVALID_PARAM);
+        zbalhip_quantize_rows_t d = {};
+        d.dtype = x->dataType;
+        d.activation = activation;
+        d.rows = x->shape[0];
+        d.width = x->shape[1];
+        ZBAL_VALIDATE_RETURN(d.width > 0 && d.width <= ZBALHIP_EXPERT_MAX_WIDTH && d.rows <= ZBALHIP_EXPERT_MAX_ROWS,
+                             op << " failed as rows " << d.rows << " and width " << d.width << " are out of range", Z_INVALID_PARAM);
+        ZBAL_VALIDATE_RETURN(activation != ZBAL_ACTIVATION_SWIGLU || d.width % 2 == 0, op << " failed as swiglu needs an even width, got " << d.width, Z_INVALID_PARAM);
+        if (Given(tokensPerExpert)) {
+            d.experts = Numel(tokensPerExpert);
+            ZBAL_VALIDATE_RETURN(d.experts > 0 && d.experts <= 1024, op << " failed as experts " << d.experts << " is out of range", Z_INVALID_PARAM);
+            ZB_CHECK(op, "tokensPerExpert", tokensPerExpert, ZBAL_DATA_TYPE_INT32, ZBAL_DATA_TYPE_INT64, d.experts);
+            d.counts = tokensPerExpert->data;
+            d.counts_are_i64 = tokensPerExpert->dataType == ZBAL_DATA_TYPE_INT64;
+        }
+        if (d.rows == 0) return Z_OK;
+        const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.width / 2 : d.width;
+        if (!CheckRouteLogits(op, "x", x, d.rows * d.width)) return Z_INVALID_PARAM;
+        ZB_CHECK(op, "quantized", quantized, ZBAL_DATA_TYPE_INT8, ZBAL_DATA_TYPE_INT8, d.rows * cols);
+        ZB_CHECK(op, "scales", scales, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, d.rows);
+        if (!Apart(op, {{"quantized", quantized}, {"scales", scales}}, {{"x", x}, {"tokensPerExpert", tokensPerExpert}})) return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_quantize_rows(&d, x->data, (int8_t *)quantized->data, (float *)scales->data, stream));
+    }
+
+    int32_t ExpertLinearInt8(const zbal_tensor_info_t *x, const zbal_tensor_info_t *xScales, const zbal_tensor_info_t *weight,
+                             const zbal_tensor_info_t *weightScales, const zbal_tensor_info_t *tokensPerExpert, const zbal_tensor_info_t *bias,
+                             zbal_activation_t activation, const zbal_tensor_info_t *residual, const zbal_tensor_info_t *y,
+                             const zbal_tensor_info_t *workspace, aclrtStream stream) override
+    {
+        const char *op = "ExpertLinearInt8";
+        zbalhip_expert_linear_t shape = {};
+        ZBAL_VALIDATE_RETURN(weight->reserved[0] == ZBAL_WEIGHT_FORMAT_NK, op << " failed as weight has format " << weight->reserved[0] << ", expected [experts, n, k]",
+                             Z_INVALID_PARAM);
+        ZBAL_VALIDATE_RETURN(x->dataType == ZBAL_DATA_TYPE_INT8, op << " failed as x has type " << DtName(x->dataType) << ", expected int8", Z_INVALID_PARAM);
+        if (!ExpertLinearOperands(op, x, weight, tokensPerExpert, activation, &shape)) return Z_INVALID_PARAM;
+        const zbalhip_expert_linear_int8_t d = {shape.weight, weightScales->data, weightScales->dataType == ZBAL_DATA_TYPE_FP32, shape.counts_are_i64, shape.counts,
+                                                activation, y->dataType, shape.rows, shape.k, shape.n, shape.experts};
+        ZB_CHECK(op, "weightScales", weightScales, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_BFP16, d.experts * d.n);
+        if (d.rows == 0) return Z_OK;
+        const int64_t cols = activation == ZBAL_ACTIVATION_SWIGLU ? d.n / 2 : d.n;
+        ZB_CHECK(op, "xScales", xScales, ZBAL_DATA_TYPE_FP32, ZBAL_DATA_TYPE_FP32, d.rows);
+        if (!CheckRouteLogits(op, "y", y, d.rows * cols)) return Z_INVALID_PARAM;
+        if (Given(bias)) ZB_CHECK(op, "bias", bias, y->dataType == ZBAL_DATA_TYPE_FP32 ? ZBAL_DATA_TYPE_BFP16 : y->dataType, ZBAL_DATA_TYPE_FP32, d.experts * d.n);
+        if (Given(residual)) ZB_CHECK(op, "residual", residual, y->dataType, y->dataType, d.rows * cols);
+        if (Given(workspace)) ZB_CHECK(op, "workspace", workspace, workspace->dataType, workspace->dataType, 0);
+        /* in place is all right for the residual: every element is read by the lane that writes it */
+        const zbal_tensor_info_t *apart = Given(residual) && residual->data != y->data ? residual : nullptr;
+        if (!Apart(op, {{"y", y}, {"workspace", workspace}},
+                   {{"x", x}, {"xScales", xScales}, {"weight", weight}, {"weightScales", weightScales}, {"tokensPerExpert", tokensPerExpert}, {"bias", bias}, {"residual", apart}}))
+            return Z_INVALID_PARAM;
+        return Launched(op, zbalhip_expert_linear_int8(&d, x->data, (const float *)xScales->data, Given(bias) ? bias->data : nullptr,
+                                                       Given(bias) && bias->dataType == ZBAL_DATA_TYPE_FP32, Given(residual) ? residual->data : nullptr, y->data,
+                                                       Given(workspace) ? workspace->data : nullptr,
+                                                       Given(workspace) ? Numel(workspace) * (int64_t)ElemSize(workspace->dataType) : 0, stream));
+    }
+
     int32_t WeightPrepack(const zbal_tensor_info_t *src, const zbal_tensor_info_t *dst, aclrtStream stream, int64_t) override
     {
         const char *op = "WeightPrepack";
@@ -1146,6 +1289,28 @@ int64_t ExpertLinearWorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t e
     d.n = n;
     d.experts = experts;
     return zbalhip_expert_linear_workspace(&d, backward);
+}
+
+int64_t RmsNormWorkspaceBytes(int64_t tokens, int64_t hidden)
+{
+    zbalhip_rms_norm_t d = {};
+    d.dtype = ZBAL_DATA_TYPE_BFP16;
+    d.eps = 1.0f;
+    d.tokens = tokens;
+    d.hidden = hidden;
+    return zbalhip_rms_norm_backward_workspace(&d);
+}
+
+int64_t ExpertLinearInt8WorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t experts, zbal_activation_t activation)
+{
+    zbalhip_expert_linear_int8_t d = {};
+    d.y_dtype = ZBAL_DATA_TYPE_BFP16;
+    d.activation = activation;
+    d.rows = rows;
+    d.k = k;
+    d.n = n;
+    d.experts = experts;
+    return zbalhip_expert_linear_int8_workspace(&d);
 }
 
 CommunicatorPtr MakeGpuCommunicator(const GroupInfo &info) { return std::make_shared<GpuCommunicator>(info); }

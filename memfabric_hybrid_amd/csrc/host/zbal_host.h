@@ -228,6 +228,18 @@ public:
                                           const zbal_tensor_info_t *topkIndex, const zbal_tensor_info_t *sendTokensIndex,
                                           int64_t expertNum, const zbal_tensor_info_t *gradTokens,
                                           const zbal_tensor_info_t *gradWeight, aclrtStream stream) = 0;
+    virtual int32_t RmsNorm(const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight, const zbal_tensor_info_t *residual, double eps,
+                            const zbal_tensor_info_t *y, const zbal_tensor_info_t *total, const zbal_tensor_info_t *quantized,
+                            const zbal_tensor_info_t *scales, aclrtStream stream) = 0;
+    virtual int32_t RmsNormBackward(const zbal_tensor_info_t *grad, const zbal_tensor_info_t *x, const zbal_tensor_info_t *weight,
+                                    const zbal_tensor_info_t *gradTotal, double eps, const zbal_tensor_info_t *gradX,
+                                    const zbal_tensor_info_t *gradWeight, const zbal_tensor_info_t *workspace, aclrtStream stream) = 0;
+    virtual int32_t QuantizeRows(const zbal_tensor_info_t *x, const zbal_tensor_info_t *tokensPerExpert, zbal_activation_t activation,
+                                 const zbal_tensor_info_t *quantized, const zbal_tensor_info_t *scales, aclrtStream stream) = 0;
+    virtual int32_t ExpertLinearInt8(const zbal_tensor_info_t *x, const zbal_tensor_info_t *xScales, const zbal_tensor_info_t *weight,
+                                     const zbal_tensor_info_t *weightScales, const zbal_tensor_info_t *tokensPerExpert,
+                                     const zbal_tensor_info_t *bias, zbal_activation_t activation, const zbal_tensor_info_t *residual,
+                                     const zbal_tensor_info_t *y, const zbal_tensor_info_t *workspace, aclrtStream stream) = 0;
     virtual int32_t WeightPrepack(const zbal_tensor_info_t *src, const zbal_tensor_info_t *dst, aclrtStream stream,
                                   int64_t flags) = 0;
 
@@ -290,6 +302,8 @@ uint64_t FusedWorkspaceBytes(int64_t tokens, int64_t hidden, int64_t topk, int64
 /* bytes of workspace of the experts' products, or -1 */
 int64_t ExpertLinearWorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t experts, zbal_activation_t activation,
                                    zbal_datatype_t dataType, int64_t weightFormat, bool backward);
+int64_t RmsNormWorkspaceBytes(int64_t tokens, int64_t hidden);
+int64_t ExpertLinearInt8WorkspaceBytes(int64_t rows, int64_t k, int64_t n, int64_t experts, zbal_activation_t activation);
 
 } // namespace zbal
 

@@ -83,6 +83,15 @@ public:
     int32_t CombineNormalBackward(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
                                   const zbal_tensor_info_t *, const zbal_tensor_info_t *, int64_t, const zbal_tensor_info_t *,
                                   const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t RmsNorm(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, double, const zbal_tensor_info_t *,
+                    const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t RmsNormBackward(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, double,
+                            const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t QuantizeRows(const zbal_tensor_info_t *, const zbal_tensor_info_t *, zbal_activation_t, const zbal_tensor_info_t *,
+                         const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
+    int32_t ExpertLinearInt8(const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *, const zbal_tensor_info_t *,
+                             const zbal_tensor_info_t *, const zbal_tensor_info_t *, zbal_activation_t, const zbal_tensor_info_t *,
+                             const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream) override { return Z_OK; }
     int32_t WeightPrepack(const zbal_tensor_info_t *, const zbal_tensor_info_t *, aclrtStream, int64_t) override { return Z_OK; }
 };
 

@@ -1,6 +1,6 @@
 /*
- * The experts' products in half precision: rows sorted by expert times the experts' weights, with bias, activation and residual
- * in the epilogue, and the gradients of the rows, the weights, the bias and the pre-activation.
+ * The experts' products in half precision and in int8: rows sorted by expert times the experts' weights, with bias, activation and residual
+ * in the epilogue, and half precision's gradients of the rows, the weights, the bias and the pre-activation.
  */
 #include <cmath>
 
@@ -9,9 +9,14 @@
 
 namespace {
 
+typedef u32x4 __attribute__((aligned(1))) x_loose1_t;
+typedef u32x4 __attribute__((aligned(2))) x_loose2_t;
+__device__ __forceinline__ u32x4 x_loose(const uint8_t *p) { return *reinterpret_cast<const x_loose1_t *>(p); }
+__device__ __forceinline__ u32x4 x_loose(const uint16_t *p) { return *reinterpret_cast<const x_loose2_t *>(p); }
+
 /*
- * Any sizes: operands pass through registers, sixteen bytes at a time from wherever they start (two bytes' alignment), the last
- * elements of a row or column one by one.
+ * Any sizes: operands pass through registers, sixteen bytes at a time from wherever they start (an element's alignment), the last
+ * elements of a row or column one by one. Elements of int8 are counted one by one here.
  */
 template <int DT, bool REDUCE, bool B_TR, int TM, int TN, int WM, int WN, bool SHORT>
 __global__ void __launch_bounds__(WM * WN * 64)
@@ -25,7 +30,9 @@ expert_gemm_any_kernel(XgemmParams p)
     uint8_t *lds_a = lds, *lds_b = lds + TM * 128;
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave / WN, wn = wave % WN;
-    typedef u32x4 __attribute__((aligned(2))) loose_t;
+    constexpr int SIZE = x_is_i8<DT> ? 1 : 2, CHUNK = 16 / SIZE, BK = XBK * 2 / SIZE;      /* bytes of an element, elements of a piece and k of a step */
+    static_assert(SIZE == 2 || (!REDUCE && !B_TR), "int8 has consecutive k");
+    typedef std::conditional_t<SIZE == 1, uint8_t, uint16_t> element_t;
 
     const int cols = p.n_half ? p.n_half : p.N, tile_cols = p.n_half ? TN / 2 : TN, n_tiles = (cols + tile_cols - 1) / tile_cols;
     int expert, m0, m_end, n0, k_begin, k_end;
@@ -51,12 +58,12 @@ expert_gemm_any_kernel(XgemmParams p)
         k_end = p.K;
     }
     if (p.splits > 1) {          /* whole steps for everyone, in order */
-        const int steps = (k_end - k_begin + XBK - 1) / XBK, each = (steps + p.splits - 1) / p.splits;
-        const int from = k_begin + split * each * XBK;
-        k_end = k_end - from > each * XBK ? from + each * XBK : k_end;
+        const int steps = (k_end - k_begin + BK - 1) / BK, each = (steps + p.splits - 1) / p.splits;
+        const int from = k_begin + split * each * BK;
+        k_end = k_end - from > each * BK ? from + each * BK : k_end;
         k_begin = from < k_end ? from : k_end;
     }
-    const uint16_t *b = p.b + (REDUCE ? 0 : expert * p.b_stride);
+    const element_t *a = reinterpret_cast<const element_t *>(p.a), *b = reinterpret_cast<const element_t *>(p.b) + (REDUCE ? 0 : expert * p.b_stride);
 
     /* tile column -> column of B; columns past the end of their half are none */
     auto b_col = [&](int c, int *end) __attribute__((always_inline)) {
@@ -65,36 +72,36 @@ expert_gemm_any_kernel(XgemmParams p)
         return c < TN / 2 ? n0 + c : p.n_half + n0 + c - TN / 2;
     };
     /*
-     * Eight elements from column `col` of a row: a piece that ends past `end` is taken from its last eight and shifted, so that all loads are alike
+     * Eight elements (int8: sixteen) from column `col` of a row: a piece that ends past `end` is taken from its last eight and shifted, so that all loads are alike
      * and under way together (one by one, the last columns' tiles took twice as long as the others: 1021 x 1001 x 1531 in 64 x 64, with gelu, bias and residual, 27 us, 41).
      */
-    struct Piece { u32x4 v; int away; };         /* elements to shift out; eight: nothing is left */
-    auto eight = [&](const uint16_t *row, int col, int end, bool there) __attribute__((always_inline)) -> Piece {
+    struct Piece { u32x4 v; int away; };         /* elements to shift out; all of them: nothing is left */
+    auto eight = [&](const element_t *row, int col, int end, bool there) __attribute__((always_inline)) -> Piece {
         if constexpr (SHORT) {
             u32x4 v = {0, 0, 0, 0};
-            for (int i = 0; there && i < 8 && col + i < end; ++i) v[i >> 1] |= (uint32_t)row[col + i] << ((i & 1) * 16);
+            for (int i = 0; there && i < CHUNK && col + i < end; ++i) v[i * SIZE >> 2] |= (uint32_t)row[col + i] << ((i * SIZE & 3) * 8);
             return {v, 0};
         } else {
-            const int from = col < end - 8 ? col : end - 8, away = col - from;
-            return {*reinterpret_cast<const loose_t *>(row + from), !there || away > 8 ? 8 : away};
+            const int from = col < end - CHUNK ? col : end - CHUNK, away = col - from;
+            return {x_loose(row + from), !there || away > CHUNK ? CHUNK : away};
         }
     };
     auto shifted = [&](const Piece &c) __attribute__((always_inline)) -> u32x4 {
         if (c.away == 0) return c.v;
-        const int bits = (c.away & 3) * 16;
+        const int bits = (c.away & (CHUNK / 2 - 1)) * (SIZE * 8);
         uint64_t lo = (uint64_t)c.v[1] << 32 | c.v[0], hi = (uint64_t)c.v[3] << 32 | c.v[2];
-        if (c.away >= 4) { lo = hi; hi = 0; }
-        if (c.away >= 8) lo = 0;
+        if (c.away >= CHUNK / 2) { lo = hi; hi = 0; }
+        if (c.away >= CHUNK) lo = 0;
         if (bits) { lo = lo >> bits | hi << (64 - bits); hi >>= bits; }
         return u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
     };
     auto load_a = [&](int c, int k0) __attribute__((always_inline)) -> Piece {
         if constexpr (REDUCE) {
             const int k = k0 + c / (TM / 8), m = m0 + c % (TM / 8) * 8;
-            return eight(p.a + (int64_t)(k < k_end ? k : k_end - 1) * p.lda, m, m_end, k < k_end);
+            return eight(a + (int64_t)(k < k_end ? k : k_end - 1) * p.lda, m, m_end, k < k_end);
         } else {
-            const int row = m0 + (c >> 3), k = k0 + (c & 7) * 8;
-            return eight(p.a + (int64_t)(row < m_end ? row : m_end - 1) * p.lda, k, k_end, row < m_end);
+            const int row = m0 + (c >> 3), k = k0 + (c & 7) * CHUNK;
+            return eight(a + (int64_t)(row < m_end ? row : m_end - 1) * p.lda, k, k_end, row < m_end);
         }
     };
     auto load_b = [&](int c, int k0) __attribute__((always_inline)) -> Piece {
@@ -103,17 +110,17 @@ expert_gemm_any_kernel(XgemmParams p)
             const int k = k0 + c / (TN / 8), n = b_col(c % (TN / 8) * 8, &end);
             return eight(b + (int64_t)(k < k_end ? k : k_end - 1) * p.ldb, n, end, k < k_end);
         } else {
-            const int n = b_col(c >> 3, &end), k = k0 + (c & 7) * 8;
+            const int n = b_col(c >> 3, &end), k = k0 + (c & 7) * CHUNK;
             return eight(b + (int64_t)(n < end ? n : end - 1) * p.ldb, k, k_end, n < end);
         }
     };
 
-    f32x4 acc[MT][NT], bias_acc[REDUCE ? (MT > NT ? MT : NT) : 1];
+    x_sums_t<DT> acc[MT][NT], bias_acc[REDUCE ? (MT > NT ? MT : NT) : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (auto &v : bias_acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = x_sums_t<DT>{0, 0, 0, 0};
+    for (auto &v : bias_acc) v = x_sums_t<DT>{0, 0, 0, 0};
     /* the tiles of the other operand's first columns sum this one's, as a product with ones */
     const bool bias_b = REDUCE && p.bias_side == 1 && m0 == 0 && wm == 0, bias_a = REDUCE && p.bias_side == 2 && n0 == 0 && wn == 0;
     const uint32_t one2 = DT == ZDT_BF16 ? 0x3f803f80u : 0x3c003c00u;
@@ -144,7 +151,7 @@ expert_gemm_any_kernel(XgemmParams p)
             *reinterpret_cast<u32x4 *>(lds_b + (REDUCE || B_TR ? tr_at<TN>(c / (TN / 8), c % (TN / 8)) : kc_at(c >> 3, c & 7))) = shifted(pb[i]);
         }
         __syncthreads();
-        fetch(pa, pb, k0 + AHEAD * XBK);          /* past the end: the last pieces again, and none of them used */
+        fetch(pa, pb, k0 + AHEAD * BK);          /* past the end: the last pieces again, and none of them used */
 #pragma unroll
         for (int s = 0; s < 2; ++s) {
             u32x4 fa[MT];
@@ -167,11 +174,11 @@ expert_gemm_any_kernel(XgemmParams p)
     };
     if (k_begin < k_end) {
 #pragma unroll
-        for (int i = 0; i < AHEAD; ++i) fetch(ra[i], rb[i], k_begin + i * XBK);
-        for (int k0 = k_begin; k0 < k_end; k0 += AHEAD * XBK)
+        for (int i = 0; i < AHEAD; ++i) fetch(ra[i], rb[i], k_begin + i * BK);
+        for (int k0 = k_begin; k0 < k_end; k0 += AHEAD * BK)
 #pragma unroll
             for (int i = 0; i < AHEAD; ++i)
-                if (k0 + i * XBK < k_end) step(ra[i], rb[i], k0 + i * XBK);
+                if (k0 + i * BK < k_end) step(ra[i], rb[i], k0 + i * BK);
     }
 
     /* a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile */
@@ -196,7 +203,7 @@ expert_gemm_any_kernel(XgemmParams p)
      */
     constexpr int LD = TN + 1, ROWS = WM * 16;
     static_assert(ROWS * LD * 4 <= (TM + TN) * 128, "sums fit the operands' place");
-    float *sums = reinterpret_cast<float *>(lds);
+    x_sum_t<DT> *sums = reinterpret_cast<x_sum_t<DT> *>(lds);
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt) {
         __syncthreads();
@@ -213,10 +220,11 @@ expert_gemm_any_kernel(XgemmParams p)
             const bool up = p.n_half && c >= TN / 2;
             const int j = n0 + (up ? c - TN / 2 : c);
             if (row >= m_end || j >= cols) continue;
-            const float z = sums[r * LD + c];
-            if (p.splits > 1) p.partial[((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + (up ? p.n_half : 0)] = z;
+            const x_sum_t<DT> z = sums[r * LD + c];
+            if (p.splits > 1) reinterpret_cast<x_sum_t<DT> *>(p.partial)[((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + (up ? p.n_half : 0)] = z;
             else if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, expert * p.out_stride + row * p.ldo + j, z);
-            else if (!up) x_finish<DT>(p, expert, row, j, z, p.n_half ? sums[r * LD + TN / 2 + c] : 0.0f);
+            else if (!up)
+                x_finish<DT>(p, expert, row, j, x_scaled<DT>(p, expert, row, j, z), p.n_half ? x_scaled<DT>(p, expert, row, p.n_half + j, sums[r * LD + TN / 2 + c]) : 0.0f);
         }
     }
 }
@@ -232,24 +240,24 @@ expert_join_kernel(XgemmParams p)
     const bool whole = p.ldo % 4 == 0 && p.N % 4 == 0 && p.n_half % 4 == 0;
     for (int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x; i < total; i += (int64_t)gridDim.x * blockDim.x) {
         const int row = (int)(i / quads), j = (int)(i - (int64_t)row * quads) * 4;
-        const float *from = p.partial + (int64_t)row * p.ldp + j;
-        f32x4 z = {0.0f, 0.0f, 0.0f, 0.0f}, up = z;
+        const x_sum_t<DT> *from = reinterpret_cast<const x_sum_t<DT> *>(p.partial) + (int64_t)row * p.ldp + j;
+        x_sums_t<DT> z = {0, 0, 0, 0}, up = z;
         if (whole) {
             for (int s = 0; s < p.splits; ++s) {
-                z += *reinterpret_cast<const f32x4 *>(from + s * plane);
-                if (p.n_half) up += *reinterpret_cast<const f32x4 *>(from + s * plane + p.n_half);
+                z += *reinterpret_cast<const x_sums_t<DT> *>(from + s * plane);
+                if (p.n_half) up += *reinterpret_cast<const x_sums_t<DT> *>(from + s * plane + p.n_half);
             }
             if constexpr (REDUCE) x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, z);
-            else x_finish4<DT>(p, 0, row, j, z, up);
+            else x_finish4<DT>(p, 0, row, j, x_scaled4<DT>(p, 0, row, j, z), p.n_half ? x_scaled4<DT>(p, 0, row, p.n_half + j, up) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
         } else {
             for (int c = 0; c < 4 && j + c < cols; ++c) {
-                float zc = 0.0f, uc = 0.0f;
+                x_sum_t<DT> zc = 0, uc = 0;
                 for (int s = 0; s < p.splits; ++s) {
                     zc += from[s * plane + c];
                     if (p.n_half) uc += from[s * plane + p.n_half + c];
                 }
                 if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, row * p.ldo + j + c, zc);
-                else x_finish<DT>(p, 0, row, j + c, zc, uc);
+                else x_finish<DT>(p, 0, row, j + c, x_scaled<DT>(p, 0, row, j + c, zc), p.n_half ? x_scaled<DT>(p, 0, row, p.n_half + j + c, uc) : 0.0f);
             }
         }
     }
@@ -479,6 +487,11 @@ template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, voi
         p.bias_partial = p.partial + (int64_t)p.splits * (REDUCE ? p.M : p.rows) * p.ldp;
         p.bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
     }
+    if constexpr (x_is_i8<DT>)
+        if (plan.cut == CUT_ANY || plan.cut == CUT_ANY_64 || plan.cut == CUT_ANY_16 || plan.cut == CUT_SHORT) {
+            p.lda = p.ldb = p.K = p.k_bytes;
+            p.b_stride = (int64_t)p.k_bytes * p.N;
+        }
     switch (plan.cut) {
         case CUT_WIDE: launch_wide<DT, REDUCE, B_TR>(p, st); break;
         case CUT_128: launch_direct<DT, REDUCE, B_TR, 128, 128, 2, 4, 4>(p, st); break;
@@ -516,16 +529,20 @@ template <bool REDUCE> void launch_types(const XgemmParams &p, int dtype, bool b
     }
 }
 
-bool linear_sizes_ok(const zbalhip_expert_linear_t *d)
+template <typename D> bool sizes_ok(const D *d)
 {
     if (!d || d->rows < 0 || d->k <= 0 || d->n <= 0 || d->experts <= 0 || d->experts > 1024) return false;
-    if (d->dtype != ZDT_BF16 && d->dtype != ZDT_FP16) return false;
     if (d->activation < ACT_NONE || d->activation > ACT_SWIGLU || (d->activation == ACT_SWIGLU && d->n % 2 != 0)) return false;
     /* the numbers of tiles stay in 32 bits */
     return d->rows <= ZBALHIP_EXPERT_MAX_ROWS && d->k <= ZBALHIP_EXPERT_MAX_WIDTH && d->n <= ZBALHIP_EXPERT_MAX_WIDTH;
 }
+bool linear_sizes_ok(const zbalhip_expert_linear_t *d) { return sizes_ok(d) && (d->dtype == ZDT_BF16 || d->dtype == ZDT_FP16); }
+bool int8_sizes_ok(const zbalhip_expert_linear_int8_t *d)
+{
+    return sizes_ok(d) && (d->y_dtype == ZDT_BF16 || d->y_dtype == ZDT_FP16 || d->y_dtype == ZDT_FP32);
+}
 
-XgemmParams common_params(const zbalhip_expert_linear_t *d)
+template <typename D> XgemmParams common_params(const D *d)
 {
     XgemmParams p = {};
     p.counts = d->counts;
@@ -562,6 +579,27 @@ XgemmParams rows_gradient_params(const zbalhip_expert_linear_t *d)
     p.K = (int)d->n;
     p.N = (int)d->k;
     p.ldo = d->k;
+    return p;
+}
+
+/*
+ * Two k of int8 are one element: the tiles then move, and multiply in the same time, what they do in half precision, and the plan's rule holds as it
+ * is. Rows that are no multiple of 16 bytes are not aligned, whatever half of them is; fewer than 16 k are short.
+ */
+XgemmParams int8_params(const zbalhip_expert_linear_int8_t *d)
+{
+    XgemmParams p = common_params(d);
+    p.k_bytes = (int)d->k;
+    p.lda = p.ldb = d->k % 16 == 0 ? d->k / 2 : 1;
+    p.b = (const uint16_t *)d->weight;
+    p.b_stride = d->k * d->n / 2;
+    p.K = (int)d->k / 2;
+    p.N = (int)d->n;
+    p.act = d->activation;
+    p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
+    p.ldo = p.n_half ? p.n_half : p.N;
+    p.b_scale = d->weight_scales;
+    p.b_scale_f32 = d->weight_scales_are_f32;
     return p;
 }
 
@@ -645,5 +683,30 @@ extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t 
         p.bias_side = grad_bias ? (d->weight_is_nk ? 2 : 1) : 0;
         launch_types<true>(p, d->dtype, true, workspace, workspace_bytes, st);
     }
+    return zbalhip_check_launch();
+}
+
+extern "C" int64_t zbalhip_expert_linear_int8_workspace(const zbalhip_expert_linear_int8_t *d)
+{
+    if (!int8_sizes_ok(d)) return -1;
+    return d->rows == 0 ? 0 : plan_product(int8_params(d), false, false).bytes;
+}
+
+extern "C" int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t *d, const void *x, const float *x_scales, const void *bias, int32_t bias_is_f32,
+                                              const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    if (!int8_sizes_ok(d) || !d->weight || !d->weight_scales || (d->experts > 1 && !d->counts)) return ZBALHIP_INVALID;
+    if (d->rows == 0) return ZBALHIP_OK;
+    if (!x || !x_scales || !y) return ZBALHIP_INVALID;
+    XgemmParams p = int8_params(d);
+    p.a = (const uint16_t *)x;
+    p.a_scale = x_scales;
+    p.out = y;
+    p.out_f32 = d->y_dtype == ZDT_FP32;
+    p.bias = bias;
+    p.bias_f32 = bias_is_f32;
+    p.residual = residual;
+    if (d->y_dtype == ZDT_FP16) launch_product<XI8 | ZDT_FP16, false, false>(p, workspace, workspace_bytes, (hipStream_t)stream);
+    else launch_product<XI8 | ZDT_BF16, false, false>(p, workspace, workspace_bytes, (hipStream_t)stream);
     return zbalhip_check_launch();
 }

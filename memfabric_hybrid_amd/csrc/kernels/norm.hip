@@ -1,0 +1,537 @@
+/*
+ * Rows of tokens between the products: the root-mean-square norm with the residual's addition and its gradient, and activations,
+ * with an output in int8 and a scale for each row.
+ *
+ * A row is read once: its elements stay in registers (eight to a piece, up to eight pieces to a lane) from the loads over the row's
+ * sum of squares and its largest element to the stores. Pieces start wherever their row starts; the last one of a row whose length is not a
+ * multiple of eight goes element by element.
+ */
+#include "zbal_expert_tile.h"
+
+namespace {
+
+constexpr int N_LANES = 1024, N_PIECES = 8;          /* of a row, and of a lane: 65536 elements */
+
+/* ---- eight elements ------------------------------------------------------------------------------------------------ */
+
+template <int DT> __device__ __forceinline__ float n_load1(const void *p, int64_t i)
+{
+    if constexpr (DT == ZDT_FP32) return static_cast<const float *>(p)[i];
+    else return zb_half_to_f32<DT>(static_cast<const uint16_t *>(p)[i]);
+}
+template <int DT> __device__ __forceinline__ void n_store1(void *p, int64_t i, float v)
+{
+    if constexpr (DT == ZDT_FP32) static_cast<float *>(p)[i] = v;
+    else static_cast<uint16_t *>(p)[i] = (uint16_t)zb_f32_to_half<DT>(v);
+}
+
+typedef u32x4 __attribute__((aligned(2))) n_halves_t;
+typedef f32x4 __attribute__((aligned(4))) n_floats_t;
+typedef u32x2 __attribute__((aligned(1))) n_bytes_t;
+
+/* as they lie in memory, so that a piece that waits takes no more registers than it must */
+template <int DT> struct Piece {
+    u32x4 w[DT == ZDT_FP32 ? 2 : 1];
+    __device__ __forceinline__ float operator[](int i) const
+    {
+        if constexpr (DT == ZDT_FP32) return __uint_as_float(w[i >> 2][i & 3]);
+        else return zb_half_to_f32<DT>(i & 1 ? w[0][i >> 1] >> 16 : w[0][i >> 1] & 0xffffu);
+    }
+};
+
+/* elements at .. at + 7 of which `n` are there; zeros for the others */
+template <int DT> __device__ __forceinline__ Piece<DT> n_load(const void *p, int64_t at, int n)
+{
+    Piece<DT> r = {};
+    if (n >= 8) {
+        if constexpr (DT == ZDT_FP32) {
+            r.w[0] = __builtin_bit_cast(u32x4, (f32x4)*reinterpret_cast<const n_floats_t *>(static_cast<const float *>(p) + at));
+            r.w[1] = __builtin_bit_cast(u32x4, (f32x4)*reinterpret_cast<const n_floats_t *>(static_cast<const float *>(p) + at + 4));
+        } else {
+            r.w[0] = *reinterpret_cast<const n_halves_t *>(static_cast<const uint16_t *>(p) + at);
+        }
+        return r;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) {
+            if constexpr (DT == ZDT_FP32) r.w[i >> 2][i & 3] = static_cast<const uint32_t *>(p)[at + i];
+            else r.w[0][i >> 1] |= (uint32_t)static_cast<const uint16_t *>(p)[at + i] << ((i & 1) * 16);
+        }
+    return r;
+}
+
+template <int DT> __device__ __forceinline__ void n_store(void *p, int64_t at, int n, const float (&v)[8])
+{
+    if (n >= 8) {
+        if constexpr (DT == ZDT_FP32) {
+            *reinterpret_cast<n_floats_t *>(static_cast<float *>(p) + at) = f32x4{v[0], v[1], v[2], v[3]};
+            *reinterpret_cast<n_floats_t *>(static_cast<float *>(p) + at + 4) = f32x4{v[4], v[5], v[6], v[7]};
+        } else {
+            *reinterpret_cast<n_halves_t *>(static_cast<uint16_t *>(p) + at) =
+                u32x4{zb_pack2_half<DT>(v[0], v[1]), zb_pack2_half<DT>(v[2], v[3]), zb_pack2_half<DT>(v[4], v[5]), zb_pack2_half<DT>(v[6], v[7])};
+        }
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) n_store1<DT>(p, at + i, v[i]);
+}
+
+__device__ __forceinline__ void n_store_int8(uint8_t *p, int64_t at, int n, const float (&v)[8])
+{
+    const u32x2 q = {zb_pack4_i8(v[0], v[1], v[2], v[3]), zb_pack4_i8(v[4], v[5], v[6], v[7])};
+    if (n >= 8) {
+        *reinterpret_cast<n_bytes_t *>(p + at) = q;
+        return;
+    }
+#pragma unroll
+    for (int i = 0; i < 7; ++i)
+        if (i < n) p[at + i] = (uint8_t)(q[i >> 2] >> ((i & 3) * 8));
+}
+
+/* ---- rows ---------------------------------------------------------------------------------------------------------- */
+
+/*
+ * The lanes of a row: `waves` whole waves, and as many rows side by side in a workgroup as there are groups of them. What a round of rows leaves
+ * in the LDS lies in one of two places in turn: who is a barrier ahead writes the other one.
+ */
+struct Lanes {
+    int lane, of_row, group, waves, rows;     /* of_row: this lane's place among its row's */
+    __device__ __forceinline__ Lanes() : lane(threadIdx.x & 63), of_row(threadIdx.x), group(threadIdx.y), waves(blockDim.x >> 6), rows(blockDim.y) {}
+    __device__ __forceinline__ int slot() const { return __builtin_amdgcn_readfirstlane(group * waves + (of_row >> 6)); }
+};
+
+template <int N> struct RowSums { float v[N]; };
+
+/* sums over a row's lanes, in all of them; always in the same order */
+template <int N> __device__ __forceinline__ RowSums<N> row_sum(RowSums<N> s, const Lanes &l, float (*red)[N])
+{
+#pragma unroll
+    for (int i = 0; i < N; ++i) s.v[i] = zb_wave_reduce_dpp<false>(s.v[i]);
+    if (l.waves == 1) return s;
+    if (l.lane == 0)
+#pragma unroll
+        for (int i = 0; i < N; ++i) red[l.slot()][i] = s.v[i];
+    __syncthreads();
+    RowSums<N> r = {};
+    for (int w = 0; w < l.waves; ++w)
+#pragma unroll
+        for (int i = 0; i < N; ++i) r.v[i] += red[l.group * l.waves + w][i];
+    return r;
+}
+
+/*
+ * The largest magnitude of a row, as its bits: ordered like the numbers, infinity above them and every NaN above that, so that neither is lost.
+ */
+__device__ __forceinline__ uint32_t n_magnitude(float v) { return __float_as_uint(v) & 0x7fffffffu; }
+__device__ __forceinline__ uint32_t n_max(uint32_t a, uint32_t b) { return a > b ? a : b; }
+__device__ __forceinline__ uint32_t row_max(uint32_t m, const Lanes &l, uint32_t *red)
+{
+#pragma unroll
+    for (int off = 1; off < 64; off <<= 1) m = n_max(m, (uint32_t)__shfl_xor((int)m, off, 64));
+    if (l.waves == 1) return m;
+    if (l.lane == 0) red[l.slot()] = m;
+    __syncthreads();
+    m = 0;
+    for (int w = 0; w < l.waves; ++w) m = n_max(m, red[l.group * l.waves + w]);
+    return m;
+}
+
+/*
+ * scale = max / 127, and what the row is multiplied by: 127 / max. The scale is a normal number (2^-126 at least, so that the factor is finite),
+ * 0 for a row of zeros, and NaN where the row holds an infinity or a NaN: then nothing that is computed from it looks sound.
+ */
+struct RowScale { float scale, by; };
+__device__ __forceinline__ RowScale row_scale(uint32_t max_bits)
+{
+    const float max = __uint_as_float(max_bits);
+    if (max_bits >= 0x7f800000u) return {__uint_as_float(0x7fc00000u), 0.0f};
+    if (max_bits == 0) return {0.0f, 0.0f};
+    if (max < 127.0f * 0x1p-126f) return {0x1p-126f, 0x1p126f};
+    return {max / 127.0f, 127.0f / max};
+}
+
+/* ---- the norm ------------------------------------------------------------------------------------------------------ */
+
+struct NormParams {
+    const void *x, *residual, *weight;
+    void *y, *total;
+    uint8_t *q;
+    float *scales;
+    const void *grad, *grad_total;    /* the gradient's */
+    void *grad_x;
+    float *partial;                   /* [row groups of the launch][ldp]: the sums of their rows for the weight's gradient */
+    int64_t rows;
+    int width, ldp, weight_f32;
+    float eps, per_width;             /* 1 / width */
+};
+
+__device__ __forceinline__ float n_rsqrt(float mean_square, float eps) { return 1.0f / __builtin_sqrtf(mean_square + eps); }
+
+/* the weight's eight elements, ones without a weight */
+template <int DT> __device__ __forceinline__ void n_weight(const NormParams &p, int at, int n, float (&w)[8])
+{
+    if (!p.weight) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = 1.0f;
+    } else if (DT != ZDT_FP32 && p.weight_f32) {
+        const Piece<ZDT_FP32> v = n_load<ZDT_FP32>(p.weight, at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = v[i];
+    } else {
+        const Piece<DT> v = n_load<DT>(p.weight, at, n);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) w[i] = v[i];
+    }
+}
+
+template <int DT, int C>
+__global__ void __launch_bounds__(N_LANES)
+rms_norm_kernel(NormParams p)
+{
+    __shared__ float sums[2][16][1];
+    __shared__ uint32_t maxima[2][16];
+    const Lanes l;
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * l.rows; base < p.rows; base += (int64_t)gridDim.x * l.rows, turn ^= 1) {
+        const int64_t row = base + l.group, at = row * p.width;
+        const bool live = row < p.rows;
+        int there[C];
+        float h[C][8];
+        {
+            Piece<DT> x[C], r[C];
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+                there[c] = live ? p.width - (l.of_row + c * (int)blockDim.x) * 8 : 0;
+                x[c] = n_load<DT>(p.x, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+                if (p.residual) r[c] = n_load<DT>(p.residual, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+            }
+#pragma unroll
+            for (int c = 0; c < C; ++c)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] = p.residual ? x[c][i] + r[c][i] : x[c][i];
+        }
+        RowSums<1> s = {};
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) s.v[0] = __builtin_fmaf(h[c][i], h[c][i], s.v[0]);
+        if (p.total)
+#pragma unroll
+            for (int c = 0; c < C; ++c) n_store<DT>(p.total, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], h[c]);
+        s = row_sum<1>(s, l, sums[turn]);
+        const float r = n_rsqrt(s.v[0] * p.per_width, p.eps);
+        uint32_t most = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float w[8];
+            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                h[c][i] = h[c][i] * r * w[i];
+                if (i < there[c]) most = n_max(most, n_magnitude(h[c][i]));
+            }
+            if (p.y) n_store<DT>(p.y, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], h[c]);
+        }
+        if (p.q) {
+            const RowScale to = row_scale(row_max(most, l, maxima[turn]));
+            if (live && l.of_row == 0) p.scales[row] = to.scale;
+#pragma unroll
+            for (int c = 0; c < C; ++c) {
+#pragma unroll
+                for (int i = 0; i < 8; ++i) h[c][i] *= to.by;
+                n_store_int8(p.q, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], h[c]);
+            }
+        }
+    }
+}
+
+/*
+ * With n = h r and d = g w: dh = r (d - n mean(d n)) + the sum's own gradient, and the weight's gradient is the sum over rows of g n. Both means of a row
+ * come from one reduction, of h^2 and of d h. A lane has the same columns of every row that its workgroup takes, so the
+ * weight's sums stay in registers until the last of them; a second launch adds up the workgroups', in order.
+ */
+template <int DT, int C>
+__global__ void __launch_bounds__(N_LANES)
+rms_norm_backward_kernel(NormParams p)
+{
+    __shared__ float sums[2][16][2];
+    const Lanes l;
+    float dw[C][8];
+#pragma unroll
+    for (int c = 0; c < C; ++c)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * l.rows; base < p.rows; base += (int64_t)gridDim.x * l.rows, turn ^= 1) {
+        const int64_t row = base + l.group, at = row * p.width;
+        const bool live = row < p.rows;
+        int there[C];
+        Piece<DT> h[C], g[C], t[C];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            there[c] = live ? p.width - (l.of_row + c * (int)blockDim.x) * 8 : 0;
+            h[c] = n_load<DT>(p.x, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+            g[c] = n_load<DT>(p.grad, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+            if (p.grad_total) t[c] = n_load<DT>(p.grad_total, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+        }
+        RowSums<2> s = {};
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float w[8];
+            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                s.v[0] = __builtin_fmaf(h[c][i], h[c][i], s.v[0]);
+                s.v[1] = __builtin_fmaf(g[c][i] * w[i], h[c][i], s.v[1]);
+            }
+        }
+        s = row_sum<2>(s, l, sums[turn]);
+        const float r = n_rsqrt(s.v[0] * p.per_width, p.eps), mean = s.v[1] * p.per_width * r;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            float w[8], d[8];
+            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float n = h[c][i] * r;
+                d[i] = r * __builtin_fmaf(-n, mean, g[c][i] * w[i]);
+                if (p.grad_total) d[i] += t[c][i];
+                dw[c][i] = __builtin_fmaf(g[c][i], n, dw[c][i]);
+            }
+            n_store<DT>(p.grad_x, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], d);
+        }
+    }
+    if (!p.partial) return;
+    float *to = p.partial + ((int64_t)blockIdx.x * l.rows + l.group) * p.ldp;
+#pragma unroll
+    for (int c = 0; c < C; ++c) {
+        const int at = (l.of_row + c * (int)blockDim.x) * 8;
+        n_store<ZDT_FP32>(to, at, p.width - at, dw[c]);
+    }
+}
+
+/* sums of `count` rows of ldp floats, sixteen columns of four by sixteen rows to a workgroup; out f32, or of type DT */
+template <int DT>
+__global__ void __launch_bounds__(256)
+rms_norm_join_kernel(const float *__restrict__ partial, int count, int ldp, int width, int out_f32, void *__restrict__ out)
+{
+    __shared__ f32x4 sums[16][16];
+    const int quad = threadIdx.x & 15, first = threadIdx.x >> 4, col = (blockIdx.x * 16 + quad) * 4;
+    f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
+    if (col < ldp)
+#pragma unroll 8
+        for (int i = first; i < count; i += 16) s += *reinterpret_cast<const f32x4 *>(partial + (int64_t)i * ldp + col);
+    sums[first][quad] = s;
+    __syncthreads();
+    if (first != 0) return;
+    for (int i = 1; i < 16; ++i) s += sums[i][quad];
+    for (int i = 0; i < 4 && col + i < width; ++i) {
+        if (out_f32) static_cast<float *>(out)[col + i] = s[i];
+        else n_store1<DT>(out, col + i, s[i]);
+    }
+}
+
+/* ---- activations in int8 ------------------------------------------------------------------------------------------- */
+
+/* ACT: ACT_NONE, ACT_SWIGLU, or ACT_SILU for whichever of the others the parameters name */
+template <int DT, int ACT, int C>
+__global__ void __launch_bounds__(N_LANES)
+quantize_rows_kernel(XgemmParams p, const void *__restrict__ x, uint8_t *__restrict__ q, float *__restrict__ scales)
+{
+    __shared__ uint32_t maxima[2][16];
+    const Lanes l;
+    const int cols = p.n_half ? p.n_half : p.N, rows = p.counts ? x_rows_of(p, p.experts - 1).end : p.rows;
+    int turn = 0;
+    for (int64_t base = (int64_t)blockIdx.x * l.rows; base < rows; base += (int64_t)gridDim.x * l.rows, turn ^= 1) {
+        const int64_t row = base + l.group, at = row * p.N;
+        const bool live = row < rows;
+        int there[C];
+        Piece<DT> z[C], up[ACT == ACT_SWIGLU ? C : 1];
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+            const int col = (l.of_row + c * (int)blockDim.x) * 8;
+            there[c] = live ? cols - col : 0;
+            z[c] = n_load<DT>(x, at + col, there[c]);
+            if constexpr (ACT == ACT_SWIGLU) up[c] = n_load<DT>(x, at + cols + col, there[c]);
+        }
+        float y[C][8];
+        uint32_t most = 0;
+#pragma unroll
+        for (int c = 0; c < C; ++c)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                if constexpr (ACT == ACT_NONE) y[c][i] = z[c][i];
+                else if constexpr (ACT == ACT_SWIGLU) y[c][i] = x_silu(z[c][i]) * up[c][i];
+                else y[c][i] = x_activate(p.act, z[c][i]);
+                if (i < there[c]) most = n_max(most, n_magnitude(y[c][i]));
+            }
+        const RowScale to = row_scale(row_max(most, l, maxima[turn]));
+        if (live && l.of_row == 0) scales[row] = to.scale;
+#pragma unroll
+        for (int c = 0; c < C; ++c) {
+#pragma unroll
+            for (int i = 0; i < 8; ++i) y[c][i] *= to.by;
+            n_store_int8(q, row * cols + (l.of_row + c * (int)blockDim.x) * 8, there[c], y[c]);
+        }
+    }
+}
+
+/* ---- launches ------------------------------------------------------------------------------------------------------ */
+
+/* lanes and pieces of a row of `width` elements: waves of one piece to a lane up to 512 lanes, then more pieces; rows side by side in 256 lanes */
+struct Shape {
+    int pieces, groups;
+    unsigned lanes;
+    dim3 block() const { return dim3(lanes, groups); }
+    unsigned blocks(int64_t rows, int64_t most) const
+    {
+        const int64_t n = (rows + groups - 1) / groups;
+        return (unsigned)(n < most ? n : most);
+    }
+};
+inline Shape shape_of(int64_t width, int most_lanes)
+{
+    const int64_t pieces = (width + 7) / 8;
+    Shape s = {1, 1, 0};
+    while (s.pieces < N_PIECES && (pieces + s.pieces - 1) / s.pieces > most_lanes) s.pieces *= 2;
+    s.lanes = (unsigned)(((pieces + s.pieces - 1) / s.pieces + 63) / 64 * 64);
+    s.groups = s.lanes >= 256 ? 1 : 256 / (int)s.lanes;
+    return s;
+}
+
+/* f(integral_constant pieces) */
+template <typename F> void with_pieces(int pieces, F f)
+{
+    switch (pieces) {
+        case 1: f(std::integral_constant<int, 1>{}); break;
+        case 2: f(std::integral_constant<int, 2>{}); break;
+        case 4: f(std::integral_constant<int, 4>{}); break;
+        default: f(std::integral_constant<int, 8>{});
+    }
+}
+template <typename F> void with_type(int dtype, F f)
+{
+    switch (dtype) {
+        case ZDT_BF16: f(std::integral_constant<int, ZDT_BF16>{}); break;
+        case ZDT_FP16: f(std::integral_constant<int, ZDT_FP16>{}); break;
+        default: f(std::integral_constant<int, ZDT_FP32>{});
+    }
+}
+
+constexpr int64_t N_MOST_BLOCKS = 1 << 20;           /* of 1024 lanes: a launch is less than 2^32 lanes */
+
+bool norm_ok(const zbalhip_rms_norm_t *d)
+{
+    if (!d || d->tokens < 0 || d->tokens > ZBALHIP_EXPERT_MAX_ROWS || d->hidden <= 0 || d->hidden > ZBALHIP_EXPERT_MAX_WIDTH) return false;
+    if (d->dtype != ZDT_BF16 && d->dtype != ZDT_FP16 && d->dtype != ZDT_FP32) return false;
+    return d->eps > 0.0f && d->eps < __builtin_inff();
+}
+
+NormParams norm_params(const zbalhip_rms_norm_t *d)
+{
+    NormParams p = {};
+    p.x = d->x;
+    p.residual = d->residual;
+    p.weight = d->weight;
+    p.weight_f32 = d->weight_is_f32;
+    p.rows = d->tokens;
+    p.width = (int)d->hidden;
+    p.ldp = (p.width + 3) / 4 * 4;
+    p.eps = d->eps;
+    p.per_width = 1.0f / (float)d->hidden;
+    return p;
+}
+
+/* row groups of the gradient's launch, each with sums of its own */
+Shape backward_shape(int64_t width) { return shape_of(width, 512); }
+unsigned backward_blocks(const zbalhip_rms_norm_t *d)
+{
+    return backward_shape(d->hidden).blocks(d->tokens, 1024);
+}
+
+} // namespace
+
+extern "C" int32_t zbalhip_rms_norm(const zbalhip_rms_norm_t *d, void *y, void *total, int8_t *q, float *scales, void *stream)
+{
+    if (!norm_ok(d) || (q && !scales)) return ZBALHIP_INVALID;
+    if (d->tokens == 0) return ZBALHIP_OK;
+    if (!d->x || (!y && !total && !q)) return ZBALHIP_INVALID;
+    NormParams p = norm_params(d);
+    p.y = y;
+    p.total = total;
+    p.q = (uint8_t *)q;
+    p.scales = scales;
+    const Shape s = shape_of(d->hidden, 512);
+    with_type(d->dtype, [&](auto dt) {
+        with_pieces(s.pieces, [&](auto c) {
+            zb_launch(rms_norm_kernel<decltype(dt)::value, decltype(c)::value>, dim3(s.blocks(p.rows, N_MOST_BLOCKS)), s.block(), 0, (hipStream_t)stream, p);
+        });
+    });
+    return zbalhip_check_launch();
+}
+
+extern "C" int64_t zbalhip_rms_norm_backward_workspace(const zbalhip_rms_norm_t *d)
+{
+    if (!norm_ok(d)) return -1;
+    return (int64_t)backward_blocks(d) * backward_shape(d->hidden).groups * ((d->hidden + 3) / 4 * 4) * 4;
+}
+
+extern "C" int32_t zbalhip_rms_norm_backward(const zbalhip_rms_norm_t *d, const void *grad, const void *grad_total, void *grad_x, void *grad_weight,
+                                             int32_t weight_grad_is_f32, void *workspace, int64_t workspace_bytes, void *stream)
+{
+    if (!norm_ok(d)) return ZBALHIP_INVALID;
+    if (d->tokens > 0 && (!d->x || !grad || !grad_x)) return ZBALHIP_INVALID;
+    if (d->tokens == 0 && !grad_weight) return ZBALHIP_OK;
+    if (grad_weight && d->tokens > 0 && (!workspace || workspace_bytes < zbalhip_rms_norm_backward_workspace(d))) return ZBALHIP_INVALID;
+    NormParams p = norm_params(d);
+    p.grad = grad;
+    p.grad_total = grad_total;
+    p.grad_x = grad_x;
+    p.partial = grad_weight ? (float *)workspace : nullptr;
+    const Shape s = backward_shape(d->hidden);
+    const unsigned blocks = backward_blocks(d);
+    hipStream_t st = (hipStream_t)stream;
+    if (d->tokens > 0)
+        with_type(d->dtype, [&](auto dt) {
+            with_pieces(s.pieces, [&](auto c) {
+                zb_launch(rms_norm_backward_kernel<decltype(dt)::value, decltype(c)::value>, dim3(blocks), s.block(), 0, st, p);
+            });
+        });
+    if (grad_weight)
+        with_type(d->dtype, [&](auto dt) {
+            zb_launch(rms_norm_join_kernel<decltype(dt)::value>, dim3((unsigned)(p.ldp + 63) / 64), dim3(256), 0, st, p.partial, (int)(blocks * s.groups), p.ldp,
+                      p.width, weight_grad_is_f32, grad_weight);
+        });
+    return zbalhip_check_launch();
+}
+
+extern "C" int32_t zbalhip_quantize_rows(const zbalhip_quantize_rows_t *d, const void *x, int8_t *q, float *scales, void *stream)
+{
+    if (!d || d->rows < 0 || d->rows > ZBALHIP_EXPERT_MAX_ROWS || d->width <= 0 || d->width > ZBALHIP_EXPERT_MAX_WIDTH) return ZBALHIP_INVALID;
+    if (d->dtype != ZDT_BF16 && d->dtype != ZDT_FP16 && d->dtype != ZDT_FP32) return ZBALHIP_INVALID;
+    if (d->activation < ACT_NONE || d->activation > ACT_SWIGLU || (d->activation == ACT_SWIGLU && d->width % 2 != 0)) return ZBALHIP_INVALID;
+    if (d->counts && (d->experts <= 0 || d->experts > 1024)) return ZBALHIP_INVALID;
+    if (d->rows == 0) return ZBALHIP_OK;
+    if (!x || !q || !scales) return ZBALHIP_INVALID;
+    XgemmParams p = {};
+    p.counts = d->counts;
+    p.counts_i64 = d->counts_are_i64;
+    p.experts = d->counts ? (int)d->experts : 1;
+    p.rows = (int)d->rows;
+    p.N = (int)d->width;
+    p.act = d->activation;
+    p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
+    const Shape s = shape_of(p.n_half ? p.n_half : p.N, 512);
+    const dim3 grid(s.blocks(d->rows, N_MOST_BLOCKS));
+    with_type(d->dtype, [&](auto dt) {
+        with_pieces(s.pieces, [&](auto c) {
+            constexpr int DT = decltype(dt)::value, C = decltype(c)::value;
+            if (p.act == ACT_NONE) zb_launch(quantize_rows_kernel<DT, ACT_NONE, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+            else if (p.act == ACT_SWIGLU) zb_launch(quantize_rows_kernel<DT, ACT_SWIGLU, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+            else zb_launch(quantize_rows_kernel<DT, ACT_SILU, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+        });
+    });
+    return zbalhip_check_launch();
+}

@@ -70,7 +70,7 @@ __device__ __forceinline__ void x_lines_out(uint32_t own, void *out, int f32, in
                     const f32x4 v = value(mt, i0 + i);
                     if constexpr (F32) *(lds_f_t)(uintptr_t)(put + (((i * 4 + g16) ^ key) << 4)) = v;
                     else *(lds_h_t)(uintptr_t)(put + (((i * 2 + (g16 >> 1)) ^ key) << 4) + (g16 & 1) * 8) =
-                        u32x2{zb_pack2_half<DT>(v[0], v[1]), zb_pack2_half<DT>(v[2], v[3])};
+                        u32x2{zb_pack2_half<x_half<DT>>(v[0], v[1]), zb_pack2_half<x_half<DT>>(v[2], v[3])};
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const int at = i0 * (F32 ? 64 : 32) + c_out * 16;
@@ -219,12 +219,12 @@ expert_gemm_kernel(XgemmParams p)
         left -= XBK;
     };
 
-    f32x4 acc[MT][NT], bias_acc[REDUCE ? (MT > NT ? MT : NT) : 1];
+    x_sums_t<DT> acc[MT][NT], bias_acc[REDUCE ? (MT > NT ? MT : NT) : 1];
 #pragma unroll
     for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-    for (auto &v : bias_acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+        for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = x_sums_t<DT>{0, 0, 0, 0};
+    for (auto &v : bias_acc) v = x_sums_t<DT>{0, 0, 0, 0};
     const bool bias_b = REDUCE && p.bias_side == 1 && m0 == 0 && wm == 0, bias_a = REDUCE && p.bias_side == 2 && n0 == 0 && wn == 0;
     const uint32_t one2 = DT == ZDT_BF16 ? 0x3f803f80u : 0x3c003c00u;
     const u32x4 ones = {one2, one2, one2, one2};
@@ -290,16 +290,24 @@ expert_gemm_kernel(XgemmParams p)
     const int cols_left = cols - n0 - wn * (p.n_half ? NT * 8 : NT * 16), row0 = m0 + wm * (MT * 16), rows_left = m_end - row0;
     const uint32_t own = __builtin_amdgcn_readfirstlane(x_lds(smem) + wave * 2048);
     static_assert(WAVES * 2048 <= STAGES * STAGE, "every wave has its own");
+    /* parts' sums stay integers until they are joined */
+    if constexpr (x_is_i8<DT>)
+        if (p.splits == 1)
+            x_scale_tile(acc, p.a_scale, p.b_scale, p.b_scale_f32, (int64_t)expert * p.N, m_end, [&](int mt) { return row0 + mt * 16 + (lane & 15); }, [&](int nt) {
+                const bool up = p.n_half && nt >= (NT + 1) / 2;
+                const int j = (cols - cols_left) + (up ? nt - NT / 2 : nt) * 16 + q4;
+                return j < cols ? j + (up ? p.n_half : 0) : -1;
+            });
     const bool plain = REDUCE || p.splits > 1 || (!p.bias && !p.residual && !p.preact && (p.act == ACT_NONE || p.act == ACT_SWIGLU));
     if (plain) {
         __syncthreads();
         if (p.splits > 1) {
             float *to = p.partial + ((int64_t)split * (REDUCE ? p.M : p.rows) + row0) * p.ldp + (cols - cols_left);
             if (NT > 1 && p.n_half) {
-                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return acc[mt][i]; });
-                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to + p.n_half, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return acc[mt][i + NT / 2]; });
+                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
+                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to + p.n_half, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i + NT / 2]); });
             } else {
-                x_lines_out<DT, MT, NT, 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return acc[mt][i]; });
+                x_lines_out<DT, MT, NT, 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
             }
             return;
         }
@@ -308,11 +316,11 @@ expert_gemm_kernel(XgemmParams p)
             x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to, p.out_f32, (int)p.ldo, rows_left, cols_left, lane, [&](int mt, int i) {
                 f32x4 y;
 #pragma unroll
-                for (int c = 0; c < 4; ++c) y[c] = x_silu(acc[mt][i][c]) * acc[mt][i + NT / 2][c];
+                for (int c = 0; c < 4; ++c) y[c] = x_silu(x_value(acc[mt][i])[c]) * x_value(acc[mt][i + NT / 2])[c];
                 return y;
             });
         else
-            x_lines_out<DT, MT, NT, 16, 0>(own, to, p.out_f32, (int)p.ldo, rows_left, cols_left, lane, [&](int mt, int i) { return acc[mt][i]; });
+            x_lines_out<DT, MT, NT, 16, 0>(own, to, p.out_f32, (int)p.ldo, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
         return;
     }
     if constexpr (REDUCE) return;
@@ -330,7 +338,7 @@ expert_gemm_kernel(XgemmParams p)
         for (int h = 0; h < PASS; ++h)
 #pragma unroll
             for (int nt = 0; nt < NT; ++nt)
-                *reinterpret_cast<f32x4 *>(sums + (wm * (PASS * 16) + h * 16 + (lane & 15)) * LD + col_of(nt) + q4) = acc[pass * PASS + h][nt];
+                *reinterpret_cast<f32x4 *>(sums + (wm * (PASS * 16) + h * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
         __syncthreads();
         constexpr int QUADS = TN / 4;
 #pragma unroll 1

@@ -1,5 +1,5 @@
 /*
- * The half-precision products of the experts for few rows, weights with consecutive k.
+ * The products of the experts for few rows, weights with consecutive k.
  *
  * A token's products read every weight once, and nothing else takes time: 2048 x 7168, one row, are 29 MB, 4.7 us at what a large read reaches. Weights that
  * only one wave needs gain nothing from the LDS: a lane loads the eight k of its column straight into the fragment that the matrix
@@ -21,7 +21,7 @@ __global__ void __launch_bounds__(WAVES * 64)
 expert_gemm_rows_kernel(XgemmParams p)
 {
     constexpr int BATCH = 8 / NT, LD = NT * 16 + 1;
-    __shared__ float sums[WAVES][16][LD];
+    __shared__ x_sum_t<DT> sums[WAVES][16][LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
     const int cols = p.n_half ? p.n_half : p.N, n_tiles = (cols + 15) / 16;
     const XTile t = x_locate<16>(p, n_tiles, blockIdx.x, XSLOTS);
@@ -34,8 +34,8 @@ expert_gemm_rows_kernel(XgemmParams p)
     const uint16_t *b = p.b + t.expert * p.b_stride + (int64_t)(col < cols ? col : cols - 1) * p.ldb;
     const int64_t up = (int64_t)p.n_half * p.ldb;
 
-    f32x4 acc[NT];
-    for (auto &v : acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+    x_sums_t<DT> acc[NT];
+    for (auto &v : acc) v = x_sums_t<DT>{0, 0, 0, 0};
     for (int k0 = wave * 64; k0 < p.K; k0 += WAVES * 64 * BATCH) {
         u32x4 fa[BATCH][2], fb[NT][BATCH][2];
 #pragma unroll
@@ -65,12 +65,13 @@ expert_gemm_rows_kernel(XgemmParams p)
     __syncthreads();
     const int r = tid >> 4, c = tid & 15;
     if (tid >= 256 || t.row_begin + r >= t.row_end || n0 + c >= cols) return;
-    float z[2] = {0.0f, 0.0f};
+    x_sum_t<DT> z[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) z[i] += sums[w][r][i * 16 + c];
-    x_finish<DT>(p, t.expert, t.row_begin + r, n0 + c, z[0], z[1]);
+    const int64_t at = t.row_begin + r;
+    x_finish<DT>(p, t.expert, at, n0 + c, x_scaled<DT>(p, t.expert, at, n0 + c, z[0]), NT > 1 ? x_scaled<DT>(p, t.expert, at, p.n_half + n0 + c, z[1]) : 0.0f);
 }
 
 } // namespace

@@ -1,5 +1,5 @@
 /*
- * What the half-precision products of the experts share: the parameter block, where a workgroup's tile lies, how operands lie in
+ * What the half-precision and int8 products of the experts share: the parameter block, where a workgroup's tile lies, how operands lie in
  * the LDS and come out of it as matrix-instruction fragments, and the epilogues.
  *
  * Three products are tiles of the same kind, C[m, n] = sum over k of A[m, k] B[k, n]:
@@ -9,6 +9,9 @@
  *
  * An operand whose k is consecutive lies in the LDS as rows of 64 k (128 bytes), one whose m or n is consecutive as rows of the
  * tile's width, 64 of them; the latter is read with ds_read_b64_tr_b16, which hands every lane four k of its column.
+ *
+ * In int8 both operands have consecutive k, and two of them are one element of 16 bits to all that moves them: the matrix instruction takes the same
+ * sixteen bytes of a lane, in the same places, for twice as many k, and adds up 32-bit integers, which no order of the sums can change.
  */
 #ifndef ZBAL_EXPERT_TILE_H_
 #define ZBAL_EXPERT_TILE_H_
@@ -30,6 +33,7 @@ struct XgemmParams {
     int counts_i64, experts;
     int rows;                    /* of the token-side tensors */
     int M, N, K;                 /* M: REDUCE only; K: not REDUCE */
+    int k_bytes;                 /* int8: K counts pairs of them, this one each */
     int n_half;                  /* swiglu: N / 2, where the up columns start; else 0 */
     void *out;
     int64_t ldo, out_stride;
@@ -38,6 +42,9 @@ struct XgemmParams {
     int bias_f32;
     const void *residual;        /* of out's type and shape */
     uint16_t *preact;            /* [rows, N] */
+    const float *a_scale;        /* int8: [rows] */
+    const void *b_scale;         /* int8: [experts, N], fp32 or bf16 */
+    int b_scale_f32;
     void *bias_grad;             /* REDUCE: [experts, bias_n], of out's type */
     int bias_side;               /* REDUCE: the operand whose columns it sums: 1 = b, 2 = a */
     float *partial;              /* split along k: [splits][rows of C][ldp] sums instead of out, and [splits][bias_ldp] of the bias's */
@@ -51,9 +58,18 @@ typedef __bf16 bf16x8_t __attribute__((ext_vector_type(8)));
 typedef _Float16 f16x8_t __attribute__((ext_vector_type(8)));
 typedef short s16x4_t __attribute__((ext_vector_type(4)));
 
-template <int DT> __device__ __forceinline__ f32x4 x_mfma(const u32x4 &rows, const u32x4 &cols, const f32x4 &c)
+/* the operands' type in DT: bf16, fp16, or int8 with the 16-bit type of the outputs */
+constexpr int XI8 = 0x100;
+template <int DT> constexpr bool x_is_i8 = (DT & XI8) != 0;
+template <int DT> constexpr int x_half = DT & ~XI8;
+template <int DT> using x_sum_t = std::conditional_t<x_is_i8<DT>, int32_t, float>;
+template <int DT> using x_sums_t = std::conditional_t<x_is_i8<DT>, i32x4, f32x4>;
+
+template <int DT> __device__ __forceinline__ x_sums_t<DT> x_mfma(const u32x4 &rows, const u32x4 &cols, const x_sums_t<DT> &c)
 {
-    if constexpr (DT == ZDT_BF16)
+    if constexpr (x_is_i8<DT>)
+        return __builtin_amdgcn_mfma_i32_16x16x64_i8(__builtin_bit_cast(i32x4, rows), __builtin_bit_cast(i32x4, cols), c, 0, 0, 0);
+    else if constexpr (DT == ZDT_BF16)
         return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(bf16x8_t, rows), __builtin_bit_cast(bf16x8_t, cols), c, 0, 0, 0);
     else
         return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(f16x8_t, rows), __builtin_bit_cast(f16x8_t, cols), c, 0, 0, 0);
@@ -271,12 +287,12 @@ __device__ __forceinline__ float x_slope(int act, float z)
 
 template <int DT> __device__ __forceinline__ float x_load(const void *p, int f32, int64_t i)
 {
-    return f32 ? static_cast<const float *>(p)[i] : zb_half_to_f32<DT>(static_cast<const uint16_t *>(p)[i]);
+    return f32 ? static_cast<const float *>(p)[i] : zb_half_to_f32<x_half<DT>>(static_cast<const uint16_t *>(p)[i]);
 }
 template <int DT> __device__ __forceinline__ void x_store(void *p, int f32, int64_t i, float v)
 {
     if (f32) static_cast<float *>(p)[i] = v;
-    else static_cast<uint16_t *>(p)[i] = (uint16_t)zb_f32_to_half<DT>(v);
+    else static_cast<uint16_t *>(p)[i] = (uint16_t)zb_f32_to_half<x_half<DT>>(v);
 }
 
 /* one value of the output from its sums: bias, activation, residual, one rounding. `j`: output column */
@@ -287,8 +303,8 @@ template <int DT> __device__ __forceinline__ void x_finish(const XgemmParams &p,
         if (p.n_half) up += x_load<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + p.n_half + j);
     }
     if (p.preact) {
-        p.preact[row * p.N + j] = (uint16_t)zb_f32_to_half<DT>(z);
-        if (p.n_half) p.preact[row * p.N + p.n_half + j] = (uint16_t)zb_f32_to_half<DT>(up);
+        p.preact[row * p.N + j] = (uint16_t)zb_f32_to_half<x_half<DT>>(z);
+        if (p.n_half) p.preact[row * p.N + p.n_half + j] = (uint16_t)zb_f32_to_half<x_half<DT>>(up);
     }
     float y = p.n_half ? x_silu(z) * up : x_activate(p.act, z);
     if (p.residual) y += x_load<DT>(p.residual, p.out_f32, row * p.ldo + j);
@@ -300,12 +316,13 @@ template <int DT> __device__ __forceinline__ f32x4 x_load4(const void *p, int f3
 {
     if (f32) return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
     const u32x2 h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i);
-    return f32x4{zb_half_to_f32<DT>(h[0] & 0xffffu), zb_half_to_f32<DT>(h[0] >> 16), zb_half_to_f32<DT>(h[1] & 0xffffu), zb_half_to_f32<DT>(h[1] >> 16)};
+    constexpr int H = x_half<DT>;
+    return f32x4{zb_half_to_f32<H>(h[0] & 0xffffu), zb_half_to_f32<H>(h[0] >> 16), zb_half_to_f32<H>(h[1] & 0xffffu), zb_half_to_f32<H>(h[1] >> 16)};
 }
 template <int DT> __device__ __forceinline__ void x_store4(void *p, int f32, int64_t i, const f32x4 &v)
 {
     if (f32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
-    else *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + i) = u32x2{zb_pack2_half<DT>(v[0], v[1]), zb_pack2_half<DT>(v[2], v[3])};
+    else *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + i) = u32x2{zb_pack2_half<x_half<DT>>(v[0], v[1]), zb_pack2_half<x_half<DT>>(v[2], v[3])};
 }
 template <int DT> __device__ __forceinline__ void x_finish4(const XgemmParams &p, int expert, int64_t row, int j, f32x4 z, f32x4 up)
 {
@@ -322,6 +339,42 @@ template <int DT> __device__ __forceinline__ void x_finish4(const XgemmParams &p
     if (p.residual) y += x_load4<DT>(p.residual, p.out_f32, row * p.ldo + j);
     x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, y);
 }
+
+/* ---- int8: sums of integers and their scales ----------------------------------------------------------------------- */
+
+/* a sum as the value that it stands for (half precision: it is that). `j`: column of W */
+template <int DT> __device__ __forceinline__ float x_scaled(const XgemmParams &p, int expert, int64_t row, int j, x_sum_t<DT> sum)
+{
+    if constexpr (x_is_i8<DT>) return (float)sum * x_load<ZDT_BF16>(p.b_scale, p.b_scale_f32, (int64_t)expert * p.N + j) * p.a_scale[row];
+    else return sum;
+}
+template <int DT> __device__ __forceinline__ f32x4 x_scaled4(const XgemmParams &p, int expert, int64_t row, int j, const x_sums_t<DT> &sum)
+{
+    if constexpr (x_is_i8<DT>) return __builtin_convertvector(sum, f32x4) * x_load4<ZDT_BF16>(p.b_scale, p.b_scale_f32, (int64_t)expert * p.N + j) * p.a_scale[row];
+    else return sum;
+}
+
+/*
+ * A lane's sub-tiles, where they are: integers become the bits of the values that they stand for. row(mt), col(nt): the row and the first of four columns
+ * of W that it has there; rows and columns from row_end and -1 on are nobody's.
+ */
+template <int MT, int NT, typename Row, typename Col>
+__device__ __forceinline__ void x_scale_tile(i32x4 (&acc)[MT][NT], const float *a_scale, const void *b_scale, int b_scale_f32, int64_t first_scale, int row_end, Row row, Col col)
+{
+    float rows[MT];
+#pragma unroll
+    for (int mt = 0; mt < MT; ++mt) rows[mt] = a_scale[row(mt) < row_end ? row(mt) : row_end - 1];
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) {
+        const int j = col(nt);
+        f32x4 cols = {0.0f, 0.0f, 0.0f, 0.0f};
+        if (j >= 0) cols = x_load4<ZDT_BF16>(b_scale, b_scale_f32, first_scale + j);
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = __builtin_bit_cast(i32x4, __builtin_convertvector(acc[mt][nt], f32x4) * cols * rows[mt]);
+    }
+}
+__device__ __forceinline__ f32x4 x_value(const f32x4 &v) { return v; }
+__device__ __forceinline__ f32x4 x_value(const i32x4 &v) { return __builtin_bit_cast(f32x4, v); }
 
 } // namespace
 

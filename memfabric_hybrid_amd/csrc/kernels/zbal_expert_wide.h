@@ -279,12 +279,12 @@ expert_gemm_wide_kernel(XgemmParams p)
 
     for (int id = id0; id < id_end; id += slots) {
         const Tile t = tile_at(id);
-        f32x4 acc[MT][NT], bias_acc[BIAS == 1 ? NT : (BIAS == 2 ? MT : 1)];
+        x_sums_t<DT> acc[MT][NT], bias_acc[BIAS == 1 ? NT : (BIAS == 2 ? MT : 1)];
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt)
 #pragma unroll
-            for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-        for (auto &v : bias_acc) v = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+            for (int nt = 0; nt < NT; ++nt) acc[mt][nt] = x_sums_t<DT>{0, 0, 0, 0};
+        for (auto &v : bias_acc) v = x_sums_t<DT>{0, 0, 0, 0};
         /* the tiles of the other operand's first columns do it, as a product with ones */
         const bool bias_b = BIAS == 1 && t.m0 == 0 && wm == 0, bias_a = BIAS == 2 && t.n0 == 0 && wn == 0;
 
@@ -417,6 +417,16 @@ expert_gemm_wide_kernel(XgemmParams p)
                     if (j < p.M) x_store<DT>(p.bias_grad, p.out_f32, (int64_t)t.expert * p.M + j, bias_acc[mt][0]);
                 }
         }
+        if constexpr (x_is_i8<DT>) {
+            const args_t p = fresh_args();
+            const int lane = fresh_lane(), first = t.n0 + (p->n_half ? wn * 32 : wn * 64) + (lane >> 4) * 4;
+            x_scale_tile(acc, p->a_scale, p->b_scale, p->b_scale_f32, (int64_t)t.expert * p->N, t.m_end, [&](int mt) { return t.m0 + mt * 32 + wm * 16 + (lane & 15); },
+                         [&](int nt) {
+                             const bool up = p->n_half && nt >= NT / 2;
+                             const int j = first + (up ? nt - NT / 2 : nt) * 16;
+                             return j < cols ? j + (up ? p->n_half : 0) : -1;
+                         });
+        }
         if (REDUCE || !p.through_lds) {
             /* the weights' gradient is not read again soon */
             const args_t p = fresh_args();
@@ -427,12 +437,12 @@ expert_gemm_wide_kernel(XgemmParams p)
                 x_lines_out<DT, MT, NT / 2, 32, 0>(own, to, p->out_f32, (int)p->ldo, t.m_end - row0, cols - first_col, lane, [&](int mt, int i) __attribute__((always_inline)) {
                     f32x4 y;
 #pragma unroll
-                    for (int c = 0; c < 4; ++c) y[c] = x_silu(acc[mt][i][c]) * acc[mt][i + NT / 2][c];
+                    for (int c = 0; c < 4; ++c) y[c] = x_silu(x_value(acc[mt][i])[c]) * x_value(acc[mt][i + NT / 2])[c];
                     return y;
                 });
             else
                 x_lines_out<DT, MT, NT, 32, REDUCE ? 2 : 0>(own, to, p->out_f32, (int)p->ldo, t.m_end - row0, cols - first_col, lane,
-                                                            [&](int mt, int i) __attribute__((always_inline)) { return acc[mt][i]; });
+                                                            [&](int mt, int i) __attribute__((always_inline)) { return x_value(acc[mt][i]); });
         } else if constexpr (!REDUCE) {
             /* the launch has a workgroup per tile, and what was brought behind its last step is nothing: the stages are free */
             constexpr int PASS = 2, ROWS = PASS * 32, LD = TN + 4;
@@ -446,7 +456,7 @@ expert_gemm_wide_kernel(XgemmParams p)
                 for (int h = 0; h < PASS; ++h)
 #pragma unroll
                     for (int nt = 0; nt < NT; ++nt)
-                        *reinterpret_cast<f32x4 *>(sums + (h * 32 + wm * 16 + (lane & 15)) * LD + col_of(nt) + q4) = acc[pass * PASS + h][nt];
+                        *reinterpret_cast<f32x4 *>(sums + (h * 32 + wm * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
                 __syncthreads();
                 const int quads = tile_cols / 4;
 #pragma unroll 1

@@ -50,6 +50,12 @@ struct Library {
     decltype(&zbal_moe_expert_linear_backward) expert_linear_backward;
     decltype(&zbal_moe_expert_linear_workspace_size) expert_linear_workspace;
     decltype(&zbal_combine_normal_backward) combine_backward;
+    decltype(&zbal_moe_rms_norm) rms_norm;
+    decltype(&zbal_moe_rms_norm_backward) rms_norm_backward;
+    decltype(&zbal_moe_rms_norm_workspace_size) rms_norm_workspace;
+    decltype(&zbal_moe_quantize_rows) quantize_rows;
+    decltype(&zbal_moe_expert_linear_int8) expert_linear_int8;
+    decltype(&zbal_moe_expert_linear_int8_workspace_size) expert_linear_int8_workspace;
 };
 Library L;
 PyObject *g_check = nullptr;        /* capi.check(op, code): raises ZbalError */
@@ -771,6 +777,108 @@ PyObject *combine_backward(PyObject *const *args, Py_ssize_t nargs)
     return tuple_of(wrap(gx), wrap(gw));
 }
 
+/* an operand of x's shape, or None */
+Info like(const Frame &f, int i, const at::Tensor &x, const char *text)
+{
+    if (f.args[i] == Py_None) return Info();
+    const at::Tensor &t = local(f, i);
+    if (t.sizes() != x.sizes()) fail(PyExc_ValueError, text);
+    return Info(t);
+}
+Info norm_weight(const Frame &f, int i, const at::Tensor &x)
+{
+    if (f.args[i] == Py_None) return Info();
+    const at::Tensor &t = local(f, i);
+    if (t.dim() != 1 || t.size(0) != x.size(1)) fail(PyExc_ValueError, "weight must be [hidden]");
+    return Info(t);
+}
+
+/* (comm, dev, x, weight, residual, eps, norm wanted, int8 wanted) -> (y, q, scales, total) */
+PyObject *rms_norm(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 8);
+    const at::Tensor &x = local(f, 2);
+    dims(x, 2, "x must be [tokens, hidden]");
+    const double eps = number(args[5]);
+    const Info ix(x), iw = norm_weight(f, 3, x), ir = like(f, 4, x, "residual must have the shape of x");
+    at::Tensor y, q, scales, total;
+    if (f.n(6)) y = f.empty(x.sizes(), x.scalar_type());
+    if (f.n(7)) {
+        q = f.empty(x.sizes(), at::kChar);
+        scales = f.empty({x.size(0)}, at::kFloat);
+    }
+    if (args[4] != Py_None) total = f.empty(x.sizes(), x.scalar_type());
+    const Info iy = info_or_null(y), iq = info_or_null(q), is = info_or_null(scales), it = info_or_null(total);
+    check("zbal_moe_rms_norm", unlocked([&] { return L.rms_norm(*ix, *iw, *ir, eps, *iy, *it, *iq, *is, f.comm, f.stream, 0); }));
+    return tuple_of(wrap_or_none(y), wrap_or_none(q), wrap_or_none(scales), wrap_or_none(total));
+}
+
+/* (comm, dev, grad, x, weight, grad of the total, eps, weight's gradient wanted, in 32 bits) -> (grad of x, of weight) */
+PyObject *rms_norm_backward(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 9);
+    const at::Tensor &x = local(f, 3);
+    dims(x, 2, "x must be [tokens, hidden]");
+    if (args[2] == Py_None) fail(PyExc_TypeError, "expected a tensor");
+    const double eps = number(args[6]);
+    const Info ix(x), ig = like(f, 2, x, "grad must have the shape of x"), iw = norm_weight(f, 4, x), it = like(f, 5, x, "grad_total must have the shape of x");
+    const at::Tensor gx = f.empty(x.sizes(), x.scalar_type());
+    at::Tensor gw, ws;
+    if (f.n(7)) {
+        gw = f.empty({x.size(1)}, f.n(8) ? at::kFloat : x.scalar_type());
+        const int64_t bytes = L.rms_norm_workspace(x.size(0), x.size(1));
+        if (bytes > 0) ws = f.empty({bytes}, at::kByte);
+    }
+    const Info igx(gx), igw = info_or_null(gw), iws = info_or_null(ws);
+    check("zbal_moe_rms_norm_backward", unlocked([&] { return L.rms_norm_backward(*ig, *ix, *iw, *it, eps, *igx, *igw, *iws, f.comm, f.stream, 0); }));
+    return tuple_of(wrap(gx), wrap_or_none(gw));
+}
+
+/* (comm, dev, x, counts, activation) -> (q, scales) */
+PyObject *quantize_rows(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 5);
+    const at::Tensor &x = local(f, 2);
+    dims(x, 2, "x must be [rows, width]");
+    const zbal_activation_t act = (zbal_activation_t)f.n(4);
+    const Info ix(x), ic = local_or_null(f, 3);
+    const at::Tensor q = f.empty({x.size(0), act == ZBAL_ACTIVATION_SWIGLU ? x.size(1) / 2 : x.size(1)}, at::kChar), scales = f.empty({x.size(0)}, at::kFloat);
+    const Info iq(q), is(scales);
+    check("zbal_moe_quantize_rows", unlocked([&] { return L.quantize_rows(*ix, *ic, act, *iq, *is, f.comm, f.stream, 0); }));
+    return tuple_of(wrap(q), wrap(scales));
+}
+
+/* (comm, dev, x, x scales, weight, weight scales, counts, bias, activation, residual, output type: 0 bf16, 1 fp16, 2 fp32, out) -> y */
+PyObject *expert_linear_int8(PyObject *const *args, Py_ssize_t nargs)
+{
+    const OnDevice here(args, nargs);
+    const Frame f(args, nargs, 12);
+    const at::Tensor &x = local(f, 2), &xs = local(f, 3), &w = local(f, 4);
+    const LinearShape s(x, w, f.n(8), true);
+    if (xs.dim() != 1 || xs.size(0) != s.rows) fail(PyExc_ValueError, "x_scales must be [rows]");
+    const at::ScalarType yt = f.n(10) == 0 ? at::kBFloat16 : (f.n(10) == 1 ? at::kHalf : at::kFloat);
+    at::Tensor y, ws;
+    if (args[11] == Py_None) {
+        y = f.empty({s.rows, s.cols}, yt);
+    } else {
+        y = local(f, 11);
+        if (y.scalar_type() != yt || y.dim() != 2 || y.size(0) != s.rows || y.size(1) != s.cols) fail(PyExc_ValueError, "out has another shape or type");
+    }
+    const int64_t bytes = L.expert_linear_int8_workspace(s.rows, s.k, s.n, s.experts, s.act);
+    if (bytes > 0) ws = f.empty({bytes}, at::kByte);
+    Info iw(w);
+    iw.ti.reserved[0] = ZBAL_WEIGHT_FORMAT_NK;
+    const Info ix(x), ixs(xs), isc = per_expert(f, 5, s, "weight_scales must be [experts, n]"), ic = counts_of(f, 6, s),
+               ib = per_expert(f, 7, s, "bias must be [experts, n]"), iy(y), iws = info_or_null(ws), ir = like(f, 9, y, "residual must have the output's shape");
+    check("zbal_moe_expert_linear_int8", unlocked([&] {
+              return L.expert_linear_int8(*ix, *ixs, *iw, *isc, *ic, *ib, s.act, *ir, *iy, *iws, f.comm, f.stream, 0);
+          }));
+    return wrap(y).release();
+}
+
 /* (tensors,) -> whether every one of them is marked as pre-packed */
 PyObject *all_prepacked(PyObject *const *args, Py_ssize_t nargs)
 {
@@ -813,7 +921,11 @@ PyObject *bind(PyObject *const *args, Py_ssize_t nargs)
         !find(h, "zbal_moe_expert_linear", &L.expert_linear) ||
         !find(h, "zbal_moe_expert_linear_backward", &L.expert_linear_backward) ||
         !find(h, "zbal_moe_expert_linear_workspace_size", &L.expert_linear_workspace) ||
-        !find(h, "zbal_combine_normal_backward", &L.combine_backward))
+        !find(h, "zbal_combine_normal_backward", &L.combine_backward) || !find(h, "zbal_moe_rms_norm", &L.rms_norm) ||
+        !find(h, "zbal_moe_rms_norm_backward", &L.rms_norm_backward) ||
+        !find(h, "zbal_moe_rms_norm_workspace_size", &L.rms_norm_workspace) || !find(h, "zbal_moe_quantize_rows", &L.quantize_rows) ||
+        !find(h, "zbal_moe_expert_linear_int8", &L.expert_linear_int8) ||
+        !find(h, "zbal_moe_expert_linear_int8_workspace_size", &L.expert_linear_int8_workspace))
         throw PyFail{};
     Py_INCREF(args[1]);
     Py_XSETREF(g_check, args[1]);
@@ -828,7 +940,8 @@ PyMethodDef g_methods[] = {ZB_METHOD(bind),     ZB_METHOD(topk_route),  ZB_METHO
                            ZB_METHOD(dispatch), ZB_METHOD(dispatch_counts), ZB_METHOD(combine), ZB_METHOD(ll_dispatch),
                            ZB_METHOD(ll_combine), ZB_METHOD(fused),     ZB_METHOD(group_route),
                            ZB_METHOD(group_route_backward), ZB_METHOD(expert_linear), ZB_METHOD(expert_linear_backward),
-                           ZB_METHOD(combine_backward), ZB_METHOD(all_prepacked), ZB_METHOD(current_stream),
+                           ZB_METHOD(combine_backward), ZB_METHOD(rms_norm), ZB_METHOD(rms_norm_backward), ZB_METHOD(quantize_rows),
+                           ZB_METHOD(expert_linear_int8), ZB_METHOD(all_prepacked), ZB_METHOD(current_stream),
                            {nullptr, nullptr, 0, nullptr}};
 PyModuleDef g_module = {PyModuleDef_HEAD_INIT, "_zbal_torch", nullptr, -1, g_methods, nullptr, nullptr, nullptr, nullptr};
 

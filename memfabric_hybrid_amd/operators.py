@@ -88,6 +88,9 @@ def _is_fp32(what, dtype, x):
     return int(dtype == torch.float32)
 
 
+_OUT_TYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
 class OperatorBuffer:
     """One-rank MoE layout / dispatch / combine / fused-MoE operators on worst-case-sized tensors."""
 
@@ -160,6 +163,28 @@ class OperatorBuffer:
             self._comm, self._dev, grad, x, weight, tokens_per_expert, _code(capi.ACTIVATIONS, "activation", activation), preact,
             int(bool(transposed)), int(bool(bias)), _is_fp32("weight_grad_dtype", weight_grad_dtype, x), int(bool(need_x)),
             int(bool(need_weight)))
+
+    # -- around the int8 exchange (extension) ----------------------------------------------------
+    def rms_norm(self, x, weight=None, residual=None, eps=1e-6, quantize=False, need_norm=True):
+        """zbal_moe_rms_norm: returns (y, q, scales, total), None for what was not asked for."""
+        return self.native.rms_norm(self._comm, self._dev, x, weight, residual, eps, int(bool(need_norm)), int(bool(quantize)))
+
+    def rms_norm_backward(self, grad, x, weight=None, grad_total=None, eps=1e-6, weight_grad_dtype=None, need_weight=True):
+        """zbal_moe_rms_norm_backward: returns (grad_x, grad_weight or None)."""
+        return self.native.rms_norm_backward(self._comm, self._dev, grad, x, weight, grad_total, eps, int(bool(need_weight)),
+                                             _is_fp32("weight_grad_dtype", weight_grad_dtype, x))
+
+    def quantize_rows(self, x, tokens_per_expert=None, activation="none"):
+        """zbal_moe_quantize_rows: returns (q, scales)."""
+        return self.native.quantize_rows(self._comm, self._dev, x, tokens_per_expert, _code(capi.ACTIVATIONS, "activation", activation))
+
+    def expert_linear_int8(self, x, x_scales, weight, weight_scales, tokens_per_expert=None, bias=None, activation="none", residual=None,
+                           out_dtype=torch.bfloat16, out=None):
+        """zbal_moe_expert_linear_int8: returns y."""
+        if out_dtype not in _OUT_TYPES:
+            raise ValueError("out_dtype must be torch.bfloat16, torch.float16 or torch.float32")
+        return self.native.expert_linear_int8(self._comm, self._dev, x, x_scales, weight, weight_scales, tokens_per_expert, bias,
+                                              _code(capi.ACTIVATIONS, "activation", activation), residual, _OUT_TYPES[out_dtype], out)
 
     # -- normal mode -------------------------------------------------------------------------
     def get_dispatch_layout(self, topk_idx, num_experts):

@@ -221,7 +221,7 @@ expert_gemm_any_kernel(XgemmParams p)
             const int j = n0 + (up ? c - TN / 2 : c);
             if (row >= m_end || j >= cols) continue;
             const x_sum_t<DT> z = sums[r * LD + c];
-            if (p.splits > 1) reinterpret_cast<x_sum_t<DT> *>(p.partial)[((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + (up ? p.n_half : 0)] = z;
+            if (p.splits > 1) reinterpret_cast<x_sum_t<DT> *>(p.partial)[((int64_t)split * (REDUCE ? p.M : p.rows) + row) * p.ldp + j + (up ? p.up_at : 0)] = z;
             else if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, expert * p.out_stride + row * p.ldo + j, z);
             else if (!up)
                 x_finish<DT>(p, expert, row, j, x_scaled<DT>(p, expert, row, j, z), p.n_half ? x_scaled<DT>(p, expert, row, p.n_half + j, sums[r * LD + TN / 2 + c]) : 0.0f);
@@ -245,7 +245,7 @@ expert_join_kernel(XgemmParams p)
         if (whole) {
             for (int s = 0; s < p.splits; ++s) {
                 z += *reinterpret_cast<const x_sums_t<DT> *>(from + s * plane);
-                if (p.n_half) up += *reinterpret_cast<const x_sums_t<DT> *>(from + s * plane + p.n_half);
+                if (p.n_half) up += *reinterpret_cast<const x_sums_t<DT> *>(from + s * plane + p.up_at);
             }
             if constexpr (REDUCE) x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, z);
             else x_finish4<DT>(p, 0, row, j, x_scaled4<DT>(p, 0, row, j, z), p.n_half ? x_scaled4<DT>(p, 0, row, p.n_half + j, up) : f32x4{0.0f, 0.0f, 0.0f, 0.0f});
@@ -254,7 +254,7 @@ expert_join_kernel(XgemmParams p)
                 x_sum_t<DT> zc = 0, uc = 0;
                 for (int s = 0; s < p.splits; ++s) {
                     zc += from[s * plane + c];
-                    if (p.n_half) uc += from[s * plane + p.n_half + c];
+                    if (p.n_half) uc += from[s * plane + p.up_at + c];
                 }
                 if constexpr (REDUCE) x_store<DT>(p.out, p.out_f32, row * p.ldo + j + c, zc);
                 else x_finish<DT>(p, 0, row, j + c, x_scaled<DT>(p, 0, row, j + c, zc), p.n_half ? x_scaled<DT>(p, 0, row, p.n_half + j + c, uc) : 0.0f);
@@ -267,6 +267,33 @@ expert_join_kernel(XgemmParams p)
             float z = 0.0f;
             for (int s = 0; s < p.splits; ++s) z += p.bias_partial[s * p.bias_ldp + i];
             x_store<DT>(p.bias_grad, p.out_f32, i, z);
+        }
+    }
+}
+
+/*
+ * Rows of int8 whose length is no multiple of 16 bytes, copied to rows of one that is, zeros behind their ends, so that the tiles for aligned operands can have
+ * them: the rows of x, then those of W. `lanes` of them to a row, sixteen bytes each at a time; the last of a row are taken from its last sixteen.
+ */
+struct XAlign { const uint8_t *from[2]; uint8_t *to[2]; int64_t rows[2]; int k, k_to, lanes; };
+__global__ void __launch_bounds__(256)
+expert_align_kernel(XAlign p)
+{
+    const int per_block = 256 / p.lanes, c0 = (threadIdx.x % p.lanes) * 16;
+    const int64_t step = (int64_t)gridDim.x * per_block;
+    for (int64_t r = (int64_t)blockIdx.x * per_block + threadIdx.x / p.lanes; r < p.rows[0] + p.rows[1]; r += step) {
+        const int of = r >= p.rows[0];
+        const int64_t row = of ? r - p.rows[0] : r;
+        const uint8_t *from = p.from[of] + row * p.k;
+        uint8_t *to = p.to[of] + row * p.k_to;
+#pragma unroll 4
+        for (int c = c0; c < p.k; c += p.lanes * 16) {
+            const int at = c < p.k - 16 ? c : p.k - 16, away = (c - at) * 8;        /* the bits that come before c are shifted out */
+            const u32x4 v = x_loose(from + at);
+            uint64_t lo = (uint64_t)v[1] << 32 | v[0], hi = (uint64_t)v[3] << 32 | v[2];
+            if (away >= 64) { lo = hi; hi = 0; }
+            if (away & 63) { lo = lo >> (away & 63) | hi << (64 - (away & 63)); hi >>= away & 63; }
+            *reinterpret_cast<u32x4 *>(to + c) = u32x4{(uint32_t)lo, (uint32_t)(lo >> 32), (uint32_t)hi, (uint32_t)(hi >> 32)};
         }
     }
 }
@@ -408,6 +435,8 @@ inline bool rows_are_aligned(const XgemmParams &p) { return p.lda % 8 == 0 && p.
 
 /* how a product is cut: the tiles, and the parts along k whose sums a second launch adds up */
 enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT, CUT_ROWS };
+/* columns of the parts' sums: either half of a swiglu's starts at a multiple of four */
+inline int64_t parts_width(const XgemmParams &p) { return p.n_half ? (p.n_half + 3) / 4 * 8 : (p.N + 3) / 4 * 4; }
 struct Plan {
     Cut cut;
     int splits;
@@ -470,28 +499,23 @@ Plan plan_product(const XgemmParams &p, bool reduce, bool b_cols)
         }
     }
     if (plan.splits > 1) {
-        const int64_t ldp = (p.N + 3) / 4 * 4, bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
+        const int64_t ldp = parts_width(p), bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
         plan.bytes = plan.splits * (rows * ldp + (reduce ? bias_ldp : 0)) * 4;
     }
     return plan;
 }
 
-template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, void *workspace, int64_t workspace_bytes, hipStream_t st)
+template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, Plan plan, void *workspace, int64_t workspace_bytes, hipStream_t st)
 {
-    Plan plan = plan_product(p, REDUCE, REDUCE || B_TR);
     if (plan.bytes > workspace_bytes || !workspace) plan.splits = 1;
     if (plan.splits > 1) {
         p.splits = plan.splits;
-        p.ldp = (p.N + 3) / 4 * 4;
+        p.ldp = parts_width(p);
+        p.up_at = (p.n_half + 3) / 4 * 4;
         p.partial = (float *)workspace;
         p.bias_partial = p.partial + (int64_t)p.splits * (REDUCE ? p.M : p.rows) * p.ldp;
         p.bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
     }
-    if constexpr (x_is_i8<DT>)
-        if (plan.cut == CUT_ANY || plan.cut == CUT_ANY_64 || plan.cut == CUT_ANY_16 || plan.cut == CUT_SHORT) {
-            p.lda = p.ldb = p.K = p.k_bytes;
-            p.b_stride = (int64_t)p.k_bytes * p.N;
-        }
     switch (plan.cut) {
         case CUT_WIDE: launch_wide<DT, REDUCE, B_TR>(p, st); break;
         case CUT_128: launch_direct<DT, REDUCE, B_TR, 128, 128, 2, 4, 4>(p, st); break;
@@ -520,12 +544,13 @@ template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, voi
 
 template <bool REDUCE> void launch_types(const XgemmParams &p, int dtype, bool b_tr, void *ws, int64_t ws_bytes, hipStream_t st)
 {
+    const Plan plan = plan_product(p, REDUCE, REDUCE || b_tr);
     if (dtype == ZDT_BF16) {
-        if (b_tr) launch_product<ZDT_BF16, REDUCE, true>(p, ws, ws_bytes, st);
-        else if constexpr (!REDUCE) launch_product<ZDT_BF16, REDUCE, false>(p, ws, ws_bytes, st);
+        if (b_tr) launch_product<ZDT_BF16, REDUCE, true>(p, plan, ws, ws_bytes, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_BF16, REDUCE, false>(p, plan, ws, ws_bytes, st);
     } else {
-        if (b_tr) launch_product<ZDT_FP16, REDUCE, true>(p, ws, ws_bytes, st);
-        else if constexpr (!REDUCE) launch_product<ZDT_FP16, REDUCE, false>(p, ws, ws_bytes, st);
+        if (b_tr) launch_product<ZDT_FP16, REDUCE, true>(p, plan, ws, ws_bytes, st);
+        else if constexpr (!REDUCE) launch_product<ZDT_FP16, REDUCE, false>(p, plan, ws, ws_bytes, st);
     }
 }
 
@@ -582,18 +607,13 @@ XgemmParams rows_gradient_params(const zbalhip_expert_linear_t *d)
     return p;
 }
 
-/*
- * Two k of int8 are one element: the tiles then move, and multiply in the same time, what they do in half precision, and the plan's rule holds as it
- * is. Rows that are no multiple of 16 bytes are not aligned, whatever half of them is; fewer than 16 k are short.
- */
+/* sizes of an int8 product, and how its rows lie: `k` bytes each */
 XgemmParams int8_params(const zbalhip_expert_linear_int8_t *d)
 {
     XgemmParams p = common_params(d);
-    p.k_bytes = (int)d->k;
-    p.lda = p.ldb = d->k % 16 == 0 ? d->k / 2 : 1;
+    p.lda = p.ldb = p.K = (int)d->k;
     p.b = (const uint16_t *)d->weight;
-    p.b_stride = d->k * d->n / 2;
-    p.K = (int)d->k / 2;
+    p.b_stride = d->k * d->n;
     p.N = (int)d->n;
     p.act = d->activation;
     p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
@@ -601,6 +621,97 @@ XgemmParams int8_params(const zbalhip_expert_linear_int8_t *d)
     p.b_scale = d->weight_scales;
     p.b_scale_f32 = d->weight_scales_are_f32;
     return p;
+}
+/* two k to an element, as the tiles for aligned operands count them; `k` a multiple of 16 */
+void in_pairs(XgemmParams *p, int k)
+{
+    p->lda = p->ldb = p->K = k / 2;
+    p->b_stride = (int64_t)k * p->N / 2;
+}
+
+/*
+ * The cut of an int8 product that takes least time, by a model of a kind's launch: rounds of workgroups, each of a fixed time and one for every step of 128 k (with
+ * few workgroups on the card, and with as many as run side by side), joined with the time that reading the weights takes as the root of the sum of their squares.
+ * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 72 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
+ * unaligned rows: the kind that it picks takes 1.02 times the best one's on average, 1.28 at most (2868 rows over 32 experts of 384 x 5056: 64 x 128 43 us, wide 34).
+ * Half precision's rule, for the same tiles, has 1.11 and 3.65 here: 512 x 512 x 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of
+ * 2048 x 1024 128 x 128 71, wide 56.
+ */
+struct Int8Cut { Cut cut; int tm, tn, at_once; double fixed, alone, full, stream; };
+const Int8Cut int8_cuts[] = {{CUT_WIDE, 256, 256, 1, 4.85, 0.9, 1.45, 7.0e6}, {CUT_128, 128, 128, 1, 2.56, 0.37, 0.66, 7.0e6}, {CUT_64_128, 64, 128, 2, 2.46, 0.44, 0.74, 6.4e6},
+                             {CUT_64, 64, 64, 2, 2.11, 0.25, 0.48, 7.0e6}, {CUT_32, 32, 128, 2, 2.2, 0.22, 0.48, 5.7e6}, {CUT_16, 16, 64, 2, 2.45, 0.14, 0.21, 5.25e6},
+                             {CUT_ROWS, 16, 16, 4, 4.22, 0.02, 0.52, 7.0e6}};
+const Int8Cut int8_any_cuts[] = {{CUT_ANY, 128, 128, 2, 6.55, 1.25, 1.9, 7.0e6}, {CUT_ANY_64, 64, 64, 4, 3.95, 0.48, 1.64, 3.6e6}, {CUT_ANY_16, 16, 128, 4, 2.59, 0.51, 1.68, 4.1e6}};
+
+/* p with k in bytes */
+Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
+{
+    *us = 0.0;
+    if (p.K < 16) return {CUT_SHORT, 1, 0};
+    const double per_expert = (double)p.rows / p.experts, steps = (p.K + 127) / 128;
+    const double reached = p.rows >= 4 * p.experts ? p.experts : p.experts * (1.0 - pow(1.0 - 1.0 / p.experts, p.rows));
+    const int cols = p.n_half ? p.n_half : p.N;
+    Plan plan = {CUT_SHORT, 1, 0};
+    for (int i = 0; i < (aligned ? 7 : 3); ++i) {
+        const Int8Cut &c = aligned ? int8_cuts[i] : int8_any_cuts[i];
+        const int tile_cols = p.n_half && c.cut != CUT_ROWS ? c.tn / 2 : c.tn;
+        double m_tiles = (p.rows + c.tm - 1) / c.tm;
+        if (p.experts > 1)       /* every expert ends with half a tile, on average, and has one at least */
+            m_tiles = per_expert < c.tm * 0.25 ? reached : fmax(p.experts * (per_expert / c.tm + 0.5), reached);
+        const double tiles = m_tiles * ((cols + tile_cols - 1) / tile_cols), memory = reached * p.N * p.K / c.stream;
+        for (int splits = 1; splits <= 8; splits *= 2) {
+            if (splits > 1 && (p.experts > 1 || c.cut == CUT_WIDE || c.cut == CUT_ROWS || steps / splits < 4 || tiles * splits > 2048)) break;
+            const double cus = tiles * splits / 256.0, rounds = cus / c.at_once, part_steps = ceil(steps / splits);
+            double t;
+            if (rounds <= 1.0) {
+                const double beside = c.at_once == 1 ? fmin(cus, 1.0) : fmin(1.0, fmax(0.0, cus - 1.0) / (c.at_once - 1));
+                t = c.fixed + (c.alone + (c.full - c.alone) * beside) * part_steps;
+            } else {
+                t = (c.fixed + c.full * part_steps) * (rounds < 4.0 ? ceil(rounds) : rounds + 0.5);
+            }
+            t = 3.0 + sqrt(t * t + memory * memory);
+            if (splits > 1) t += 2.5 + (double)splits * p.rows * p.N * 8 / 5e6;      /* the parts' sums, written and read again */
+            if (*us == 0.0 || t < *us) {
+                *us = t;
+                plan.cut = c.cut;
+                plan.splits = splits;
+            }
+        }
+    }
+    if (plan.splits > 1) plan.bytes = plan.splits * p.rows * parts_width(p) * 4;
+    return plan;
+}
+
+/*
+ * Rows that are not aligned: multiplied as they lie, or copied to the workspace first, whichever the model expects to be done sooner. A copy is a launch, and writes
+ * both operands at 2.4 TB/s: 4093 x 4099 x 4093 194 us as it lies, 83 copied; 16 rows over 32 experts of 4001 x 1531 32 and 115.
+ */
+struct Int8Plan {
+    XgemmParams p;
+    Plan cut;
+    bool copies;
+    int64_t x_bytes, w_bytes, bytes;
+};
+constexpr int64_t X_MOST_COPIED = (int64_t)1 << 31;
+Int8Plan plan_int8(const zbalhip_expert_linear_int8_t *d, bool may_copy = true)
+{
+    Int8Plan plan = {};
+    plan.p = int8_params(d);
+    double us, copied_us;
+    plan.cut = plan_int8_cut(plan.p, d->k % 16 == 0, &us);
+    plan.bytes = plan.cut.bytes;
+    if (d->k % 16 == 0) {
+        in_pairs(&plan.p, (int)d->k);
+        return plan;
+    }
+    const int64_t k = (d->k + 15) / 16 * 16, x_bytes = d->rows * k, w_bytes = d->experts * d->n * k;
+    if (!may_copy || d->k < 16 || x_bytes + w_bytes > X_MOST_COPIED) return plan;
+    XgemmParams to = plan.p;
+    to.K = (int)k;
+    const Plan copied = plan_int8_cut(to, true, &copied_us);
+    if (copied_us + 2.5 + (double)(x_bytes + w_bytes) / 2.4e6 >= us) return plan;
+    in_pairs(&to, (int)k);
+    return {to, copied, true, x_bytes, w_bytes, x_bytes + w_bytes + copied.bytes};
 }
 
 XgemmParams weights_gradient_params(const zbalhip_expert_linear_t *d)
@@ -689,7 +800,7 @@ extern "C" int32_t zbalhip_expert_linear_backward(const zbalhip_expert_linear_t 
 extern "C" int64_t zbalhip_expert_linear_int8_workspace(const zbalhip_expert_linear_int8_t *d)
 {
     if (!int8_sizes_ok(d)) return -1;
-    return d->rows == 0 ? 0 : plan_product(int8_params(d), false, false).bytes;
+    return d->rows == 0 ? 0 : plan_int8(d).bytes;
 }
 
 extern "C" int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t *d, const void *x, const float *x_scales, const void *bias, int32_t bias_is_f32,
@@ -698,15 +809,28 @@ extern "C" int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t
     if (!int8_sizes_ok(d) || !d->weight || !d->weight_scales || (d->experts > 1 && !d->counts)) return ZBALHIP_INVALID;
     if (d->rows == 0) return ZBALHIP_OK;
     if (!x || !x_scales || !y) return ZBALHIP_INVALID;
-    XgemmParams p = int8_params(d);
+    Int8Plan plan = plan_int8(d);
+    if (plan.copies && (!workspace || workspace_bytes < plan.x_bytes + plan.w_bytes)) plan = plan_int8(d, false);
+    XgemmParams p = plan.p;
     p.a = (const uint16_t *)x;
+    if (plan.copies) {
+        uint8_t *to = (uint8_t *)workspace;
+        XAlign c = {{(const uint8_t *)x, (const uint8_t *)d->weight}, {to, to + plan.x_bytes}, {d->rows, d->experts * d->n}, (int)d->k, p.K * 2, 1};
+        while (c.lanes < 64 && c.lanes * 16 < c.k) c.lanes *= 2;
+        const int64_t blocks = (c.rows[0] + c.rows[1] + 256 / c.lanes - 1) / (256 / c.lanes);
+        zb_launch(expert_align_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream, c);
+        p.a = (const uint16_t *)c.to[0];
+        p.b = (const uint16_t *)c.to[1];
+        workspace = c.to[1] + plan.w_bytes;
+        workspace_bytes -= plan.x_bytes + plan.w_bytes;
+    }
     p.a_scale = x_scales;
     p.out = y;
     p.out_f32 = d->y_dtype == ZDT_FP32;
     p.bias = bias;
     p.bias_f32 = bias_is_f32;
     p.residual = residual;
-    if (d->y_dtype == ZDT_FP16) launch_product<XI8 | ZDT_FP16, false, false>(p, workspace, workspace_bytes, (hipStream_t)stream);
-    else launch_product<XI8 | ZDT_BF16, false, false>(p, workspace, workspace_bytes, (hipStream_t)stream);
+    if (d->y_dtype == ZDT_FP16) launch_product<XI8 | ZDT_FP16, false, false>(p, plan.cut, workspace, workspace_bytes, (hipStream_t)stream);
+    else launch_product<XI8 | ZDT_BF16, false, false>(p, plan.cut, workspace, workspace_bytes, (hipStream_t)stream);
     return zbalhip_check_launch();
 }

@@ -74,11 +74,21 @@ __device__ __forceinline__ void x_lines_out(uint32_t own, void *out, int f32, in
                 }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
                 const int at = i0 * (F32 ? 64 : 32) + c_out * 16;
-                const bool in = at < cols * width && r_out < 16;
+                const bool some = at < cols * width && r_out < 16, in = some && (!x_is_i8<DT> || at + 16 <= cols * width);
                 const uint32_t off = in ? (uint32_t)((mt * ROW_STEP + r_out) * ldo_b + at) : XNOWHERE;
                 __builtin_amdgcn_raw_buffer_store_b128(*(lds128_t)(uintptr_t)from, to, (int)off, 0, CACHE);
                 if constexpr (AT_ONCE < 16)
                     __builtin_amdgcn_raw_buffer_store_b128(*(lds128_t)(uintptr_t)(from + 1024), to, (int)(in ? off + 8 * ldo_b : XNOWHERE), 0, CACHE);
+                if (x_is_i8<DT> && some && !in)              /* a row's last sixteen bytes, not all of which are its own */
+#pragma unroll
+                    for (int half = 0; half < (AT_ONCE < 16 ? 2 : 1); ++half)
+#pragma unroll
+                        for (int e = 0; e < 16 / (F32 ? 4 : 2) - 1; ++e) {
+                            const uint32_t src = from + half * 1024 + e * (F32 ? 4 : 2), at_e = (uint32_t)((mt * ROW_STEP + r_out + half * 8) * ldo_b + at + e * width);
+                            if (at + e * width >= cols * width) continue;
+                            if constexpr (F32) __builtin_amdgcn_raw_buffer_store_b32(*(const uint32_t __attribute__((address_space(3))) *)(uintptr_t)src, to, (int)at_e, 0, CACHE);
+                            else __builtin_amdgcn_raw_buffer_store_b16(*(const uint16_t __attribute__((address_space(3))) *)(uintptr_t)src, to, (int)at_e, 0, CACHE);
+                        }
                 __builtin_amdgcn_fence(__ATOMIC_ACQ_REL, "wavefront");
             }
         }
@@ -294,20 +304,21 @@ expert_gemm_kernel(XgemmParams p)
     if constexpr (x_is_i8<DT>)
         if (p.splits == 1)
             x_scale_tile(acc, p.a_scale, p.b_scale, p.b_scale_f32, (int64_t)expert * p.N, m_end, [&](int mt) { return row0 + mt * 16 + (lane & 15); }, [&](int nt) {
-                const bool up = p.n_half && nt >= (NT + 1) / 2;
+                const bool up = p.n_half && nt >= NT / 2;
                 const int j = (cols - cols_left) + (up ? nt - NT / 2 : nt) * 16 + q4;
-                return j < cols ? j + (up ? p.n_half : 0) : -1;
+                return XCols{j + (up ? p.n_half : 0), cols - j};
             });
     const bool plain = REDUCE || p.splits > 1 || (!p.bias && !p.residual && !p.preact && (p.act == ACT_NONE || p.act == ACT_SWIGLU));
     if (plain) {
         __syncthreads();
         if (p.splits > 1) {
+            const int parts_left = x_is_i8<DT> ? (cols_left + 3) & ~3 : cols_left;       /* rows of sums are padded to four */
             float *to = p.partial + ((int64_t)split * (REDUCE ? p.M : p.rows) + row0) * p.ldp + (cols - cols_left);
             if (NT > 1 && p.n_half) {
-                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
-                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to + p.n_half, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i + NT / 2]); });
+                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to, 1, (int)p.ldp, rows_left, parts_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
+                x_lines_out<DT, MT, (NT > 1 ? NT / 2 : 1), 16, 0>(own, to + (x_is_i8<DT> ? p.up_at : p.n_half), 1, (int)p.ldp, rows_left, parts_left, lane, [&](int mt, int i) { return x_value(acc[mt][i + NT / 2]); });
             } else {
-                x_lines_out<DT, MT, NT, 16, 0>(own, to, 1, (int)p.ldp, rows_left, cols_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
+                x_lines_out<DT, MT, NT, 16, 0>(own, to, 1, (int)p.ldp, rows_left, parts_left, lane, [&](int mt, int i) { return x_value(acc[mt][i]); });
             }
             return;
         }
@@ -353,7 +364,7 @@ expert_gemm_kernel(XgemmParams p)
             if (!up) {
                 f32x4 other = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (p.n_half) other = *reinterpret_cast<const f32x4 *>(sums + r * LD + TN / 2 + c);
-                x_finish4<DT>(p, expert, row, j, z, other);
+                x_finish_some<DT>(p, expert, row, j, cols - j, z, other);
             }
         }
     }

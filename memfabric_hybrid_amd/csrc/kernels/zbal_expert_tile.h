@@ -33,7 +33,6 @@ struct XgemmParams {
     int counts_i64, experts;
     int rows;                    /* of the token-side tensors */
     int M, N, K;                 /* M: REDUCE only; K: not REDUCE */
-    int k_bytes;                 /* int8: K counts pairs of them, this one each */
     int n_half;                  /* swiglu: N / 2, where the up columns start; else 0 */
     void *out;
     int64_t ldo, out_stride;
@@ -50,6 +49,7 @@ struct XgemmParams {
     float *partial;              /* split along k: [splits][rows of C][ldp] sums instead of out, and [splits][bias_ldp] of the bias's */
     float *bias_partial;
     int64_t ldp, bias_ldp;
+    int up_at;                   /* where the up columns start in a row of parts' sums */
     int splits;
     int through_lds;             /* the wide kernel's epilogue: more than a swiglu, with a workgroup per tile */
 };
@@ -311,17 +311,30 @@ template <int DT> __device__ __forceinline__ void x_finish(const XgemmParams &p,
     x_store<DT>(p.out, p.out_f32, row * p.ldo + j, y);
 }
 
-/* four values, where every row of outputs, bias and residual starts at a multiple of four and is one of four long */
+/*
+ * Four values, where every row of outputs, bias and residual starts at a multiple of four and is one of four long. In int8 rows start, and end, anywhere, which
+ * loads and stores of several elements allow; what is less than four is not loaded or stored here.
+ */
+typedef f32x4 __attribute__((aligned(4))) x_floats_t;
+typedef u32x2 __attribute__((aligned(2))) x_halves_t;
 template <int DT> __device__ __forceinline__ f32x4 x_load4(const void *p, int f32, int64_t i)
 {
-    if (f32) return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
-    const u32x2 h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i);
+    if (f32) {
+        if constexpr (x_is_i8<DT>) return *reinterpret_cast<const x_floats_t *>(static_cast<const float *>(p) + i);
+        else return *reinterpret_cast<const f32x4 *>(static_cast<const float *>(p) + i);
+    }
+    u32x2 h;
+    if constexpr (x_is_i8<DT>) h = *reinterpret_cast<const x_halves_t *>(static_cast<const uint16_t *>(p) + i);
+    else h = *reinterpret_cast<const u32x2 *>(static_cast<const uint16_t *>(p) + i);
     constexpr int H = x_half<DT>;
     return f32x4{zb_half_to_f32<H>(h[0] & 0xffffu), zb_half_to_f32<H>(h[0] >> 16), zb_half_to_f32<H>(h[1] & 0xffffu), zb_half_to_f32<H>(h[1] >> 16)};
 }
 template <int DT> __device__ __forceinline__ void x_store4(void *p, int f32, int64_t i, const f32x4 &v)
 {
-    if (f32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
+    if constexpr (x_is_i8<DT>) {
+        if (f32) *reinterpret_cast<x_floats_t *>(static_cast<float *>(p) + i) = v;
+        else *reinterpret_cast<x_halves_t *>(static_cast<uint16_t *>(p) + i) = u32x2{zb_pack2_half<x_half<DT>>(v[0], v[1]), zb_pack2_half<x_half<DT>>(v[2], v[3])};
+    } else if (f32) *reinterpret_cast<f32x4 *>(static_cast<float *>(p) + i) = v;
     else *reinterpret_cast<u32x2 *>(static_cast<uint16_t *>(p) + i) = u32x2{zb_pack2_half<x_half<DT>>(v[0], v[1]), zb_pack2_half<x_half<DT>>(v[2], v[3])};
 }
 template <int DT> __device__ __forceinline__ void x_finish4(const XgemmParams &p, int expert, int64_t row, int j, f32x4 z, f32x4 up)
@@ -350,14 +363,15 @@ template <int DT> __device__ __forceinline__ float x_scaled(const XgemmParams &p
 }
 template <int DT> __device__ __forceinline__ f32x4 x_scaled4(const XgemmParams &p, int expert, int64_t row, int j, const x_sums_t<DT> &sum)
 {
-    if constexpr (x_is_i8<DT>) return __builtin_convertvector(sum, f32x4) * x_load4<ZDT_BF16>(p.b_scale, p.b_scale_f32, (int64_t)expert * p.N + j) * p.a_scale[row];
+    if constexpr (x_is_i8<DT>) return __builtin_convertvector(sum, f32x4) * x_load4<XI8 | ZDT_BF16>(p.b_scale, p.b_scale_f32, (int64_t)expert * p.N + j) * p.a_scale[row];
     else return sum;
 }
 
 /*
- * A lane's sub-tiles, where they are: integers become the bits of the values that they stand for. row(mt), col(nt): the row and the first of four columns
- * of W that it has there; rows and columns from row_end and -1 on are nobody's.
+ * A lane's sub-tiles, where they are: integers become the bits of the values that they stand for. row(mt): the row that it has there, nobody's from row_end
+ * on; col(nt): the first of its four columns and how many of them there are.
  */
+struct XCols { int first, there; };
 template <int MT, int NT, typename Row, typename Col>
 __device__ __forceinline__ void x_scale_tile(i32x4 (&acc)[MT][NT], const float *a_scale, const void *b_scale, int b_scale_f32, int64_t first_scale, int row_end, Row row, Col col)
 {
@@ -366,12 +380,26 @@ __device__ __forceinline__ void x_scale_tile(i32x4 (&acc)[MT][NT], const float *
     for (int mt = 0; mt < MT; ++mt) rows[mt] = a_scale[row(mt) < row_end ? row(mt) : row_end - 1];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
-        const int j = col(nt);
+        const XCols c = col(nt);
         f32x4 cols = {0.0f, 0.0f, 0.0f, 0.0f};
-        if (j >= 0) cols = x_load4<ZDT_BF16>(b_scale, b_scale_f32, first_scale + j);
+        if (c.there >= 4) {
+            cols = x_load4<XI8 | ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (i < c.there) cols[i] = x_load<ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first + i);
+        }
 #pragma unroll
         for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = __builtin_bit_cast(i32x4, __builtin_convertvector(acc[mt][nt], f32x4) * cols * rows[mt]);
     }
+}
+/* the last columns of a row one by one */
+template <int DT> __device__ __forceinline__ void x_finish_some(const XgemmParams &p, int expert, int64_t row, int j, int there, const f32x4 &z, const f32x4 &up)
+{
+    if (!x_is_i8<DT> || there >= 4) return x_finish4<DT>(p, expert, row, j, z, up);
+#pragma unroll
+    for (int i = 0; i < 3; ++i)
+        if (i < there) x_finish<DT>(p, expert, row, j + i, z[i], up[i]);
 }
 __device__ __forceinline__ f32x4 x_value(const f32x4 &v) { return v; }
 __device__ __forceinline__ f32x4 x_value(const i32x4 &v) { return __builtin_bit_cast(f32x4, v); }

@@ -424,7 +424,7 @@ expert_gemm_wide_kernel(XgemmParams p)
                          [&](int nt) {
                              const bool up = p->n_half && nt >= NT / 2;
                              const int j = first + (up ? nt - NT / 2 : nt) * 16;
-                             return j < cols ? j + (up ? p->n_half : 0) : -1;
+                             return XCols{j + (up ? p->n_half : 0), cols - j};
                          });
         }
         if (REDUCE || !p.through_lds) {
@@ -466,7 +466,7 @@ expert_gemm_wide_kernel(XgemmParams p)
                     const f32x4 z = *reinterpret_cast<const f32x4 *>(sums + r * LD + c);
                     f32x4 up = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (p.n_half) up = *reinterpret_cast<const f32x4 *>(sums + r * LD + TN / 2 + c);
-                    x_finish4<DT>(p, t.expert, row, j, z, up);
+                    x_finish_some<DT>(p, t.expert, row, j, cols - j, z, up);
                 }
             }
         }

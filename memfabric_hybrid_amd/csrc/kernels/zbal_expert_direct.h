@@ -243,6 +243,36 @@ expert_gemm_kernel(XgemmParams p)
         return !p.n_half ? wn * (NT * 16) + nt * 16 : (nt < NT / 2 ? wn * (NT * 8) + nt * 16 : TN / 2 + wn * (NT * 8) + (nt - NT / 2) * 16);
     };
 
+    constexpr int PASS = MT % 2 == 0 && WM * 32 * (TN + 4) * 4 <= STAGES * STAGE ? 2 : 1, ROWS = WM * PASS * 16, LD = TN + 4, QUADS = TN / 4;
+    /*
+     * What int8's epilogue reads, asked for in front of the first transfers: behind the last products it would be waited for, twice (1021 x 1001 x 1531 with gelu, bias and
+     * residual FIXME).
+     */
+    constexpr int TURNS = ROWS * QUADS / (WAVES * 64), ROW_STEP = WAVES * 64 / QUADS;
+    static_assert(!x_is_i8<DT> || (TURNS % 2 == 0 && TURNS * WAVES * 64 == ROWS * QUADS && ROW_STEP * QUADS == WAVES * 64), "a lane has the same columns in every turn");
+    const int q_col = tid % QUADS * 4, q_row = tid / QUADS, q_j = n0 + q_col;      /* its first of four columns of the tile, not of the up ones, and its first row of a pass */
+    const int q_there = p.splits == 1 && q_col < (p.n_half ? TN / 2 : TN) ? cols - q_j : 0;                    /* columns of it */
+    auto row_of = [&](int pass, int r) __attribute__((always_inline)) { return m0 + r / (PASS * 16) * (MT * 16) + pass * (PASS * 16) + r % (PASS * 16); };
+    XScales<MT, NT> scales;
+    u32x4 bias4 = {0, 0, 0, 0}, bias_up4 = bias4, residual4[x_is_i8<DT> ? MT / PASS * TURNS : 1];
+    if constexpr (x_is_i8<DT>) {
+        if (p.splits == 1)
+            x_load_scales(scales, p.a_scale, p.b_scale, p.b_scale_f32, (int64_t)expert * p.N, m_end, [&](int mt) { return m0 + wm * (MT * 16) + mt * 16 + (lane & 15); }, [&](int nt) {
+                const bool up = p.n_half && nt >= NT / 2;
+                const int j = n0 + wn * (p.n_half ? NT * 8 : NT * 16) + (up ? nt - NT / 2 : nt) * 16 + (lane >> 4) * 4;
+                return XCols{j + (up ? p.n_half : 0), cols - j};
+            });
+        if (p.bias) {
+            bias4 = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + q_j, q_there);
+            if (p.n_half) bias_up4 = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + p.n_half + q_j, q_there);
+        }
+        if (p.residual)
+#pragma unroll
+            for (int i = 0; i < MT / PASS * TURNS; ++i) {
+                const int row = row_of(i / TURNS, q_row + i % TURNS * ROW_STEP);
+                residual4[i] = x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + q_j, row < m_end ? q_there : 0);
+            }
+    }
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) bring_next(i);
     int stage = 0;
@@ -302,12 +332,7 @@ expert_gemm_kernel(XgemmParams p)
     static_assert(WAVES * 2048 <= STAGES * STAGE, "every wave has its own");
     /* parts' sums stay integers until they are joined */
     if constexpr (x_is_i8<DT>)
-        if (p.splits == 1)
-            x_scale_tile(acc, p.a_scale, p.b_scale, p.b_scale_f32, (int64_t)expert * p.N, m_end, [&](int mt) { return row0 + mt * 16 + (lane & 15); }, [&](int nt) {
-                const bool up = p.n_half && nt >= NT / 2;
-                const int j = (cols - cols_left) + (up ? nt - NT / 2 : nt) * 16 + q4;
-                return XCols{j + (up ? p.n_half : 0), cols - j};
-            });
+        if (p.splits == 1) x_scale_tile(acc, scales);
     const bool plain = REDUCE || p.splits > 1 || (!p.bias && !p.residual && !p.preact && (p.act == ACT_NONE || p.act == ACT_SWIGLU));
     if (plain) {
         __syncthreads();
@@ -339,7 +364,6 @@ expert_gemm_kernel(XgemmParams p)
      * Everything else through the LDS, up to two row sub-tiles of every wave at a time, so that the activations' code is there once: rows of TN
      * sums, and four more for the banks.
      */
-    constexpr int PASS = MT % 2 == 0 && WM * 32 * (TN + 4) * 4 <= STAGES * STAGE ? 2 : 1, ROWS = WM * PASS * 16, LD = TN + 4;
     static_assert(ROWS * LD * 4 <= STAGES * STAGE, "sums fit the stages");
     float *sums = reinterpret_cast<float *>(smem);
 #pragma unroll
@@ -351,11 +375,38 @@ expert_gemm_kernel(XgemmParams p)
             for (int nt = 0; nt < NT; ++nt)
                 *reinterpret_cast<f32x4 *>(sums + (wm * (PASS * 16) + h * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
         __syncthreads();
-        constexpr int QUADS = TN / 4;
+        if constexpr (x_is_i8<DT>) {
+            /* two rows at a time */
+            u32x4 waiting[TURNS];
+#pragma unroll
+            for (int i = 0; i < TURNS; ++i) waiting[i] = residual4[pass * TURNS + i];
+            const f32x4 b = x_of_raw4<DT>(bias4, p.bias_f32), bu = x_of_raw4<DT>(bias_up4, p.bias_f32);
+#pragma unroll 1
+            for (int i = 0; i < TURNS; i += 2) {
+                const u32x4 now[2] = {waiting[0], waiting[1]};
+#pragma unroll
+                for (int k = 2; k < TURNS; ++k) waiting[k - 2] = waiting[k];
+                if (q_there <= 0) continue;
+                f32x4 z[2], up[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const float *from = sums + (q_row + (i + h) * ROW_STEP) * LD + q_col;
+                    z[h] = *reinterpret_cast<const f32x4 *>(from) + b;
+                    if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + bu;
+                }
+                x_activate_all<2>(p, z, up);
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int row = row_of(pass, q_row + (i + h) * ROW_STEP);
+                    if (row < m_end) x_put<DT>(p, row, q_j, q_there, z[h], now[h]);
+                }
+            }
+            continue;
+        }
 #pragma unroll 1
         for (int i = tid; i < ROWS * QUADS; i += WAVES * 64) {
             const int r = i / QUADS, c = i % QUADS * 4;
-            const int row = m0 + r / (PASS * 16) * (MT * 16) + pass * (PASS * 16) + r % (PASS * 16);
+            const int row = row_of(pass, r);
             if (row >= m_end) continue;
             const f32x4 z = *reinterpret_cast<const f32x4 *>(sums + r * LD + c);
             const bool up = p.n_half && c >= TN / 2;
@@ -364,7 +415,7 @@ expert_gemm_kernel(XgemmParams p)
             if (!up) {
                 f32x4 other = {0.0f, 0.0f, 0.0f, 0.0f};
                 if (p.n_half) other = *reinterpret_cast<const f32x4 *>(sums + r * LD + TN / 2 + c);
-                x_finish_some<DT>(p, expert, row, j, cols - j, z, other);
+                x_finish4<DT>(p, expert, row, j, z, other);
             }
         }
     }

@@ -34,6 +34,20 @@ expert_gemm_rows_kernel(XgemmParams p)
     const uint16_t *b = p.b + t.expert * p.b_stride + (int64_t)(col < cols ? col : cols - 1) * p.ldb;
     const int64_t up = (int64_t)p.n_half * p.ldb;
 
+    /* what int8's epilogue reads, for the element that the lane will finish, asked for in front of the operands */
+    const int r_out = tid >> 4, c_out = n0 + (tid & 15);
+    const int64_t at = t.row_begin + r_out, first = (int64_t)t.expert * p.N;
+    const bool mine = tid < 256 && at < t.row_end && c_out < cols;
+    float row_scale = 0.0f, col_scale[2] = {0.0f, 0.0f}, bias[2] = {0.0f, 0.0f}, residual = 0.0f;
+    if (x_is_i8<DT> && mine) {
+        row_scale = p.a_scale[at];
+#pragma unroll
+        for (int i = 0; i < NT; ++i) {
+            col_scale[i] = x_load<ZDT_BF16>(p.b_scale, p.b_scale_f32, first + i * p.n_half + c_out);
+            if (p.bias) bias[i] = x_load<DT>(p.bias, p.bias_f32, first + i * p.n_half + c_out);
+        }
+        if (p.residual) residual = x_load<DT>(p.residual, p.out_f32, at * p.ldo + c_out);
+    }
     x_sums_t<DT> acc[NT];
     for (auto &v : acc) v = x_sums_t<DT>{0, 0, 0, 0};
     for (int k0 = wave * 64; k0 < p.K; k0 += WAVES * 64 * BATCH) {
@@ -64,14 +78,20 @@ expert_gemm_rows_kernel(XgemmParams p)
         for (int j = 0; j < 4; ++j) sums[wave][lane & 15][i * 16 + quad * 4 + j] = acc[i][j];
     __syncthreads();
     const int r = tid >> 4, c = tid & 15;
-    if (tid >= 256 || t.row_begin + r >= t.row_end || n0 + c >= cols) return;
+    if (!mine) return;
     x_sum_t<DT> z[2] = {0, 0};
 #pragma unroll
     for (int i = 0; i < NT; ++i)
 #pragma unroll
         for (int w = 0; w < WAVES; ++w) z[i] += sums[w][r][i * 16 + c];
-    const int64_t at = t.row_begin + r;
-    x_finish<DT>(p, t.expert, at, n0 + c, x_scaled<DT>(p, t.expert, at, n0 + c, z[0]), NT > 1 ? x_scaled<DT>(p, t.expert, at, p.n_half + n0 + c, z[1]) : 0.0f);
+    if constexpr (x_is_i8<DT>) {
+        float v[2];
+#pragma unroll
+        for (int i = 0; i < 2; ++i) v[i] = (float)z[i] * col_scale[i] * row_scale + bias[i];
+        x_store<DT>(p.out, p.out_f32, at * p.ldo + c_out, (NT > 1 ? x_silu(v[0]) * v[1] : x_activate(p.act, v[0])) + residual);
+    } else {
+        x_finish<DT>(p, t.expert, at, c_out, z[0], z[1]);
+    }
 }
 
 } // namespace

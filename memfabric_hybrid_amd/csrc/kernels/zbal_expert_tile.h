@@ -368,38 +368,92 @@ template <int DT> __device__ __forceinline__ f32x4 x_scaled4(const XgemmParams &
 }
 
 /*
- * A lane's sub-tiles, where they are: integers become the bits of the values that they stand for. row(mt): the row that it has there, nobody's from row_end
- * on; col(nt): the first of its four columns and how many of them there are.
+ * The scales of a lane's sub-tiles. row(mt): the row that it has there, nobody's from row_end on; col(nt): the first of its four columns and how many of them there
+ * are.
  */
 struct XCols { int first, there; };
+template <int MT, int NT> struct XScales { float rows[MT]; f32x4 cols[NT]; };
 template <int MT, int NT, typename Row, typename Col>
-__device__ __forceinline__ void x_scale_tile(i32x4 (&acc)[MT][NT], const float *a_scale, const void *b_scale, int b_scale_f32, int64_t first_scale, int row_end, Row row, Col col)
+__device__ __forceinline__ void x_load_scales(XScales<MT, NT> &s, const float *a_scale, const void *b_scale, int b_scale_f32, int64_t first_scale, int row_end, Row row, Col col)
 {
-    float rows[MT];
 #pragma unroll
-    for (int mt = 0; mt < MT; ++mt) rows[mt] = a_scale[row(mt) < row_end ? row(mt) : row_end - 1];
+    for (int mt = 0; mt < MT; ++mt) s.rows[mt] = a_scale[row(mt) < row_end ? row(mt) : row_end - 1];
 #pragma unroll
     for (int nt = 0; nt < NT; ++nt) {
         const XCols c = col(nt);
-        f32x4 cols = {0.0f, 0.0f, 0.0f, 0.0f};
+        s.cols[nt] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
         if (c.there >= 4) {
-            cols = x_load4<XI8 | ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first);
+            s.cols[nt] = x_load4<XI8 | ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first);
         } else {
 #pragma unroll
             for (int i = 0; i < 3; ++i)
-                if (i < c.there) cols[i] = x_load<ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first + i);
+                if (i < c.there) s.cols[nt][i] = x_load<ZDT_BF16>(b_scale, b_scale_f32, first_scale + c.first + i);
         }
-#pragma unroll
-        for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = __builtin_bit_cast(i32x4, __builtin_convertvector(acc[mt][nt], f32x4) * cols * rows[mt]);
     }
 }
-/* the last columns of a row one by one */
-template <int DT> __device__ __forceinline__ void x_finish_some(const XgemmParams &p, int expert, int64_t row, int j, int there, const f32x4 &z, const f32x4 &up)
+/* integers become the bits of the values that they stand for, where they are */
+template <int MT, int NT> __device__ __forceinline__ void x_scale_tile(i32x4 (&acc)[MT][NT], const XScales<MT, NT> &s)
 {
-    if (!x_is_i8<DT> || there >= 4) return x_finish4<DT>(p, expert, row, j, z, up);
 #pragma unroll
-    for (int i = 0; i < 3; ++i)
-        if (i < there) x_finish<DT>(p, expert, row, j + i, z[i], up[i]);
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = __builtin_bit_cast(i32x4, __builtin_convertvector(acc[mt][nt], f32x4) * s.cols[nt] * s.rows[mt]);
+}
+/* four values as they lie in memory, so that what is asked for early is waited for late; at the end of a row `there` of them */
+template <int DT> __device__ __forceinline__ u32x4 x_raw4(const void *p, int f32, int64_t i, int there)
+{
+    u32x4 r = {0, 0, 0, 0};
+    if (there >= 4) {
+        if (f32) return __builtin_bit_cast(u32x4, (f32x4)*reinterpret_cast<const x_floats_t *>(static_cast<const float *>(p) + i));
+        const u32x2 h = *reinterpret_cast<const x_halves_t *>(static_cast<const uint16_t *>(p) + i);
+        r[0] = h[0];
+        r[1] = h[1];
+        return r;
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k)
+        if (k < there) {
+            if (f32) r[k] = static_cast<const uint32_t *>(p)[i + k];
+            else r[k >> 1] |= (uint32_t)static_cast<const uint16_t *>(p)[i + k] << ((k & 1) * 16);
+        }
+    return r;
+}
+template <int DT> __device__ __forceinline__ f32x4 x_of_raw4(const u32x4 &r, int f32)
+{
+    constexpr int H = x_half<DT>;
+    if (f32) return __builtin_bit_cast(f32x4, r);
+    return f32x4{zb_half_to_f32<H>(r[0] & 0xffffu), zb_half_to_f32<H>(r[0] >> 16), zb_half_to_f32<H>(r[1] & 0xffffu), zb_half_to_f32<H>(r[1] >> 16)};
+}
+
+/* T times four values behind the activation, which is chosen once for all of them, so that their chains of operations run side by side; z and up have their biases */
+template <int T> __device__ __forceinline__ void x_activate_all(const XgemmParams &p, f32x4 (&z)[T], const f32x4 (&up)[T])
+{
+    auto all = [&](auto f) __attribute__((always_inline)) {
+#pragma unroll
+        for (int t = 0; t < T; ++t)
+#pragma unroll
+            for (int k = 0; k < 4; ++k) z[t][k] = f(z[t][k], up[t][k]);
+    };
+    if (p.n_half) return all([](float v, float u) __attribute__((always_inline)) { return x_silu(v) * u; });
+    switch (p.act) {
+        case ACT_RELU: return all([](float v, float) __attribute__((always_inline)) { return x_activate(ACT_RELU, v); });
+        case ACT_SILU: return all([](float v, float) __attribute__((always_inline)) { return x_activate(ACT_SILU, v); });
+        case ACT_GELU: return all([](float v, float) __attribute__((always_inline)) { return x_activate(ACT_GELU, v); });
+        case ACT_GELU_TANH: return all([](float v, float) __attribute__((always_inline)) { return x_activate(ACT_GELU_TANH, v); });
+        default: return;
+    }
+}
+/* four values of the output, `there` of them */
+template <int DT> __device__ __forceinline__ void x_put(const XgemmParams &p, int64_t row, int j, int there, f32x4 y, const u32x4 &residual)
+{
+    if (p.residual) y += x_of_raw4<DT>(residual, p.out_f32);
+    if (there >= 4) {
+        x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, y);
+    } else {
+#pragma unroll
+        for (int k = 0; k < 3; ++k)
+            if (k < there) x_store<DT>(p.out, p.out_f32, row * p.ldo + j + k, y[k]);
+    }
 }
 __device__ __forceinline__ f32x4 x_value(const f32x4 &v) { return v; }
 __device__ __forceinline__ f32x4 x_value(const i32x4 &v) { return __builtin_bit_cast(f32x4, v); }

@@ -420,12 +420,14 @@ expert_gemm_wide_kernel(XgemmParams p)
         if constexpr (x_is_i8<DT>) {
             const args_t p = fresh_args();
             const int lane = fresh_lane(), first = t.n0 + (p->n_half ? wn * 32 : wn * 64) + (lane >> 4) * 4;
-            x_scale_tile(acc, p->a_scale, p->b_scale, p->b_scale_f32, (int64_t)t.expert * p->N, t.m_end, [&](int mt) { return t.m0 + mt * 32 + wm * 16 + (lane & 15); },
-                         [&](int nt) {
-                             const bool up = p->n_half && nt >= NT / 2;
-                             const int j = first + (up ? nt - NT / 2 : nt) * 16;
-                             return XCols{j + (up ? p->n_half : 0), cols - j};
-                         });
+            XScales<MT, NT> scales;
+            x_load_scales(scales, p->a_scale, p->b_scale, p->b_scale_f32, (int64_t)t.expert * p->N, t.m_end, [&](int mt) { return t.m0 + mt * 32 + wm * 16 + (lane & 15); },
+                          [&](int nt) {
+                              const bool up = p->n_half && nt >= NT / 2;
+                              const int j = first + (up ? nt - NT / 2 : nt) * 16;
+                              return XCols{j + (up ? p->n_half : 0), cols - j};
+                          });
+            x_scale_tile(acc, scales);
         }
         if (REDUCE || !p.through_lds) {
             /* the weights' gradient is not read again soon */
@@ -466,7 +468,18 @@ expert_gemm_wide_kernel(XgemmParams p)
                     const f32x4 z = *reinterpret_cast<const f32x4 *>(sums + r * LD + c);
                     f32x4 up = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (p.n_half) up = *reinterpret_cast<const f32x4 *>(sums + r * LD + TN / 2 + c);
-                    x_finish_some<DT>(p, t.expert, row, j, cols - j, z, up);
+                    if constexpr (x_is_i8<DT>) {
+                        const int there = cols - j;
+                        f32x4 zs[1] = {z}, ups[1] = {up};
+                        if (p.bias) {
+                            zs[0] += x_of_raw4<DT>(x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there), p.bias_f32);
+                            if (p.n_half) ups[0] += x_of_raw4<DT>(x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there), p.bias_f32);
+                        }
+                        x_activate_all<1>(p, zs, ups);
+                        x_put<DT>(p, row, j, there, zs[0], p.residual ? x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + j, there) : u32x4{0, 0, 0, 0});
+                    } else {
+                        x_finish4<DT>(p, t.expert, row, j, z, up);
+                    }
                 }
             }
         }

@@ -425,6 +425,9 @@ template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStr
         if (p.bias_side == 1) zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 1>, grid, block, 0, st, p);
         else if (p.bias_side == 2) zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 2>, grid, block, 0, st, p);
         else zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 0>, grid, block, 0, st, p);
+    } else if constexpr (x_is_i8<DT>) {
+        if (p.through_lds) zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR, 0, true>, grid, block, 0, st, p);
+        else zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR>, grid, block, 0, st, p);
     } else {
         zb_launch(expert_gemm_wide_kernel<DT, REDUCE, B_TR>, grid, block, 0, st, p);
     }

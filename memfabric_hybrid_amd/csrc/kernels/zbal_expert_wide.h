@@ -17,8 +17,11 @@ namespace {
 
 constexpr int XW_CUS = 256;
 
-/* BIAS (REDUCE): the operand whose columns are summed for the bias's gradient besides, 1 = b, 2 = a, 0 = none */
-template <int DT, bool REDUCE, bool B_TR, int BIAS = 0>
+/*
+ * BIAS (REDUCE): the operand whose columns are summed for the bias's gradient besides, 1 = b, 2 = a, 0 = none. FULL (int8): an epilogue of more than a swiglu, with a
+ * workgroup per tile; the registers of the next tile's fragments are then its own (half precision chooses between the two as it runs).
+ */
+template <int DT, bool REDUCE, bool B_TR, int BIAS = 0, bool FULL = false>
 __global__ void __launch_bounds__(512, 2)
 expert_gemm_wide_kernel(XgemmParams p)
 {
@@ -429,7 +432,57 @@ expert_gemm_wide_kernel(XgemmParams p)
                           });
             x_scale_tile(acc, scales);
         }
-        if (REDUCE || !p.through_lds) {
+        if constexpr (FULL) {
+            /* as the smaller tiles have it (zbal_expert_direct.h), four rows at a time: 64 of them in a pass, a lane has four columns of every eighth (without halves) */
+            constexpr int PASS = 2, ROWS = PASS * 32, LD = TN + 4, AT_ONCE = 4;
+            static_assert(x_is_i8<DT> && ROWS * LD * 4 <= 2 * STAGE, "sums fit the stages");
+            float *sums = reinterpret_cast<float *>(smem);
+            const int quads = tile_cols / 4, c = tid % quads * 4, j = t.n0 + c, there = cols - j, r0 = tid / quads, step = WAVES * 64 / quads;
+            u32x4 b = {0, 0, 0, 0}, bu = b;
+            if (p.bias) {
+                b = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there);
+                if (p.n_half) bu = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there);
+            }
+            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+#pragma unroll
+            for (int pass = 0; pass < MT / PASS; ++pass) {
+                __syncthreads();
+#pragma unroll
+                for (int h = 0; h < PASS; ++h)
+#pragma unroll
+                    for (int nt = 0; nt < NT; ++nt)
+                        *reinterpret_cast<f32x4 *>(sums + (h * 32 + wm * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
+                __syncthreads();
+                const int row0 = t.m0 + pass * ROWS;
+#pragma unroll 1
+                for (int r = r0; r < ROWS; r += step * AT_ONCE) {
+                    if (there <= 0) continue;
+                    u32x4 residual[AT_ONCE];
+                    f32x4 z[AT_ONCE], up[AT_ONCE];
+#pragma unroll
+                    for (int h = 0; h < AT_ONCE; ++h) {
+                        const int row = row0 + r + h * step;
+                        residual[h] = u32x4{0, 0, 0, 0};
+                        if (p.residual) residual[h] = x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + j, row < t.m_end ? there : 0);
+                    }
+#pragma unroll
+                    for (int h = 0; h < AT_ONCE; ++h) {
+                        const float *from = sums + (r + h * step) * LD + c;
+                        z[h] = *reinterpret_cast<const f32x4 *>(from) + x_of_raw4<DT>(b, p.bias_f32);
+                        up[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                        if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + x_of_raw4<DT>(bu, p.bias_f32);
+                    }
+                    x_activate_all<AT_ONCE>(p, z, up);
+#pragma unroll
+                    for (int h = 0; h < AT_ONCE; ++h) {
+                        const int row = row0 + r + h * step;
+                        if (row < t.m_end) x_put<DT>(p, row, j, there, z[h], residual[h]);
+                    }
+                }
+            }
+            return;                                             /* nothing was brought behind the last step */
+        }
+        if (REDUCE || x_is_i8<DT> || !p.through_lds) {
             /* the weights' gradient is not read again soon */
             const args_t p = fresh_args();
             const int lane = fresh_lane(), first_col = t.n0 + (p->n_half ? wn * 32 : wn * 64), row0 = t.m0 + wm * 16;
@@ -468,18 +521,7 @@ expert_gemm_wide_kernel(XgemmParams p)
                     const f32x4 z = *reinterpret_cast<const f32x4 *>(sums + r * LD + c);
                     f32x4 up = {0.0f, 0.0f, 0.0f, 0.0f};
                     if (p.n_half) up = *reinterpret_cast<const f32x4 *>(sums + r * LD + TN / 2 + c);
-                    if constexpr (x_is_i8<DT>) {
-                        const int there = cols - j;
-                        f32x4 zs[1] = {z}, ups[1] = {up};
-                        if (p.bias) {
-                            zs[0] += x_of_raw4<DT>(x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there), p.bias_f32);
-                            if (p.n_half) ups[0] += x_of_raw4<DT>(x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there), p.bias_f32);
-                        }
-                        x_activate_all<1>(p, zs, ups);
-                        x_put<DT>(p, row, j, there, zs[0], p.residual ? x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + j, there) : u32x4{0, 0, 0, 0});
-                    } else {
-                        x_finish4<DT>(p, t.expert, row, j, z, up);
-                    }
+                    x_finish4<DT>(p, t.expert, row, j, z, up);
                 }
             }
         }

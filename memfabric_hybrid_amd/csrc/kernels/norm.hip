@@ -10,7 +10,7 @@
 
 namespace {
 
-constexpr int N_LANES = 1024, N_PIECES = 8;          /* of a row, and of a lane: 65536 elements */
+constexpr int N_LANES = 512, N_MOST_LANES = 1024, N_PIECES = 8;      /* lanes of a row, those of one that 512 cannot hold (32768 elements), and pieces of a lane */
 
 /* ---- eight elements ------------------------------------------------------------------------------------------------ */
 
@@ -78,9 +78,17 @@ template <int DT> __device__ __forceinline__ void n_store(void *p, int64_t at, i
         if (i < n) n_store1<DT>(p, at + i, v[i]);
 }
 
+/* four numbers of at most 127 (and a rounding), to the nearest integers: the addition of 1.5 * 2^23 leaves them in the low bits */
+__device__ __forceinline__ uint32_t n_pack4(float a, float b, float c, float d)
+{
+    constexpr float MAGIC = 12582912.0f;
+    const uint32_t ab = __builtin_amdgcn_perm(__float_as_uint(b + MAGIC), __float_as_uint(a + MAGIC), 0x0c0c0400);
+    const uint32_t cd = __builtin_amdgcn_perm(__float_as_uint(d + MAGIC), __float_as_uint(c + MAGIC), 0x04000c0c);
+    return ab | cd;
+}
 __device__ __forceinline__ void n_store_int8(uint8_t *p, int64_t at, int n, const float (&v)[8])
 {
-    const u32x2 q = {zb_pack4_i8(v[0], v[1], v[2], v[3]), zb_pack4_i8(v[4], v[5], v[6], v[7])};
+    const u32x2 q = {n_pack4(v[0], v[1], v[2], v[3]), n_pack4(v[4], v[5], v[6], v[7])};
     if (n >= 8) {
         *reinterpret_cast<n_bytes_t *>(p + at) = q;
         return;
@@ -169,30 +177,29 @@ struct NormParams {
 
 __device__ __forceinline__ float n_rsqrt(float mean_square, float eps) { return 1.0f / __builtin_sqrtf(mean_square + eps); }
 
-/* the weight's eight elements, ones without a weight */
-template <int DT> __device__ __forceinline__ void n_weight(const NormParams &p, int at, int n, float (&w)[8])
+/*
+ * Eight elements of the weight, ones without one: of the rows' type (W is DT) or of 32 bits. A lane has the same columns of every row, so they are loaded once, in front of the
+ * first row, and are there when its sum is.
+ */
+template <int W> __device__ __forceinline__ Piece<W> n_weight(const NormParams &p, int at)
 {
-    if (!p.weight) {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = 1.0f;
-    } else if (DT != ZDT_FP32 && p.weight_f32) {
-        const Piece<ZDT_FP32> v = n_load<ZDT_FP32>(p.weight, at, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = v[i];
-    } else {
-        const Piece<DT> v = n_load<DT>(p.weight, at, n);
-#pragma unroll
-        for (int i = 0; i < 8; ++i) w[i] = v[i];
-    }
+    if (p.weight) return n_load<W>(p.weight, at, p.width - at);
+    Piece<W> ones;
+    constexpr uint32_t one = W == ZDT_FP32 ? 0x3f800000u : (W == ZDT_BF16 ? 0x3f803f80u : 0x3c003c00u);
+    for (auto &v : ones.w) v = u32x4{one, one, one, one};
+    return ones;
 }
 
-template <int DT, int C>
-__global__ void __launch_bounds__(N_LANES)
+template <int DT, int W, int C, int L>
+__global__ void __launch_bounds__(L)
 rms_norm_kernel(NormParams p)
 {
     __shared__ float sums[2][16][1];
     __shared__ uint32_t maxima[2][16];
     const Lanes l;
+    Piece<W> w[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) w[c] = n_weight<W>(p, (l.of_row + c * (int)blockDim.x) * 8);
     int turn = 0;
     for (int64_t base = (int64_t)blockIdx.x * l.rows; base < p.rows; base += (int64_t)gridDim.x * l.rows, turn ^= 1) {
         const int64_t row = base + l.group, at = row * p.width;
@@ -225,12 +232,10 @@ rms_norm_kernel(NormParams p)
         uint32_t most = 0;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            float w[8];
-            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                h[c][i] = h[c][i] * r * w[i];
-                if (i < there[c]) most = n_max(most, n_magnitude(h[c][i]));
+                h[c][i] = h[c][i] * r * w[c][i];              /* zeros where the row has ended, or NaN where it has one */
+                most = n_max(most, n_magnitude(h[c][i]));
             }
             if (p.y) n_store<DT>(p.y, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], h[c]);
         }
@@ -252,56 +257,65 @@ rms_norm_kernel(NormParams p)
  * come from one reduction, of h^2 and of d h. A lane has the same columns of every row that its workgroup takes, so the
  * weight's sums stay in registers until the last of them; a second launch adds up the workgroups', in order.
  */
-template <int DT, int C>
-__global__ void __launch_bounds__(N_LANES)
+template <int DT, int W, int C, int L>
+__global__ void __launch_bounds__(L)
 rms_norm_backward_kernel(NormParams p)
 {
     __shared__ float sums[2][16][2];
     const Lanes l;
+    Piece<W> w[C];
+#pragma unroll
+    for (int c = 0; c < C; ++c) w[c] = n_weight<W>(p, (l.of_row + c * (int)blockDim.x) * 8);
     float dw[C][8];
 #pragma unroll
     for (int c = 0; c < C; ++c)
 #pragma unroll
         for (int i = 0; i < 8; ++i) dw[c][i] = 0.0f;
-    int turn = 0;
-    for (int64_t base = (int64_t)blockIdx.x * l.rows; base < p.rows; base += (int64_t)gridDim.x * l.rows, turn ^= 1) {
-        const int64_t row = base + l.group, at = row * p.width;
-        const bool live = row < p.rows;
-        int there[C];
-        Piece<DT> h[C], g[C], t[C];
+    /* where registers allow, the next row's pieces are on their way while this one's are summed up, and its gradient stored (16384 x 2048 58 -> 53 us, in half the workgroups) */
+    constexpr bool AHEAD = C <= 2;
+    struct Row { Piece<DT> h[C], g[C], t[C]; };
+    auto load = [&](Row &r, int64_t row) __attribute__((always_inline)) {
+        const int64_t at = row * p.width;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            there[c] = live ? p.width - (l.of_row + c * (int)blockDim.x) * 8 : 0;
-            h[c] = n_load<DT>(p.x, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
-            g[c] = n_load<DT>(p.grad, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
-            if (p.grad_total) t[c] = n_load<DT>(p.grad_total, at + (l.of_row + c * (int)blockDim.x) * 8, there[c]);
+            const int col = (l.of_row + c * (int)blockDim.x) * 8, there = row < p.rows ? p.width - col : 0;
+            r.h[c] = n_load<DT>(p.x, at + col, there);
+            r.g[c] = n_load<DT>(p.grad, at + col, there);
+            if (p.grad_total) r.t[c] = n_load<DT>(p.grad_total, at + col, there);
         }
+    };
+    const int64_t first = (int64_t)blockIdx.x * l.rows, step = (int64_t)gridDim.x * l.rows;
+    int turn = 0;
+    Row now, next;
+    if (AHEAD) load(now, first + l.group);
+    for (int64_t base = first; base < p.rows; base += step, turn ^= 1) {
+        const int64_t row = base + l.group, at = row * p.width;
+        if (!AHEAD) load(now, row);
+        else if (base + step < p.rows) load(next, row + step);
         RowSums<2> s = {};
 #pragma unroll
-        for (int c = 0; c < C; ++c) {
-            float w[8];
-            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
+        for (int c = 0; c < C; ++c)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                s.v[0] = __builtin_fmaf(h[c][i], h[c][i], s.v[0]);
-                s.v[1] = __builtin_fmaf(g[c][i] * w[i], h[c][i], s.v[1]);
+                s.v[0] = __builtin_fmaf(now.h[c][i], now.h[c][i], s.v[0]);
+                s.v[1] = __builtin_fmaf(now.g[c][i] * w[c][i], now.h[c][i], s.v[1]);
             }
-        }
         s = row_sum<2>(s, l, sums[turn]);
         const float r = n_rsqrt(s.v[0] * p.per_width, p.eps), mean = s.v[1] * p.per_width * r;
 #pragma unroll
         for (int c = 0; c < C; ++c) {
-            float w[8], d[8];
-            n_weight<DT>(p, (l.of_row + c * (int)blockDim.x) * 8, there[c], w);
+            const int col = (l.of_row + c * (int)blockDim.x) * 8;
+            float d[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float n = h[c][i] * r;
-                d[i] = r * __builtin_fmaf(-n, mean, g[c][i] * w[i]);
-                if (p.grad_total) d[i] += t[c][i];
-                dw[c][i] = __builtin_fmaf(g[c][i], n, dw[c][i]);
+                const float n = now.h[c][i] * r;
+                d[i] = r * __builtin_fmaf(-n, mean, now.g[c][i] * w[c][i]);
+                if (p.grad_total) d[i] += now.t[c][i];
+                dw[c][i] = __builtin_fmaf(now.g[c][i], n, dw[c][i]);
             }
-            n_store<DT>(p.grad_x, at + (l.of_row + c * (int)blockDim.x) * 8, there[c], d);
+            n_store<DT>(p.grad_x, at + col, row < p.rows ? p.width - col : 0, d);
         }
+        if (AHEAD) now = next;
     }
     if (!p.partial) return;
     float *to = p.partial + ((int64_t)blockIdx.x * l.rows + l.group) * p.ldp;
@@ -312,21 +326,32 @@ rms_norm_backward_kernel(NormParams p)
     }
 }
 
-/* sums of `count` rows of ldp floats, sixteen columns of four by sixteen rows to a workgroup; out f32, or of type DT */
+/*
+ * Sums of `count` rows of ldp floats, 32 columns (a line) to a workgroup and every 128th row to a lane, then in two steps through the LDS: few columns are few
+ * workgroups, so that each has to have many rows under way. out f32, or of type DT.
+ */
 template <int DT>
-__global__ void __launch_bounds__(256)
+__global__ void __launch_bounds__(1024)
 rms_norm_join_kernel(const float *__restrict__ partial, int count, int ldp, int width, int out_f32, void *__restrict__ out)
 {
-    __shared__ f32x4 sums[16][16];
-    const int quad = threadIdx.x & 15, first = threadIdx.x >> 4, col = (blockIdx.x * 16 + quad) * 4;
+    __shared__ f32x4 sums[128][8], some[8][8];
+    const int quad = threadIdx.x & 7, first = threadIdx.x >> 3, col = (blockIdx.x * 8 + quad) * 4;
     f32x4 s = {0.0f, 0.0f, 0.0f, 0.0f};
     if (col < ldp)
 #pragma unroll 8
-        for (int i = first; i < count; i += 16) s += *reinterpret_cast<const f32x4 *>(partial + (int64_t)i * ldp + col);
+        for (int i = first; i < count; i += 128) s += *reinterpret_cast<const f32x4 *>(partial + (int64_t)i * ldp + col);
     sums[first][quad] = s;
     __syncthreads();
+    if (first < 8) {
+        s = sums[first][quad];
+#pragma unroll
+        for (int i = 1; i < 16; ++i) s += sums[first + i * 8][quad];
+        some[first][quad] = s;
+    }
+    __syncthreads();
     if (first != 0) return;
-    for (int i = 1; i < 16; ++i) s += sums[i][quad];
+#pragma unroll
+    for (int i = 1; i < 8; ++i) s += some[i][quad];
     for (int i = 0; i < 4 && col + i < width; ++i) {
         if (out_f32) static_cast<float *>(out)[col + i] = s[i];
         else n_store1<DT>(out, col + i, s[i]);
@@ -335,9 +360,15 @@ rms_norm_join_kernel(const float *__restrict__ partial, int count, int ldp, int 
 
 /* ---- activations in int8 ------------------------------------------------------------------------------------------- */
 
+/*
+ * silu in a dozen cycles: an exponential of two and a reciprocal, each a step off (2^-23). The kernel is a stream: with the division of the products' epilogue the vector units
+ * took longer than the memory (32768 x 4096, swiglu: 78 us, now 57).
+ */
+__device__ __forceinline__ float n_silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
+
 /* ACT: ACT_NONE, ACT_SWIGLU, or ACT_SILU for whichever of the others the parameters name */
-template <int DT, int ACT, int C>
-__global__ void __launch_bounds__(N_LANES)
+template <int DT, int ACT, int C, int L>
+__global__ void __launch_bounds__(L)
 quantize_rows_kernel(XgemmParams p, const void *__restrict__ x, uint8_t *__restrict__ q, float *__restrict__ scales)
 {
     __shared__ uint32_t maxima[2][16];
@@ -363,9 +394,9 @@ quantize_rows_kernel(XgemmParams p, const void *__restrict__ x, uint8_t *__restr
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 if constexpr (ACT == ACT_NONE) y[c][i] = z[c][i];
-                else if constexpr (ACT == ACT_SWIGLU) y[c][i] = x_silu(z[c][i]) * up[c][i];
+                else if constexpr (ACT == ACT_SWIGLU) y[c][i] = n_silu(z[c][i]) * up[c][i];
                 else y[c][i] = x_activate(p.act, z[c][i]);
-                if (i < there[c]) most = n_max(most, n_magnitude(y[c][i]));
+                most = n_max(most, n_magnitude(y[c][i]));    /* where the row has ended there are zeros, and all activations of zero are that */
             }
         const RowScale to = row_scale(row_max(most, l, maxima[turn]));
         if (live && l.of_row == 0) scales[row] = to.scale;
@@ -380,7 +411,10 @@ quantize_rows_kernel(XgemmParams p, const void *__restrict__ x, uint8_t *__restr
 
 /* ---- launches ------------------------------------------------------------------------------------------------------ */
 
-/* lanes and pieces of a row of `width` elements: waves of one piece to a lane up to 512 lanes, then more pieces; rows side by side in 256 lanes */
+/*
+ * Lanes and pieces of a row of `width` elements: one piece to a lane up to `most` lanes, then more; rows side by side in 256 lanes. A gradient of more than 16384
+ * elements, and a norm of more than 32768, has more in hand than its registers hold, and is slower for it.
+ */
 struct Shape {
     int pieces, groups;
     unsigned lanes;
@@ -391,24 +425,30 @@ struct Shape {
         return (unsigned)(n < most ? n : most);
     }
 };
-inline Shape shape_of(int64_t width, int most_lanes)
+inline Shape shape_of(int64_t width, int most)
 {
     const int64_t pieces = (width + 7) / 8;
     Shape s = {1, 1, 0};
-    while (s.pieces < N_PIECES && (pieces + s.pieces - 1) / s.pieces > most_lanes) s.pieces *= 2;
+    while (s.pieces < N_PIECES && (pieces + s.pieces - 1) / s.pieces > most) s.pieces *= 2;
     s.lanes = (unsigned)(((pieces + s.pieces - 1) / s.pieces + 63) / 64 * 64);
     s.groups = s.lanes >= 256 ? 1 : 256 / (int)s.lanes;
     return s;
 }
 
-/* f(integral_constant pieces) */
-template <typename F> void with_pieces(int pieces, F f)
+/* few rows have a lane to a piece as far as that goes; many of them more rows side by side on a CU (8192 x 4096, no activation: 512 lanes 19.3 us, 256 16.5) */
+inline Shape forward_shape(int64_t width, int64_t rows) { return shape_of(width, rows > 2048 ? 256 : N_LANES); }
+
+/* f(pieces, most lanes) as integral constants */
+template <typename F> void with_shape(const Shape &s, F f)
 {
-    switch (pieces) {
-        case 1: f(std::integral_constant<int, 1>{}); break;
-        case 2: f(std::integral_constant<int, 2>{}); break;
-        case 4: f(std::integral_constant<int, 4>{}); break;
-        default: f(std::integral_constant<int, 8>{});
+    const std::integral_constant<int, N_LANES> lanes = {};
+    switch (s.pieces) {
+        case 1: f(std::integral_constant<int, 1>{}, lanes); break;
+        case 2: f(std::integral_constant<int, 2>{}, lanes); break;
+        case 4: f(std::integral_constant<int, 4>{}, lanes); break;
+        default:
+            if (s.lanes <= N_LANES) f(std::integral_constant<int, 8>{}, lanes);
+            else f(std::integral_constant<int, 8>{}, std::integral_constant<int, N_MOST_LANES>{});
     }
 }
 template <typename F> void with_type(int dtype, F f)
@@ -444,11 +484,18 @@ NormParams norm_params(const zbalhip_rms_norm_t *d)
     return p;
 }
 
-/* row groups of the gradient's launch, each with sums of its own */
-Shape backward_shape(int64_t width) { return shape_of(width, 512); }
+/*
+ * Workgroups of the gradient's launch, each with sums of its own: 512 lanes a CU (twice that where a row is not asked for ahead of its time), the same number on every CU, are
+ * enough for the memory, and sums of two rows at least cost less than their rows once every CU has one. us at 256 / 512 / 1024 workgroups: 16384 x 2048 67 / 52 / 56;
+ * 4096 x 7168 (of 448 lanes) 48 / 52 / 58, 292 of them 63; 1000 x 1024 8.6 / 11.0 / 11.0.
+ */
+Shape backward_shape(int64_t width) { return shape_of(width, N_LANES); }
 unsigned backward_blocks(const zbalhip_rms_norm_t *d)
 {
-    return backward_shape(d->hidden).blocks(d->tokens, 1024);
+    const Shape s = backward_shape(d->hidden);
+    const int64_t rounds = (d->tokens + s.groups - 1) / s.groups, each = (s.pieces <= 2 ? 512 : 1024) / (int64_t)(s.lanes * s.groups);
+    const int64_t full = each > 1 ? each * 256 : 256, most = full < (rounds + 1) / 2 ? full : (rounds + 1) / 2;
+    return s.blocks(d->tokens, most > 256 ? most : 256);
 }
 
 } // namespace
@@ -463,10 +510,13 @@ extern "C" int32_t zbalhip_rms_norm(const zbalhip_rms_norm_t *d, void *y, void *
     p.total = total;
     p.q = (uint8_t *)q;
     p.scales = scales;
-    const Shape s = shape_of(d->hidden, 512);
+    const Shape s = forward_shape(d->hidden, d->tokens);
     with_type(d->dtype, [&](auto dt) {
-        with_pieces(s.pieces, [&](auto c) {
-            zb_launch(rms_norm_kernel<decltype(dt)::value, decltype(c)::value>, dim3(s.blocks(p.rows, N_MOST_BLOCKS)), s.block(), 0, (hipStream_t)stream, p);
+        with_shape(s, [&](auto c, auto l) {
+            constexpr int DT = decltype(dt)::value, C = decltype(c)::value, L = decltype(l)::value;
+            const dim3 grid(s.blocks(p.rows, N_MOST_BLOCKS));
+            if (p.weight && p.weight_f32) zb_launch(rms_norm_kernel<DT, ZDT_FP32, C, L>, grid, s.block(), 0, (hipStream_t)stream, p);
+            else zb_launch(rms_norm_kernel<DT, DT, C, L>, grid, s.block(), 0, (hipStream_t)stream, p);
         });
     });
     return zbalhip_check_launch();
@@ -495,13 +545,15 @@ extern "C" int32_t zbalhip_rms_norm_backward(const zbalhip_rms_norm_t *d, const 
     hipStream_t st = (hipStream_t)stream;
     if (d->tokens > 0)
         with_type(d->dtype, [&](auto dt) {
-            with_pieces(s.pieces, [&](auto c) {
-                zb_launch(rms_norm_backward_kernel<decltype(dt)::value, decltype(c)::value>, dim3(blocks), s.block(), 0, st, p);
+            with_shape(s, [&](auto c, auto l) {
+                constexpr int DT = decltype(dt)::value, C = decltype(c)::value, L = decltype(l)::value;
+                if (p.weight && p.weight_f32) zb_launch(rms_norm_backward_kernel<DT, ZDT_FP32, C, L>, dim3(blocks), s.block(), 0, st, p);
+                else zb_launch(rms_norm_backward_kernel<DT, DT, C, L>, dim3(blocks), s.block(), 0, st, p);
             });
         });
     if (grad_weight)
         with_type(d->dtype, [&](auto dt) {
-            zb_launch(rms_norm_join_kernel<decltype(dt)::value>, dim3((unsigned)(p.ldp + 63) / 64), dim3(256), 0, st, p.partial, (int)(blocks * s.groups), p.ldp,
+            zb_launch(rms_norm_join_kernel<decltype(dt)::value>, dim3((unsigned)(p.ldp + 31) / 32), dim3(1024), 0, st, p.partial, (int)(blocks * s.groups), p.ldp,
                       p.width, weight_grad_is_f32, grad_weight);
         });
     return zbalhip_check_launch();
@@ -523,14 +575,14 @@ extern "C" int32_t zbalhip_quantize_rows(const zbalhip_quantize_rows_t *d, const
     p.N = (int)d->width;
     p.act = d->activation;
     p.n_half = d->activation == ACT_SWIGLU ? p.N / 2 : 0;
-    const Shape s = shape_of(p.n_half ? p.n_half : p.N, 512);
+    const Shape s = forward_shape(p.n_half ? p.n_half : p.N, d->rows);
     const dim3 grid(s.blocks(d->rows, N_MOST_BLOCKS));
     with_type(d->dtype, [&](auto dt) {
-        with_pieces(s.pieces, [&](auto c) {
-            constexpr int DT = decltype(dt)::value, C = decltype(c)::value;
-            if (p.act == ACT_NONE) zb_launch(quantize_rows_kernel<DT, ACT_NONE, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
-            else if (p.act == ACT_SWIGLU) zb_launch(quantize_rows_kernel<DT, ACT_SWIGLU, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
-            else zb_launch(quantize_rows_kernel<DT, ACT_SILU, C>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+        with_shape(s, [&](auto c, auto l) {
+            constexpr int DT = decltype(dt)::value, C = decltype(c)::value, L = decltype(l)::value;
+            if (p.act == ACT_NONE) zb_launch(quantize_rows_kernel<DT, ACT_NONE, C, L>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+            else if (p.act == ACT_SWIGLU) zb_launch(quantize_rows_kernel<DT, ACT_SWIGLU, C, L>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
+            else zb_launch(quantize_rows_kernel<DT, ACT_SILU, C, L>, grid, s.block(), 0, (hipStream_t)stream, p, x, (uint8_t *)q, scales);
         });
     });
     return zbalhip_check_launch();

@@ -246,7 +246,7 @@ expert_gemm_kernel(XgemmParams p)
     constexpr int PASS = MT % 2 == 0 && WM * 32 * (TN + 4) * 4 <= STAGES * STAGE ? 2 : 1, ROWS = WM * PASS * 16, LD = TN + 4, QUADS = TN / 4;
     /*
      * What int8's epilogue reads, asked for in front of the first transfers: behind the last products it would be waited for, twice (1021 x 1001 x 1531 with gelu, bias and
-     * residual FIXME).
+     * residual, its copies included, 24.6 us, now 17.6).
      */
     constexpr int TURNS = ROWS * QUADS / (WAVES * 64), ROW_STEP = WAVES * 64 / QUADS;
     static_assert(!x_is_i8<DT> || (TURNS % 2 == 0 && TURNS * WAVES * 64 == ROWS * QUADS && ROW_STEP * QUADS == WAVES * 64), "a lane has the same columns in every turn");

@@ -406,6 +406,18 @@ template <int DT> void launch_rows(const XgemmParams &p, hipStream_t st)
 {
     /* eight waves where four have more than one batch of loads */
     const dim3 grid(tiles_of_cols<16>(p, 16)), four(256), eight(512);
+    if constexpr (x_is_i8<DT>) {
+        /* a load or two of a lane at a time, and so many waves that the others' are under way: one row of 2048 x 7168 4.6 us (eight loads at a time 7.4), of 7168 x 7168 10.7 (14.3);
+           four waves where eight would have a load each or none: 16 rows over 32 experts of 2048 x 7168 35 us, 44 with eight */
+        if (p.n_half) {
+            if (p.K > 1024) zb_launch(expert_gemm_rows_kernel<DT, 2, 8, 1>, grid, eight, 0, st, p);
+            else zb_launch(expert_gemm_rows_kernel<DT, 2, 4, 1>, grid, four, 0, st, p);
+        } else {
+            if (p.K > 1024) zb_launch(expert_gemm_rows_kernel<DT, 1, 8, 1>, grid, eight, 0, st, p);
+            else zb_launch(expert_gemm_rows_kernel<DT, 1, 4, 1>, grid, four, 0, st, p);
+        }
+        return;
+    }
     if (p.n_half) {
         if (p.K > 1024) zb_launch(expert_gemm_rows_kernel<DT, 2, 8>, grid, eight, 0, st, p);
         else zb_launch(expert_gemm_rows_kernel<DT, 2, 4>, grid, four, 0, st, p);
@@ -635,16 +647,16 @@ void in_pairs(XgemmParams *p, int k)
 /*
  * The cut of an int8 product that takes least time, by a model of a kind's launch: rounds of workgroups, each of a fixed time and one for every step of 128 k (with
  * few workgroups on the card, and with as many as run side by side), joined with the time that reading the weights takes as the root of the sum of their squares.
- * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 72 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
- * unaligned rows: the kind that it picks takes 1.02 times the best one's on average, 1.28 at most (2868 rows over 32 experts of 384 x 5056: 64 x 128 43 us, wide 34).
- * Half precision's rule, for the same tiles, has 1.11 and 3.65 here: 512 x 512 x 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of
+ * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 98 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
+ * unaligned rows: the kind that it picks takes 1.02 times the best one's on average, 1.32 at most (2868 rows over 32 experts of 384 x 5056: 64 x 128 44 us, wide 33).
+ * Half precision's rule, for the same tiles, had 1.11 and 3.65 here: 512 x 512 x 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of
  * 2048 x 1024 128 x 128 71, wide 56.
  */
 struct Int8Cut { Cut cut; int tm, tn, at_once; double fixed, alone, full, stream; };
-const Int8Cut int8_cuts[] = {{CUT_WIDE, 256, 256, 1, 4.85, 0.9, 1.45, 7.0e6}, {CUT_128, 128, 128, 1, 2.56, 0.37, 0.66, 7.0e6}, {CUT_64_128, 64, 128, 2, 2.46, 0.44, 0.74, 6.4e6},
-                             {CUT_64, 64, 64, 2, 2.11, 0.25, 0.48, 7.0e6}, {CUT_32, 32, 128, 2, 2.2, 0.22, 0.48, 5.7e6}, {CUT_16, 16, 64, 2, 2.45, 0.14, 0.21, 5.25e6},
-                             {CUT_ROWS, 16, 16, 4, 4.22, 0.02, 0.52, 7.0e6}};
-const Int8Cut int8_any_cuts[] = {{CUT_ANY, 128, 128, 2, 6.55, 1.25, 1.9, 7.0e6}, {CUT_ANY_64, 64, 64, 4, 3.95, 0.48, 1.64, 3.6e6}, {CUT_ANY_16, 16, 128, 4, 2.59, 0.51, 1.68, 4.1e6}};
+const Int8Cut int8_cuts[] = {{CUT_WIDE, 256, 256, 1, 4.2, 0.92, 1.42, 7.0e6}, {CUT_128, 128, 128, 1, 2.49, 0.38, 0.66, 7.0e6}, {CUT_64_128, 64, 128, 2, 2.38, 0.4, 0.72, 6.16e6},
+                             {CUT_64, 64, 64, 2, 2.09, 0.25, 0.47, 7.0e6}, {CUT_32, 32, 128, 2, 2.15, 0.24, 0.49, 5.6e6}, {CUT_16, 16, 64, 2, 2.49, 0.15, 0.23, 5.5e6},
+                             {CUT_ROWS, 16, 16, 4, 0.71, 0.05, 0.42, 6.0e6}};
+const Int8Cut int8_any_cuts[] = {{CUT_ANY, 128, 128, 2, 7.5, 1.25, 2.4, 7.0e6}, {CUT_ANY_64, 64, 64, 4, 4.8, 0.55, 1.8, 6.4e6}, {CUT_ANY_16, 16, 128, 4, 2.7, 0.52, 1.75, 6.2e6}};
 
 /* p with k in bytes */
 Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
@@ -687,7 +699,7 @@ Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
 
 /*
  * Rows that are not aligned: multiplied as they lie, or copied to the workspace first, whichever the model expects to be done sooner. A copy is a launch, and writes
- * both operands at 2.4 TB/s: 4093 x 4099 x 4093 194 us as it lies, 83 copied; 16 rows over 32 experts of 4001 x 1531 32 and 115.
+ * both operands at 2.4 TB/s: 4093 x 4099 x 4093 194 us as it lies, 83 copied; 16 rows over 32 experts of 4001 x 1531 32 and 114.
  */
 struct Int8Plan {
     XgemmParams p;
@@ -695,7 +707,7 @@ struct Int8Plan {
     bool copies;
     int64_t x_bytes, w_bytes, bytes;
 };
-constexpr int64_t X_MOST_COPIED = (int64_t)1 << 31;
+constexpr int64_t X_MOST_COPIED = (int64_t)1 << 29;
 Int8Plan plan_int8(const zbalhip_expert_linear_int8_t *d, bool may_copy = true)
 {
     Int8Plan plan = {};
@@ -712,7 +724,7 @@ Int8Plan plan_int8(const zbalhip_expert_linear_int8_t *d, bool may_copy = true)
     XgemmParams to = plan.p;
     to.K = (int)k;
     const Plan copied = plan_int8_cut(to, true, &copied_us);
-    if (copied_us + 2.5 + (double)(x_bytes + w_bytes) / 2.4e6 >= us) return plan;
+    if (copied_us + 3.7 + (double)(x_bytes + w_bytes) / 2.4e6 >= us) return plan;
     in_pairs(&to, (int)k);
     return {to, copied, true, x_bytes, w_bytes, x_bytes + w_bytes + copied.bytes};
 }

@@ -15,12 +15,12 @@
 
 namespace {
 
-/* NT sub-tiles of sixteen columns: one, or the gate's and the up columns */
-template <int DT, int NT, int WAVES>
+/* NT sub-tiles of sixteen columns: one, or the gate's and the up columns; BATCH: k in steps of 64 that a wave asks for at a time */
+template <int DT, int NT, int WAVES, int BATCH = 8 / NT>
 __global__ void __launch_bounds__(WAVES * 64)
 expert_gemm_rows_kernel(XgemmParams p)
 {
-    constexpr int BATCH = 8 / NT, LD = NT * 16 + 1;
+    constexpr int LD = NT * 16 + 1;
     __shared__ x_sum_t<DT> sums[WAVES][16][LD];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6), quad = lane >> 4;
     const int cols = p.n_half ? p.n_half : p.N, n_tiles = (cols + 15) / 16;

@@ -130,6 +130,23 @@ def test_every_cut(buf, rows, E, K, N):
         case(buf, rows, E, K, N, torch.float16, "swiglu", bias=torch.float32, residual=True, seed=3)
 
 
+# what the rule gives each kind of tiles, whole and in parts, aligned rows and rows that are copied, or multiplied as they lie; columns that end anywhere
+@pytest.mark.parametrize("rows,E,K,N,act", [
+    (1915, 1, 144, 2157, "none"), (1130, 20, 176, 3078, "swiglu"), (2130, 1, 175, 1880, "swiglu"), (2100, 1, 296, 1815, "none"),                      # 128 x 128
+    (15, 20, 736, 1983, "none"), (3505, 1, 1616, 114, "swiglu"), (327, 1, 1890, 1280, "swiglu"),                                                     # 16 x 64
+    (27, 20, 16, 2865, "none"), (4597, 1, 5168, 80, "none"), (564, 1, 4416, 248, "none"), (1066, 1, 7744, 226, "swiglu"), (337, 1, 6032, 350, "none"),     # 32 x 128
+    (10, 20, 224, 2071, "none"), (1429, 1, 6096, 280, "swiglu"), (711, 1, 6100, 271, "none"), (434, 1, 8196, 568, "swiglu"), (2722, 1, 6416, 35, "none"),   # 64 x 64
+    (639, 20, 16, 2198, "none"), (4564, 20, 16, 394, "swiglu"), (921, 20, 52, 3888, "none"),                                                         # 64 x 128
+    (2222, 8, 16, 1697, "none"), (1917, 20, 16, 1836, "swiglu"), (7187, 1, 20, 772, "swiglu"), (3816, 1, 17, 1485, "none"),                          # 256 x 256
+    (1835, 3, 17, 2147, "none"), (5613, 1, 18, 778, "swiglu"), (68, 1, 1727, 2674, "none"), (1, 1, 3644, 2302, "none"), (1, 1, 3537, 2120, "swiglu"),  # as they lie
+    (1, 1, 4115, 1105, "none"), (2511, 8, 17, 787, "none"), (8692, 1, 1775, 12, "none"), (5719, 1, 3268, 10, "swiglu"), (1336, 1, 8604, 9, "none"),
+    (7, 3, 1040, 77, "none"), (9, 2, 2064, 90, "swiglu"), (5, 4, 528, 131, "none"), (30, 3, 3104, 46, "swiglu")])                                      # 16 columns
+def test_every_kind_of_the_rule(buf, rows, E, K, N, act):
+    case(buf, rows, E, K, N, torch.float32, act)
+    case(buf, rows, E, K, N, torch.float16, "silu" if act == "none" else act, bias=torch.float16, residual=True, seed=1)
+    case(buf, rows, E, K, N, torch.bfloat16, act, bias=torch.float32, scale_type=torch.bfloat16, seed=2)
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 0, 0], [0, 0, 0, 50], [50, 0, 0, 0], [10, 10, 10, 10], [-5, 20, -(1 << 31), 10], [30, 1 << 30, 7, (1 << 31) - 1],
                                     [1, 47, 1, 1], [20, 20, 20, 20]])
 @pytest.mark.parametrize("K,N", [(128, 128), (130, 131)])
@@ -229,11 +246,11 @@ def test_the_same_every_time_and_captured(buf, rows, E, K, N):
         assert all(torch.equal(p, q) for p, q in zip(got, want)) and all(torch.equal(p, q) for p, q in zip(got2, want))
 
 
-def test_parts_give_the_same_bits(buf):
-    """without a workspace a product is not split along k; its integers add up to the same"""
+def test_parts_and_copies_give_the_same_bits(buf):
+    """without a workspace a product is not split along k, and its rows are not copied; its integers add up to the same"""
     import ctypes
     lib, split = capi.load(), 0
-    for rows, K, N, act in ((500, 8192, 128, 0), (70, 4240, 520, 5), (130, 8208, 264, 2), (100, 8193, 250, 3)):
+    for rows, K, N, act in ((564, 4416, 248, 0), (1066, 7744, 226, 5), (337, 6032, 350, 2), (711, 6100, 271, 3), (434, 8196, 568, 5), (2000, 4099, 1003, 2), (1, 3644, 2302, 0)):
         g, x, xs, w, ws, _ = make(rows, 1, K, N, 3)
         cols = N // 2 if act == 5 else N
         d = capi.ExpertLinearInt8(w.data_ptr(), ws.data_ptr(), 1, 0, None, act, capi.DT_FP32, rows, K, N, 1)
@@ -247,7 +264,7 @@ def test_parts_give_the_same_bits(buf):
                                                   torch.cuda.current_stream().cuda_stream) == 0
             ys.append(y)
         assert torch.equal(*ys)
-    assert split > 0
+    assert split == 7
 
 
 def test_residual_in_place(buf):

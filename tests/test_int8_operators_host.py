@@ -113,6 +113,10 @@ def test_linear_workspace_sizes(lib):
         assert 0 <= b < 1 << 32
         assert b == 0 or e == 1
     assert lib.zbal_moe_expert_linear_int8_workspace_size(16, 64, 63, 1, 5) == -1
+    # unaligned rows are copied where that is sooner, never past 512 MiB
+    assert lib.zbal_moe_expert_linear_int8_workspace_size(4093, 4099, 4093, 1, 0) == 2 * 4093 * 4112
+    assert lib.zbal_moe_expert_linear_int8_workspace_size(16, 4001, 1531, 32, 0) == 0
+    assert lib.zbal_moe_expert_linear_int8_workspace_size(1 << 20, 4099, 4093, 1, 0) == 0
 
 
 def test_outer_calls_check_their_arguments_first(lib):

@@ -170,6 +170,8 @@ struct NormParams {
     const void *grad, *grad_total;    /* the gradient's */
     void *grad_x;
     float *partial;                   /* [row groups of the launch][ldp]: the sums of their rows for the weight's gradient */
+    void *grad_weight;                /* of a workgroup alone */
+    int weight_grad_f32;
     int64_t rows;
     int width, ldp, weight_f32;
     float eps, per_width;             /* 1 / width */
@@ -255,12 +257,15 @@ rms_norm_kernel(NormParams p)
 /*
  * With n = h r and d = g w: dh = r (d - n mean(d n)) + the sum's own gradient, and the weight's gradient is the sum over rows of g n. Both means of a row
  * come from one reduction, of h^2 and of d h. A lane has the same columns of every row that its workgroup takes, so the
- * weight's sums stay in registers until the last of them; a second launch adds up the workgroups', in order.
+ * weight's sums stay in registers until the last of them; a second launch adds up the workgroups', in order. ALONE: one workgroup has all rows, side by side
+ * in its lanes, and adds up their sums itself.
  */
-template <int DT, int W, int C, int L>
+template <int DT, int W, int C, int L, bool ALONE>
 __global__ void __launch_bounds__(L)
 rms_norm_backward_kernel(NormParams p)
 {
+    static_assert(!ALONE || C == 1, "a row is a piece to a lane");
+    __shared__ float columns[ALONE ? L * 8 : 1];
     __shared__ float sums[2][16][2];
     const Lanes l;
     Piece<W> w[C];
@@ -316,6 +321,19 @@ rms_norm_backward_kernel(NormParams p)
             n_store<DT>(p.grad_x, at + col, row < p.rows ? p.width - col : 0, d);
         }
         if (AHEAD) now = next;
+    }
+    if constexpr (ALONE) {
+        const int per_row = blockDim.x * 8;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) columns[l.group * per_row + l.of_row * 8 + i] = dw[0][i];
+        __syncthreads();
+        for (int col = l.group * (int)blockDim.x + l.of_row; p.grad_weight && col < p.width; col += blockDim.x * blockDim.y) {
+            float sum = 0.0f;
+            for (int g = 0; g < l.rows; ++g) sum += columns[g * per_row + col];
+            if (p.weight_grad_f32) static_cast<float *>(p.grad_weight)[col] = sum;
+            else n_store1<DT>(p.grad_weight, col, sum);
+        }
+        return;
     }
     if (!p.partial) return;
     float *to = p.partial + ((int64_t)blockIdx.x * l.rows + l.group) * p.ldp;
@@ -489,13 +507,23 @@ NormParams norm_params(const zbalhip_rms_norm_t *d)
  * enough for the memory, and sums of two rows at least cost less than their rows once every CU has one. us at 256 / 512 / 1024 workgroups: 16384 x 2048 67 / 52 / 56;
  * 4096 x 7168 (of 448 lanes) 48 / 52 / 58, 292 of them 63; 1000 x 1024 8.6 / 11.0 / 11.0.
  */
-Shape backward_shape(int64_t width) { return shape_of(width, N_LANES); }
+Shape backward_shape(const zbalhip_rms_norm_t *d)
+{
+    return shape_of(d->hidden, N_LANES);
+}
 unsigned backward_blocks(const zbalhip_rms_norm_t *d)
 {
-    const Shape s = backward_shape(d->hidden);
+    const Shape s = backward_shape(d);
     const int64_t rounds = (d->tokens + s.groups - 1) / s.groups, each = (s.pieces <= 2 ? 512 : 1024) / (int64_t)(s.lanes * s.groups);
     const int64_t full = each > 1 ? each * 256 : 256, most = full < (rounds + 1) / 2 ? full : (rounds + 1) / 2;
     return s.blocks(d->tokens, most > 256 ? most : 256);
+}
+/* rows that one workgroup is through with before a second launch would have begun: a round takes 0.6 to 2 us, a launch 2.3 (32 x 512 6.2 -> 4.5 us) */
+int backward_alone(const zbalhip_rms_norm_t *d)
+{
+    const Shape s = backward_shape(d);
+    const int groups = N_MOST_LANES / (int)s.lanes;
+    return s.pieces == 1 && d->tokens > 0 && d->tokens <= (int64_t)groups * 2 ? groups : 0;
 }
 
 } // namespace
@@ -525,7 +553,7 @@ extern "C" int32_t zbalhip_rms_norm(const zbalhip_rms_norm_t *d, void *y, void *
 extern "C" int64_t zbalhip_rms_norm_backward_workspace(const zbalhip_rms_norm_t *d)
 {
     if (!norm_ok(d)) return -1;
-    return (int64_t)backward_blocks(d) * backward_shape(d->hidden).groups * ((d->hidden + 3) / 4 * 4) * 4;
+    return backward_alone(d) ? 0 : (int64_t)backward_blocks(d) * backward_shape(d).groups * ((d->hidden + 3) / 4 * 4) * 4;
 }
 
 extern "C" int32_t zbalhip_rms_norm_backward(const zbalhip_rms_norm_t *d, const void *grad, const void *grad_total, void *grad_x, void *grad_weight,
@@ -534,21 +562,34 @@ extern "C" int32_t zbalhip_rms_norm_backward(const zbalhip_rms_norm_t *d, const 
     if (!norm_ok(d)) return ZBALHIP_INVALID;
     if (d->tokens > 0 && (!d->x || !grad || !grad_x)) return ZBALHIP_INVALID;
     if (d->tokens == 0 && !grad_weight) return ZBALHIP_OK;
-    if (grad_weight && d->tokens > 0 && (!workspace || workspace_bytes < zbalhip_rms_norm_backward_workspace(d))) return ZBALHIP_INVALID;
+    const int64_t need = grad_weight && d->tokens > 0 ? zbalhip_rms_norm_backward_workspace(d) : 0;
+    if (need > 0 && (!workspace || workspace_bytes < need)) return ZBALHIP_INVALID;
     NormParams p = norm_params(d);
     p.grad = grad;
     p.grad_total = grad_total;
     p.grad_x = grad_x;
     p.partial = grad_weight ? (float *)workspace : nullptr;
-    const Shape s = backward_shape(d->hidden);
-    const unsigned blocks = backward_blocks(d);
     hipStream_t st = (hipStream_t)stream;
+    const int groups = grad_weight ? backward_alone(d) : 0;
+    if (groups) {
+        p.grad_weight = grad_weight;
+        p.weight_grad_f32 = weight_grad_is_f32;
+        const dim3 block(backward_shape(d).lanes, groups);
+        with_type(d->dtype, [&](auto dt) {
+            constexpr int DT = decltype(dt)::value;
+            if (p.weight && p.weight_f32) zb_launch(rms_norm_backward_kernel<DT, ZDT_FP32, 1, N_MOST_LANES, true>, dim3(1), block, 0, st, p);
+            else zb_launch(rms_norm_backward_kernel<DT, DT, 1, N_MOST_LANES, true>, dim3(1), block, 0, st, p);
+        });
+        return zbalhip_check_launch();
+    }
+    const Shape s = backward_shape(d);
+    const unsigned blocks = backward_blocks(d);
     if (d->tokens > 0)
         with_type(d->dtype, [&](auto dt) {
             with_shape(s, [&](auto c, auto l) {
                 constexpr int DT = decltype(dt)::value, C = decltype(c)::value, L = decltype(l)::value;
-                if (p.weight && p.weight_f32) zb_launch(rms_norm_backward_kernel<DT, ZDT_FP32, C, L>, dim3(blocks), s.block(), 0, st, p);
-                else zb_launch(rms_norm_backward_kernel<DT, DT, C, L>, dim3(blocks), s.block(), 0, st, p);
+                if (p.weight && p.weight_f32) zb_launch(rms_norm_backward_kernel<DT, ZDT_FP32, C, L, false>, dim3(blocks), s.block(), 0, st, p);
+                else zb_launch(rms_norm_backward_kernel<DT, DT, C, L, false>, dim3(blocks), s.block(), 0, st, p);
             });
         });
     if (grad_weight)

@@ -162,7 +162,7 @@ def backward_case(buf, tokens, hidden, dtype, weight, total, wgrad, seed=0):
 
 
 @pytest.mark.parametrize("dtype", TYPES)
-@pytest.mark.parametrize("tokens,hidden", SIZES + [(5000, 64), (2100, 1030), (1100, 2048), (0, 72)])
+@pytest.mark.parametrize("tokens,hidden", SIZES + [(5000, 64), (2100, 1030), (1100, 2048), (0, 72), (96, 512), (97, 512), (77, 64), (41, 1025), (12, 4090), (13, 4090), (18, 2000)])
 def test_gradients(buf, tokens, hidden, dtype):
     backward_case(buf, tokens, hidden, dtype, "same", True, None)
     backward_case(buf, tokens, hidden, dtype, "fp32", False, torch.float32)

@@ -53,10 +53,12 @@ def test_norm_null_pointers(lib):
     assert lib.zbalhip_rms_norm(None, 4096, None, None, None, None) == INVALID
     assert lib.zbalhip_rms_norm(d, None, None, None, 4096, None) == INVALID                    # no output
     assert lib.zbalhip_rms_norm(d, None, None, 4096, None, None) == INVALID                    # int8 without scales
-    need = lib.zbalhip_rms_norm_backward_workspace(d)
+    assert lib.zbalhip_rms_norm_backward_workspace(d) == 0                                     # so few rows that one workgroup has them all
+    many = ctypes.byref(norm(tokens=4096))
+    need = lib.zbalhip_rms_norm_backward_workspace(many)
     assert need > 0
-    for grad, gx, gw, ws, size in ((None, 4096, None, None, 0), (4096, None, None, None, 0), (4096, 4096, 4096, None, need), (4096, 4096, 4096, 4096, need - 1)):
-        assert lib.zbalhip_rms_norm_backward(d, grad, None, gx, gw, 0, ws, size, None) == INVALID
+    for of, grad, gx, gw, ws, size in ((d, None, 4096, None, None, 0), (d, 4096, None, None, None, 0), (many, 4096, 4096, 4096, None, need), (many, 4096, 4096, 4096, 4096, need - 1)):
+        assert lib.zbalhip_rms_norm_backward(of, grad, None, gx, gw, 0, ws, size, None) == INVALID
     none = ctypes.byref(norm(tokens=0, x=None))
     assert lib.zbalhip_rms_norm(none, None, None, None, None, None) == 0
     assert lib.zbalhip_rms_norm_backward(none, None, None, None, None, 0, None, 0, None) == 0
@@ -66,7 +68,7 @@ def test_norm_workspace_is_bounded(lib):
     for tokens in (0, 1, 61, 16384, 1 << 24):
         for hidden in (1, 64, 2048, 7168, 65536):
             b = lib.zbal_moe_rms_norm_workspace_size(tokens, hidden)
-            assert (b > 0) == (tokens > 0) and b <= 1 << 30
+            assert 0 <= b <= 1 << 30 and (tokens > 0 or b == 0)
     assert lib.zbal_moe_rms_norm_workspace_size(4, 65537) == lib.zbal_moe_rms_norm_workspace_size(-1, 64) == -1
 
 

@@ -449,7 +449,7 @@ template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStr
 inline bool rows_are_aligned(const XgemmParams &p) { return p.lda % 8 == 0 && p.ldb % 8 == 0 && p.ldo % 8 == 0 && p.N % 8 == 0 && p.n_half % 8 == 0; }
 
 /* how a product is cut: the tiles, and the parts along k whose sums a second launch adds up */
-enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT, CUT_ROWS };
+enum Cut { CUT_WIDE, CUT_128, CUT_64_128, CUT_64, CUT_32, CUT_16, CUT_ANY, CUT_ANY_64, CUT_ANY_16, CUT_SHORT, CUT_ROWS, CUT_64_FLAT, CUT_32_FLAT, CUT_16_FLAT };
 /* columns of the parts' sums: either half of a swiglu's starts at a multiple of four */
 inline int64_t parts_width(const XgemmParams &p) { return p.n_half ? (p.n_half + 3) / 4 * 8 : (p.N + 3) / 4 * 4; }
 struct Plan {
@@ -531,7 +531,18 @@ template <int DT, bool REDUCE, bool B_TR> void launch_product(XgemmParams p, Pla
         p.bias_partial = p.partial + (int64_t)p.splits * (REDUCE ? p.M : p.rows) * p.ldp;
         p.bias_ldp = ((p.M > p.N ? p.M : p.N) + 3) / 4 * 4;
     }
+    constexpr bool I8 = x_is_i8<DT>;
     switch (plan.cut) {
+        /* two stages: what a ring has in one workgroup, more of them have side by side */
+        case CUT_64_FLAT:
+            if constexpr (I8) launch_direct<DT, REDUCE, B_TR, 64, 64, 2, 2, 2>(p, st);
+            break;
+        case CUT_32_FLAT:
+            if constexpr (I8) launch_direct<DT, REDUCE, B_TR, 32, 128, 2, 2, 2>(p, st);
+            break;
+        case CUT_16_FLAT:
+            if constexpr (I8) launch_direct<DT, REDUCE, B_TR, 16, 64, 1, 2, 2>(p, st);
+            break;
         case CUT_WIDE: launch_wide<DT, REDUCE, B_TR>(p, st); break;
         case CUT_128: launch_direct<DT, REDUCE, B_TR, 128, 128, 2, 4, 4>(p, st); break;
         case CUT_64_128: launch_direct<DT, REDUCE, B_TR, 64, 128, 2, 2, 3>(p, st); break;
@@ -647,16 +658,20 @@ void in_pairs(XgemmParams *p, int k)
 /*
  * The cut of an int8 product that takes least time, by a model of a kind's launch: rounds of workgroups, each of a fixed time and one for every step of 128 k (with
  * few workgroups on the card, and with as many as run side by side), joined with the time that reading the weights takes as the root of the sum of their squares.
- * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 98 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
- * unaligned rows: the kind that it picks takes 1.02 times the best one's on average, 1.32 at most (2868 rows over 32 experts of 384 x 5056: 64 x 128 44 us, wide 33).
- * Half precision's rule, for the same tiles, had 1.11 and 3.65 here: 512 x 512 x 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of
- * 2048 x 1024 128 x 128 71, wide 56.
+ * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 136 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
+ * unaligned rows: the kind that it picks takes 1.03 times the best one's on average, 1.31 at most (one row of 1001 x 4001: copied 10.1 us, as it lies 7.7). For 27 more, of 1
+ * to 1021 rows over 8 to 128 experts, that no figure was fitted to, 1.02 and 1.17. Half precision's rule, for the tiles that both have, had 1.11 and 3.65 here: 512 x 512 x
+ * 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of 2048 x 1024 128 x 128 71, wide 56. FLAT: rings of two stages and three to eight
+ * workgroups to a CU instead of two, which gain where tiles are many and short: 423 rows over 64 experts, k 128 and n 4480, 25 -> 15 us, 425 over 64, k 384 and n 6912, silu
+ * 63 -> 43; and lose where they are few and long: 4 rows over 8, k 7168 and n 2048, 16 -> 42.
  */
 struct Int8Cut { Cut cut; int tm, tn, at_once; double fixed, alone, full, stream; };
-const Int8Cut int8_cuts[] = {{CUT_WIDE, 256, 256, 1, 4.2, 0.92, 1.42, 7.0e6}, {CUT_128, 128, 128, 1, 2.49, 0.38, 0.66, 7.0e6}, {CUT_64_128, 64, 128, 2, 2.38, 0.4, 0.72, 6.16e6},
-                             {CUT_64, 64, 64, 2, 2.09, 0.25, 0.47, 7.0e6}, {CUT_32, 32, 128, 2, 2.15, 0.24, 0.49, 5.6e6}, {CUT_16, 16, 64, 2, 2.49, 0.15, 0.23, 5.5e6},
-                             {CUT_ROWS, 16, 16, 4, 0.71, 0.05, 0.42, 6.0e6}};
+const Int8Cut int8_cuts[] = {{CUT_WIDE, 256, 256, 1, 4.33, 0.93, 1.39, 7.0e6}, {CUT_128, 128, 128, 1, 2.66, 0.36, 0.66, 7.0e6}, {CUT_64_128, 64, 128, 2, 2.55, 0.39, 0.79, 5.8e6},
+                             {CUT_64, 64, 64, 2, 2.29, 0.24, 0.5, 6.7e6}, {CUT_32, 32, 128, 2, 2.4, 0.22, 0.52, 5.25e6}, {CUT_16, 16, 64, 2, 2.72, 0.13, 0.24, 5.2e6},
+                             {CUT_ROWS, 16, 16, 4, 0.84, 0.05, 0.42, 6.0e6}, {CUT_64_FLAT, 64, 64, 4, 1.57, 0.44, 1.11, 6.25e6}, {CUT_32_FLAT, 32, 128, 4, 1.63, 0.49, 1.18, 5.0e6},
+                             {CUT_16_FLAT, 16, 64, 8, 1.38, 0.33, 0.95, 5.2e6}};
 const Int8Cut int8_any_cuts[] = {{CUT_ANY, 128, 128, 2, 7.5, 1.25, 2.4, 7.0e6}, {CUT_ANY_64, 64, 64, 4, 4.8, 0.55, 1.8, 6.4e6}, {CUT_ANY_16, 16, 128, 4, 2.7, 0.52, 1.75, 6.2e6}};
+static_assert(sizeof(int8_cuts) / sizeof(int8_cuts[0]) == 10 && sizeof(int8_any_cuts) / sizeof(int8_any_cuts[0]) == 3, "as many as the rule looks at");
 
 /* p with k in bytes */
 Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
@@ -667,7 +682,7 @@ Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
     const double reached = p.rows >= 4 * p.experts ? p.experts : p.experts * (1.0 - pow(1.0 - 1.0 / p.experts, p.rows));
     const int cols = p.n_half ? p.n_half : p.N;
     Plan plan = {CUT_SHORT, 1, 0};
-    for (int i = 0; i < (aligned ? 7 : 3); ++i) {
+    for (int i = 0; i < (aligned ? 10 : 3); ++i) {
         const Int8Cut &c = aligned ? int8_cuts[i] : int8_any_cuts[i];
         const int tile_cols = p.n_half && c.cut != CUT_ROWS ? c.tn / 2 : c.tn;
         double m_tiles = (p.rows + c.tm - 1) / c.tm;
@@ -675,7 +690,7 @@ Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
             m_tiles = per_expert < c.tm * 0.25 ? reached : fmax(p.experts * (per_expert / c.tm + 0.5), reached);
         const double tiles = m_tiles * ((cols + tile_cols - 1) / tile_cols), memory = reached * p.N * p.K / c.stream;
         for (int splits = 1; splits <= 8; splits *= 2) {
-            if (splits > 1 && (p.experts > 1 || c.cut == CUT_WIDE || c.cut == CUT_ROWS || steps / splits < 4 || tiles * splits > 2048)) break;
+            if (splits > 1 && (p.experts > 1 || c.cut == CUT_WIDE || c.cut >= CUT_ROWS || steps / splits < 4 || tiles * splits > 2048)) break;
             const double cus = tiles * splits / 256.0, rounds = cus / c.at_once, part_steps = ceil(steps / splits);
             double t;
             if (rounds <= 1.0) {

@@ -410,12 +410,18 @@ template <int DT> __device__ __forceinline__ u32x4 x_raw4(const void *p, int f32
         r[1] = h[1];
         return r;
     }
+    if (there <= 0) return r;
+    /* all three loads are made, of the first element where there is no other, and are under way together */
+    uint32_t v[3];
+    if (f32) {
 #pragma unroll
-    for (int k = 0; k < 3; ++k)
-        if (k < there) {
-            if (f32) r[k] = static_cast<const uint32_t *>(p)[i + k];
-            else r[k >> 1] |= (uint32_t)static_cast<const uint16_t *>(p)[i + k] << ((k & 1) * 16);
-        }
+        for (int k = 0; k < 3; ++k) v[k] = static_cast<const uint32_t *>(p)[k < there ? i + k : i];
+        return u32x4{v[0], there > 1 ? v[1] : 0, there > 2 ? v[2] : 0, 0};
+    }
+#pragma unroll
+    for (int k = 0; k < 3; ++k) v[k] = static_cast<const uint16_t *>(p)[k < there ? i + k : i];
+    r[0] = there > 1 ? v[1] << 16 | v[0] : v[0];
+    r[1] = there > 2 ? v[2] : 0;
     return r;
 }
 template <int DT> __device__ __forceinline__ f32x4 x_of_raw4(const u32x4 &r, int f32)
@@ -443,17 +449,22 @@ template <int T> __device__ __forceinline__ void x_activate_all(const XgemmParam
         default: return;
     }
 }
-/* four values of the output, `there` of them */
-template <int DT> __device__ __forceinline__ void x_put(const XgemmParams &p, int64_t row, int j, int there, f32x4 y, const u32x4 &residual)
+/* four values, `there` of them */
+template <int DT> __device__ __forceinline__ void x_put4(void *p, int f32, int64_t i, int there, const f32x4 &y)
 {
-    if (p.residual) y += x_of_raw4<DT>(residual, p.out_f32);
     if (there >= 4) {
-        x_store4<DT>(p.out, p.out_f32, row * p.ldo + j, y);
+        x_store4<DT>(p, f32, i, y);
     } else {
 #pragma unroll
         for (int k = 0; k < 3; ++k)
-            if (k < there) x_store<DT>(p.out, p.out_f32, row * p.ldo + j + k, y[k]);
+            if (k < there) x_store<DT>(p, f32, i + k, y[k]);
     }
+}
+/* of the output */
+template <int DT> __device__ __forceinline__ void x_put(const XgemmParams &p, int64_t row, int j, int there, f32x4 y, const u32x4 &residual)
+{
+    if (p.residual) y += x_of_raw4<DT>(residual, p.out_f32);
+    x_put4<DT>(p.out, p.out_f32, row * p.ldo + j, there, y);
 }
 __device__ __forceinline__ f32x4 x_value(const f32x4 &v) { return v; }
 __device__ __forceinline__ f32x4 x_value(const i32x4 &v) { return __builtin_bit_cast(f32x4, v); }

@@ -433,53 +433,84 @@ expert_gemm_wide_kernel(XgemmParams p)
             x_scale_tile(acc, scales);
         }
         if constexpr (FULL) {
-            /* as the smaller tiles have it (zbal_expert_direct.h), four rows at a time: 64 of them in a pass, a lane has four columns of every eighth (without halves) */
+            /*
+             * As the smaller tiles have it (zbal_expert_direct.h), four rows at a time: 64 of them in a pass, a lane has four columns of every eighth (without halves). What
+             * a row has in memory is on its way before the rows in front of it are stored, and the type of both is chosen outside the loop, so that nothing in it waits for a
+             * store (4096 x 2048 x 7168, bf16: 58 us; with bias 77 -> 67, with a residual 110 -> 81, with gelu and both 128 -> 98).
+             */
             constexpr int PASS = 2, ROWS = PASS * 32, LD = TN + 4, AT_ONCE = 4;
             static_assert(x_is_i8<DT> && ROWS * LD * 4 <= 2 * STAGE, "sums fit the stages");
+            static_assert(ROWS % (WAVES * 64 / (TN / 8) * AT_ONCE) == 0, "a pass is whole turns of four rows, also of halves");
             float *sums = reinterpret_cast<float *>(smem);
             const int quads = tile_cols / 4, c = tid % quads * 4, j = t.n0 + c, there = cols - j, r0 = tid / quads, step = WAVES * 64 / quads;
-            u32x4 b = {0, 0, 0, 0}, bu = b;
-            if (p.bias) {
-                b = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there);
-                if (p.n_half) bu = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there);
-            }
-            asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+            auto rest = [&](auto in_32_bits, auto with_residual) __attribute__((always_inline)) {
+                constexpr bool F32 = decltype(in_32_bits)::value, RESIDUAL = decltype(with_residual)::value;
+                u32x4 b = {0, 0, 0, 0}, bu = b, next[AT_ONCE] = {b, b, b, b};
+                if (p.bias) {
+                    b = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there);
+                    if (p.n_half) bu = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there);
+                }
+                auto bring = [&](int from) __attribute__((always_inline)) {
+                    auto rows = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
-            for (int pass = 0; pass < MT / PASS; ++pass) {
-                __syncthreads();
-#pragma unroll
-                for (int h = 0; h < PASS; ++h)
-#pragma unroll
-                    for (int nt = 0; nt < NT; ++nt)
-                        *reinterpret_cast<f32x4 *>(sums + (h * 32 + wm * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
-                __syncthreads();
-                const int row0 = t.m0 + pass * ROWS;
+                        for (int h = 0; h < AT_ONCE; ++h) {
+                            const int row = t.m0 + from + h * step;
+                            next[h] = x_raw4<DT>(p.residual, F32, (row < t.m_end ? row : t.m_end - 1) * p.ldo + j, n);
+                        }
+                    };
+                    if (there >= 4) rows(4);
+                    else if (there > 0) rows(there);
+                };
+                asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
+                if constexpr (RESIDUAL) bring(r0);
 #pragma unroll 1
-                for (int r = r0; r < ROWS; r += step * AT_ONCE) {
-                    if (there <= 0) continue;
-                    u32x4 residual[AT_ONCE];
-                    f32x4 z[AT_ONCE], up[AT_ONCE];
+                for (int pass = 0; pass < MT / PASS; ++pass) {
+                    __syncthreads();
 #pragma unroll
-                    for (int h = 0; h < AT_ONCE; ++h) {
-                        const int row = row0 + r + h * step;
-                        residual[h] = u32x4{0, 0, 0, 0};
-                        if (p.residual) residual[h] = x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + j, row < t.m_end ? there : 0);
-                    }
+                    for (int k = 0; k < MT / PASS; ++k)
+                        if (pass == k) {
 #pragma unroll
-                    for (int h = 0; h < AT_ONCE; ++h) {
-                        const float *from = sums + (r + h * step) * LD + c;
-                        z[h] = *reinterpret_cast<const f32x4 *>(from) + x_of_raw4<DT>(b, p.bias_f32);
-                        up[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                        if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + x_of_raw4<DT>(bu, p.bias_f32);
-                    }
-                    x_activate_all<AT_ONCE>(p, z, up);
+                            for (int h = 0; h < PASS; ++h)
 #pragma unroll
-                    for (int h = 0; h < AT_ONCE; ++h) {
-                        const int row = row0 + r + h * step;
-                        if (row < t.m_end) x_put<DT>(p, row, j, there, z[h], residual[h]);
+                                for (int nt = 0; nt < NT; ++nt)
+                                    *reinterpret_cast<f32x4 *>(sums + (h * 32 + wm * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[k * PASS + h][nt]);
+                            asm volatile("" : : "n"(k));        /* without it the four become one, which picks its sums out of memory */
+                        }
+                    __syncthreads();
+#pragma unroll 1
+                    for (int r = r0; r < ROWS; r += step * AT_ONCE) {
+                        const int at = pass * ROWS + r;
+                        u32x4 now[AT_ONCE];
+                        f32x4 z[AT_ONCE], up[AT_ONCE];
+#pragma unroll
+                        for (int h = 0; h < AT_ONCE; ++h) now[h] = next[h];
+                        if constexpr (RESIDUAL)
+                            if (at + step * AT_ONCE < TM) bring(at + step * AT_ONCE);
+#pragma unroll
+                        for (int h = 0; h < AT_ONCE; ++h) {
+                            const float *from = sums + (r + h * step) * LD + c;
+                            z[h] = *reinterpret_cast<const f32x4 *>(from) + x_of_raw4<DT>(b, p.bias_f32);
+                            up[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
+                            if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + x_of_raw4<DT>(bu, p.bias_f32);
+                        }
+                        x_activate_all<AT_ONCE>(p, z, up);
+                        if constexpr (RESIDUAL)
+#pragma unroll
+                            for (int h = 0; h < AT_ONCE; ++h) z[h] += x_of_raw4<DT>(now[h], F32);
+                        auto out = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+                            for (int h = 0; h < AT_ONCE; ++h)
+                                if (t.m0 + at + h * step < t.m_end) x_put4<DT>(p.out, F32, (t.m0 + at + h * step) * p.ldo + j, n, z[h]);
+                        };
+                        if (there >= 4) out(4);
+                        else if (there > 0) out(there);
                     }
                 }
-            }
+            };
+            const std::true_type yes = {};
+            const std::false_type no = {};
+            if (p.out_f32) p.residual ? rest(yes, yes) : rest(yes, no);
+            else p.residual ? rest(no, yes) : rest(no, no);
             return;                                             /* nothing was brought behind the last step */
         }
         if (REDUCE || x_is_i8<DT> || !p.through_lds) {

@@ -469,7 +469,8 @@ ZBALHIP_API int32_t zbalhip_combine_backward(const void *grad, const void *y, in
  * weight [H] of x's type or fp32 (null: ones).
  *   h = x + residual, y = h weight / sqrt(mean(h^2) + eps), both in 32 bits; each output is rounded once from them.
  * y and total (= h), both [T, H] of x's type, and q [T, H] with scales [T] may be null, not all three: scale = the row's largest |y| / 127, q = y / scale,
- * rounded to nearest even. A row of zeros has the scale 0, another one 2^-126 at least, one with an infinity or a NaN the scale NaN (and any q).
+ * rounded to nearest even. A row of zeros has the scale 0, another one 2^-126 at least, one with an infinity or a NaN the scale NaN (and any q). A row whose
+ * squares add up to more than 32 bits hold (elements of 2^64 / sqrt(H) and more) has zeros for y, as 1 / sqrt(infinity) is.
  * The gradient: x is h (total, where there was a residual); residual is not read. grad [T, H] (of y) and grad_total (of total, may be null) of x's type ->
  * grad_x, that of x and of the residual, and grad_weight [H] (may be null) of x's type or fp32, a sum over the rows always in the same order; zeros
  * without rows. workspace: zbalhip_rms_norm_backward_workspace bytes (-1: the sizes are not allowed) where grad_weight is asked for, 16-byte aligned, undefined

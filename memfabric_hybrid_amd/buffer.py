@@ -448,7 +448,8 @@ class Buffer:
         residual (where there was one). quantize: y in int8 besides, q [tokens, hidden] with scales [tokens] fp32, the row's
         largest magnitude / 127, as an int8 dispatch leaves rows; need_norm=False leaves out y itself. Everything is computed
         in 32 bits and rounded once, q from the unrounded y. A row of zeros has the scale 0, one with an infinity or a NaN the
-        scale NaN. Returns (y, q, scales, total): None for what was not asked for."""
+        scale NaN; where the squares of a row add up to more than 32 bits hold, y is zeros. Returns (y, q, scales, total): None
+        for what was not asked for."""
         return self.runtime.rms_norm(x, weight, residual, eps, quantize, need_norm)
 
     def rms_norm_backward(self, grad: torch.Tensor, x: torch.Tensor, weight: Optional[torch.Tensor] = None,

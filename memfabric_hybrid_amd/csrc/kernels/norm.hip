@@ -327,7 +327,7 @@ rms_norm_backward_kernel(NormParams p)
 #pragma unroll
         for (int i = 0; i < 8; ++i) columns[l.group * per_row + l.of_row * 8 + i] = dw[0][i];
         __syncthreads();
-        for (int col = l.group * (int)blockDim.x + l.of_row; p.grad_weight && col < p.width; col += blockDim.x * blockDim.y) {
+        for (int col = l.group * (int)blockDim.x + l.of_row; col < p.width; col += blockDim.x * blockDim.y) {
             float sum = 0.0f;
             for (int g = 0; g < l.rows; ++g) sum += columns[g * per_row + col];
             if (p.weight_grad_f32) static_cast<float *>(p.grad_weight)[col] = sum;

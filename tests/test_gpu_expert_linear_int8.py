@@ -223,6 +223,19 @@ def test_past_32_bits_of_offset(buf):
         del x, y
 
 
+def test_past_32_bits_of_offset_with_an_epilogue(buf):
+    """bias, residual and outputs of more than 2^31 elements"""
+    rows, K, N = 33000, 64, 65536
+    g, x, xs, w, ws, _ = make(rows, 1, K, N, 5)
+    b, r = torch.randn((N,), device="cuda", generator=g), torch.randn((rows, N), device="cuda", generator=g, dtype=torch.bfloat16)
+    y = buf.expert_linear_int8(x, xs, w, ws, bias=b, residual=r, activation="relu")
+    for at in (slice(0, 3), slice(rows // 2, rows // 2 + 3), slice(rows - 3, rows)):
+        z = product64(x[at], xs[at], w, ws, [3]) + b.double()
+        v = torch.relu(z) + r[at].double()
+        err = 4 * U * (z - b.double()).abs() + 2 * U * z.abs() + U * v.abs()
+        assert ((y[at].double() - v).abs() <= half_step(torch.bfloat16) * (v.abs() + err) + err).all()
+
+
 @pytest.mark.parametrize("rows,E,K,N", [(4, 1, 4096, 512), (40, 8, 512, 512), (2000, 4, 1024, 520), (500, 1, 8192, 128), (8200, 1, 512, 264), (1000, 1, 1001, 333), (9000, 8, 272, 2048)])
 def test_the_same_every_time_and_captured(buf, rows, E, K, N):
     g, x, xs, w, ws, counts = make(rows, E, K, N, 5)
@@ -278,6 +291,43 @@ def test_residual_in_place(buf):
     r = torch.randn((70, 264), device="cuda").to(torch.bfloat16)
     want = buf.expert_linear_int8(x, xs, w, ws, residual=r)
     assert torch.equal(buf.expert_linear_int8(x, xs, w, ws, residual=r, out=r), want)
+
+
+@pytest.mark.parametrize("rows,E,K,N,act", [(3, 1, 2048, 512, "none"), (600, 1, 1101, 700, "swiglu"), (2000, 1, 4099, 1003, "silu"), (4100, 3, 256, 2056, "swiglu"),
+                                            (4100, 1, 256, 2053, "gelu"), (300, 8, 512, 520, "silu")])
+@pytest.mark.parametrize("out", TYPES)
+def test_residual_in_place_of_every_tile(buf, rows, E, K, N, act, out):
+    """the residual's rows are read ahead of what is stored on them"""
+    g, x, xs, w, ws, counts = make(rows, E, K, N, 14)
+    ct = torch.tensor(counts, dtype=torch.int32, device="cuda")
+    r = torch.randn((rows, N // 2 if act == "swiglu" else N), device="cuda", generator=g).to(out)
+    want = buf.expert_linear_int8(x, xs, w, ws, ct, activation=act, residual=r, out_dtype=out)
+    for _ in range(3):
+        y = r.clone()
+        assert torch.equal(buf.expert_linear_int8(x, xs, w, ws, ct, activation=act, residual=y, out_dtype=out, out=y), want)
+
+
+def test_streams_side_by_side(buf):
+    """calls that run side by side share nothing: parts, copies and a gradient's sums lie in workspaces of their own"""
+    sets = []
+    for rows, K, N in ((1087, 5264, 364), (2000, 4099, 1003), (64, 4096, 512)):
+        g, x, xs, w, ws, _ = make(rows, 1, K, N, 15)
+        sets.append([(torch.randint(-128, 128, x.shape, device="cuda", generator=g, dtype=torch.int8), xs, w, ws) for _ in range(4)])
+    h = [torch.randn((500, 1536), device="cuda") for _ in range(8)]
+    norm = lambda i: buf.rms_norm_backward(h[i], h[i + 4])  # noqa: E731
+    want = [[buf.expert_linear_int8(*v) for v in s] for s in sets]
+    back = [norm(i) for i in range(4)]
+    streams = [torch.cuda.Stream() for _ in range(4)]
+    torch.cuda.synchronize()
+    got, gradients = [], []
+    for _ in range(3):
+        for i, stream in enumerate(streams):
+            with torch.cuda.stream(stream):
+                got.append((i, [buf.expert_linear_int8(*s[i]) for s in sets]))
+                gradients.append((i, norm(i)))
+    torch.cuda.synchronize()
+    assert all(torch.equal(a, want[k][i]) for i, ys in got for k, a in enumerate(ys))
+    assert all(torch.equal(a, b) for i, ys in gradients for a, b in zip(ys, back[i]))
 
 
 def test_refusals(buf):

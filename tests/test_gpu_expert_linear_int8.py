@@ -162,6 +162,14 @@ def test_counts(buf, counts, K, N):
     case(buf, 50, 4, K, N, torch.bfloat16, counts=counts, count_dtype=torch.int64)
 
 
+@pytest.mark.parametrize("rows,K,N,act", [(5, 640, 256, "none"), (40, 133, 66, "silu"), (711, 6100, 271, "none"), (1066, 7744, 226, "swiglu"), (700, 528, 1032, "gelu"),
+                                          (1, 3644, 2302, "none"), (4100, 272, 2053, "silu"), (4100, 256, 2056, "none"), (2000, 4099, 1003, "none")])
+@pytest.mark.parametrize("share", [0, 0.4, 1, 5])
+def test_one_experts_count(buf, rows, K, N, act, share):
+    """one expert that has fewer rows than there are, or claims more, in every kind of tile and in parts"""
+    case(buf, rows, 1, K, N, torch.bfloat16, act, counts=[int(rows * share)], residual=act != "none", seed=4)
+
+
 def test_sums_are_exact(buf):
     """all products at their largest: 2^14 each, 2^30 in all, and values that differ in the last bit of a sum of 2^24"""
     for K in (65536, 65535):

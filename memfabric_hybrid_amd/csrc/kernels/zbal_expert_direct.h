@@ -266,12 +266,23 @@ expert_gemm_kernel(XgemmParams p)
             bias4 = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + q_j, q_there);
             if (p.n_half) bias_up4 = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)expert * p.N + p.n_half + q_j, q_there);
         }
-        if (p.residual)
+        /* one branch for all of them, so that nothing comes between the loads */
+        auto bring_residual = [&](int f32, int n) __attribute__((always_inline)) {
 #pragma unroll
             for (int i = 0; i < MT / PASS * TURNS; ++i) {
                 const int row = row_of(i / TURNS, q_row + i % TURNS * ROW_STEP);
-                residual4[i] = x_raw4<DT>(p.residual, p.out_f32, row * p.ldo + q_j, row < m_end ? q_there : 0);
+                residual4[i] = x_raw4<DT>(p.residual, f32, (row < m_end ? row : m_end - 1) * p.ldo + q_j, n);
             }
+        };
+        if (p.residual) {
+            if (q_there < 4) {
+                if (q_there > 0) bring_residual(p.out_f32, q_there);
+            } else if (p.out_f32) {
+                bring_residual(1, 4);
+            } else {
+                bring_residual(0, 4);
+            }
+        }
     }
 #pragma unroll
     for (int i = 0; i < STAGES - 1; ++i) bring_next(i);
@@ -376,31 +387,46 @@ expert_gemm_kernel(XgemmParams p)
                 *reinterpret_cast<f32x4 *>(sums + (wm * (PASS * 16) + h * 16 + (lane & 15)) * LD + col_of(nt) + q4) = x_value(acc[pass * PASS + h][nt]);
         __syncthreads();
         if constexpr (x_is_i8<DT>) {
-            /* two rows at a time */
-            u32x4 waiting[TURNS];
+            /* two rows at a time, the types chosen outside the loop (1021 x 1008 x 1536 with residual 10.1 -> 9.7 us, with gelu, bias and residual 11.3 -> 10.8) */
+            auto rows_out = [&](auto in_32_bits, auto with_residual) __attribute__((always_inline)) {
+                constexpr bool F32 = decltype(in_32_bits)::value, RESIDUAL = decltype(with_residual)::value;
+                u32x4 waiting[RESIDUAL ? TURNS : 1];
+                if constexpr (RESIDUAL)
 #pragma unroll
-            for (int i = 0; i < TURNS; ++i) waiting[i] = residual4[pass * TURNS + i];
-            const f32x4 b = x_of_raw4<DT>(bias4, p.bias_f32), bu = x_of_raw4<DT>(bias_up4, p.bias_f32);
+                    for (int i = 0; i < TURNS; ++i) waiting[i] = residual4[pass * TURNS + i];
+                const f32x4 b = x_of_raw4<DT>(bias4, p.bias_f32), bu = x_of_raw4<DT>(bias_up4, p.bias_f32);
 #pragma unroll 1
-            for (int i = 0; i < TURNS; i += 2) {
-                const u32x4 now[2] = {waiting[0], waiting[1]};
+                for (int i = 0; i < TURNS; i += 2) {
+                    if (q_there <= 0) continue;
+                    f32x4 z[2], up[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
 #pragma unroll
-                for (int k = 2; k < TURNS; ++k) waiting[k - 2] = waiting[k];
-                if (q_there <= 0) continue;
-                f32x4 z[2], up[2] = {{0.0f, 0.0f, 0.0f, 0.0f}, {0.0f, 0.0f, 0.0f, 0.0f}};
+                    for (int h = 0; h < 2; ++h) {
+                        const float *from = sums + (q_row + (i + h) * ROW_STEP) * LD + q_col;
+                        z[h] = *reinterpret_cast<const f32x4 *>(from) + b;
+                        if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + bu;
+                    }
+                    x_activate_all<2>(p, z, up);
+                    if constexpr (RESIDUAL) {
 #pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const float *from = sums + (q_row + (i + h) * ROW_STEP) * LD + q_col;
-                    z[h] = *reinterpret_cast<const f32x4 *>(from) + b;
-                    if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + bu;
+                        for (int h = 0; h < 2; ++h) z[h] += x_of_raw4<DT>(waiting[h], F32);
+#pragma unroll
+                        for (int k = 2; k < TURNS; ++k) waiting[k - 2] = waiting[k];
+                    }
+                    auto out = [&](int n) __attribute__((always_inline)) {
+#pragma unroll
+                        for (int h = 0; h < 2; ++h) {
+                            const int row = row_of(pass, q_row + (i + h) * ROW_STEP);
+                            if (row < m_end) x_put4<DT>(p.out, F32, row * p.ldo + q_j, n, z[h]);
+                        }
+                    };
+                    if (q_there >= 4) out(4);
+                    else out(q_there);
                 }
-                x_activate_all<2>(p, z, up);
-#pragma unroll
-                for (int h = 0; h < 2; ++h) {
-                    const int row = row_of(pass, q_row + (i + h) * ROW_STEP);
-                    if (row < m_end) x_put<DT>(p, row, q_j, q_there, z[h], now[h]);
-                }
-            }
+            };
+            const std::true_type yes = {};
+            const std::false_type no = {};
+            if (p.out_f32) p.residual ? rows_out(yes, yes) : rows_out(yes, no);
+            else p.residual ? rows_out(no, yes) : rows_out(no, no);
             continue;
         }
 #pragma unroll 1

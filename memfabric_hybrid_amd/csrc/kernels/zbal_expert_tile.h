@@ -449,7 +449,7 @@ template <int T> __device__ __forceinline__ void x_activate_all(const XgemmParam
         default: return;
     }
 }
-/* four values, `there` of them */
+/* four values of the output, `there` of them */
 template <int DT> __device__ __forceinline__ void x_put4(void *p, int f32, int64_t i, int there, const f32x4 &y)
 {
     if (there >= 4) {
@@ -459,12 +459,6 @@ template <int DT> __device__ __forceinline__ void x_put4(void *p, int f32, int64
         for (int k = 0; k < 3; ++k)
             if (k < there) x_store<DT>(p, f32, i + k, y[k]);
     }
-}
-/* of the output */
-template <int DT> __device__ __forceinline__ void x_put(const XgemmParams &p, int64_t row, int j, int there, f32x4 y, const u32x4 &residual)
-{
-    if (p.residual) y += x_of_raw4<DT>(residual, p.out_f32);
-    x_put4<DT>(p.out, p.out_f32, row * p.ldo + j, there, y);
 }
 __device__ __forceinline__ f32x4 x_value(const f32x4 &v) { return v; }
 __device__ __forceinline__ f32x4 x_value(const i32x4 &v) { return __builtin_bit_cast(f32x4, v); }

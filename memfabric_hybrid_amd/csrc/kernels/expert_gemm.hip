@@ -429,7 +429,7 @@ template <int DT> void launch_rows(const XgemmParams &p, hipStream_t st)
 
 template <int DT, bool REDUCE, bool B_TR> void launch_wide(XgemmParams p, hipStream_t st)
 {
-    p.through_lds = !REDUCE && (p.bias || p.residual || p.preact || (p.act != ACT_NONE && p.act != ACT_SWIGLU));
+    p.through_lds = !REDUCE && ((p.bias && !x_is_i8<DT>) || p.residual || p.preact || (p.act != ACT_NONE && p.act != ACT_SWIGLU));
     unsigned blocks = tiles_of<REDUCE, 256, 256>(p);
     if (!p.through_lds && blocks > XW_CUS) blocks = XW_CUS;
     const dim3 grid(blocks), block(512);

@@ -431,6 +431,21 @@ template <int DT> __device__ __forceinline__ f32x4 x_of_raw4(const u32x4 &r, int
     return f32x4{zb_half_to_f32<H>(r[0] & 0xffffu), zb_half_to_f32<H>(r[0] >> 16), zb_half_to_f32<H>(r[1] & 0xffffu), zb_half_to_f32<H>(r[1] >> 16)};
 }
 
+/* the bias of a lane's columns, as it lies in memory, and its addition to the bits of the values that integers have become */
+template <int DT, int NT, typename Col>
+__device__ __forceinline__ void x_load_bias(u32x4 (&b)[NT], const void *bias, int bias_f32, int64_t first, Col col)
+{
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt) b[nt] = x_raw4<DT>(bias, bias_f32, first + col(nt).first, col(nt).there);
+}
+template <int DT, int MT, int NT> __device__ __forceinline__ void x_add_bias(i32x4 (&acc)[MT][NT], const u32x4 (&b)[NT], int bias_f32)
+{
+#pragma unroll
+    for (int nt = 0; nt < NT; ++nt)
+#pragma unroll
+        for (int mt = 0; mt < MT; ++mt) acc[mt][nt] = __builtin_bit_cast(i32x4, __builtin_bit_cast(f32x4, acc[mt][nt]) + x_of_raw4<DT>(b[nt], bias_f32));
+}
+
 /* T times four values behind the activation, which is chosen once for all of them, so that their chains of operations run side by side; z and up have their biases */
 template <int T> __device__ __forceinline__ void x_activate_all(const XgemmParams &p, f32x4 (&z)[T], const f32x4 (&up)[T])
 {

@@ -18,7 +18,7 @@ namespace {
 constexpr int XW_CUS = 256;
 
 /*
- * BIAS (REDUCE): the operand whose columns are summed for the bias's gradient besides, 1 = b, 2 = a, 0 = none. FULL (int8): an epilogue of more than a swiglu, with a
+ * BIAS (REDUCE): the operand whose columns are summed for the bias's gradient besides, 1 = b, 2 = a, 0 = none. FULL (int8): an epilogue of more than a bias and a swiglu, with a
  * workgroup per tile; the registers of the next tile's fragments are then its own (half precision chooses between the two as it runs).
  */
 template <int DT, bool REDUCE, bool B_TR, int BIAS = 0, bool FULL = false>
@@ -423,20 +423,26 @@ expert_gemm_wide_kernel(XgemmParams p)
         if constexpr (x_is_i8<DT>) {
             const args_t p = fresh_args();
             const int lane = fresh_lane(), first = t.n0 + (p->n_half ? wn * 32 : wn * 64) + (lane >> 4) * 4;
+            auto col = [&](int nt) __attribute__((always_inline)) {
+                const bool up = p->n_half && nt >= NT / 2;
+                const int j = first + (up ? nt - NT / 2 : nt) * 16;
+                return XCols{j + (up ? p->n_half : 0), cols - j};
+            };
             XScales<MT, NT> scales;
-            x_load_scales(scales, p->a_scale, p->b_scale, p->b_scale_f32, (int64_t)t.expert * p->N, t.m_end, [&](int mt) { return t.m0 + mt * 32 + wm * 16 + (lane & 15); },
-                          [&](int nt) {
-                              const bool up = p->n_half && nt >= NT / 2;
-                              const int j = first + (up ? nt - NT / 2 : nt) * 16;
-                              return XCols{j + (up ? p->n_half : 0), cols - j};
-                          });
+            x_load_scales(scales, p->a_scale, p->b_scale, p->b_scale_f32, (int64_t)t.expert * p->N, t.m_end, [&](int mt) { return t.m0 + mt * 32 + wm * 16 + (lane & 15); }, col);
             x_scale_tile(acc, scales);
+            /* a bias is added where the sums are (4096 x 2048 x 7168 68 us on their way through the LDS, 59) */
+            if (p->bias) {
+                u32x4 b[NT];
+                x_load_bias<DT>(b, p->bias, p->bias_f32, (int64_t)t.expert * p->N, col);
+                x_add_bias<DT>(acc, b, p->bias_f32);
+            }
         }
         if constexpr (FULL) {
             /*
              * As the smaller tiles have it (zbal_expert_direct.h), four rows at a time: 64 of them in a pass, a lane has four columns of every eighth (without halves). What
              * a row has in memory is on its way before the rows in front of it are stored, and the type of both is chosen outside the loop, so that nothing in it waits for a
-             * store (4096 x 2048 x 7168, bf16: 58 us; with bias 77 -> 67, with a residual 110 -> 81, with gelu and both 128 -> 98).
+             * store (4096 x 2048 x 7168, bf16: 58 us; with a residual 110 -> 81, with gelu, bias and residual 128 -> 99).
              */
             constexpr int PASS = 2, ROWS = PASS * 32, LD = TN + 4, AT_ONCE = 4;
             static_assert(x_is_i8<DT> && ROWS * LD * 4 <= 2 * STAGE, "sums fit the stages");
@@ -445,11 +451,7 @@ expert_gemm_wide_kernel(XgemmParams p)
             const int quads = tile_cols / 4, c = tid % quads * 4, j = t.n0 + c, there = cols - j, r0 = tid / quads, step = WAVES * 64 / quads;
             auto rest = [&](auto in_32_bits, auto with_residual) __attribute__((always_inline)) {
                 constexpr bool F32 = decltype(in_32_bits)::value, RESIDUAL = decltype(with_residual)::value;
-                u32x4 b = {0, 0, 0, 0}, bu = b, next[AT_ONCE] = {b, b, b, b};
-                if (p.bias) {
-                    b = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + j, there);
-                    if (p.n_half) bu = x_raw4<DT>(p.bias, p.bias_f32, (int64_t)t.expert * p.N + p.n_half + j, there);
-                }
+                u32x4 next[AT_ONCE] = {};
                 auto bring = [&](int from) __attribute__((always_inline)) {
                     auto rows = [&](int n) __attribute__((always_inline)) {
 #pragma unroll
@@ -489,9 +491,9 @@ expert_gemm_wide_kernel(XgemmParams p)
 #pragma unroll
                         for (int h = 0; h < AT_ONCE; ++h) {
                             const float *from = sums + (r + h * step) * LD + c;
-                            z[h] = *reinterpret_cast<const f32x4 *>(from) + x_of_raw4<DT>(b, p.bias_f32);
+                            z[h] = *reinterpret_cast<const f32x4 *>(from);
                             up[h] = f32x4{0.0f, 0.0f, 0.0f, 0.0f};
-                            if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2) + x_of_raw4<DT>(bu, p.bias_f32);
+                            if (p.n_half) up[h] = *reinterpret_cast<const f32x4 *>(from + TN / 2);
                         }
                         x_activate_all<AT_ONCE>(p, z, up);
                         if constexpr (RESIDUAL)

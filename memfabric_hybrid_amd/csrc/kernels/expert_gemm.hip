@@ -273,16 +273,19 @@ expert_join_kernel(XgemmParams p)
 
 /*
  * Rows of int8 whose length is no multiple of 16 bytes, copied to rows of one that is, zeros behind their ends, so that the tiles for aligned operands can have
- * them: the rows of x, then those of W. `lanes` of them to a row, sixteen bytes each at a time; the last of a row are taken from its last sixteen.
+ * them: the rows of x that experts have, then those of W. `lanes` of them to a row, sixteen bytes each at a time; the last of a row are taken from its last sixteen.
  */
 struct XAlign { const uint8_t *from[2]; uint8_t *to[2]; int64_t rows[2]; int k, k_to, lanes; };
 __global__ void __launch_bounds__(256)
-expert_align_kernel(XAlign p)
+expert_align_kernel(XgemmParams of_rows, XAlign p)
 {
     const int per_block = 256 / p.lanes, c0 = (threadIdx.x % p.lanes) * 16;
-    const int64_t step = (int64_t)gridDim.x * per_block;
-    for (int64_t r = (int64_t)blockIdx.x * per_block + threadIdx.x / p.lanes; r < p.rows[0] + p.rows[1]; r += step) {
+    const int64_t first = (int64_t)blockIdx.x * per_block, step = (int64_t)gridDim.x * per_block;
+    /* workgroups that come to no row of x need not know where those of nobody begin */
+    const int64_t x_end = of_rows.counts && first < p.rows[0] ? x_rows_in_all(of_rows) : p.rows[0];
+    for (int64_t r = first + threadIdx.x / p.lanes; r < p.rows[0] + p.rows[1]; r += step) {
         const int of = r >= p.rows[0];
+        if (!of && r >= x_end) continue;
         const int64_t row = of ? r - p.rows[0] : r;
         const uint8_t *from = p.from[of] + row * p.k;
         uint8_t *to = p.to[of] + row * p.k_to;
@@ -847,8 +850,10 @@ extern "C" int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t
         uint8_t *to = (uint8_t *)workspace;
         XAlign c = {{(const uint8_t *)x, (const uint8_t *)d->weight}, {to, to + plan.x_bytes}, {d->rows, d->experts * d->n}, (int)d->k, p.K * 2, 1};
         while (c.lanes < 64 && c.lanes * 16 < c.k) c.lanes *= 2;
-        const int64_t blocks = (c.rows[0] + c.rows[1] + 256 / c.lanes - 1) / (256 / c.lanes);
-        zb_launch(expert_align_kernel, dim3((unsigned)(blocks < 8192 ? blocks : 8192)), dim3(256), 0, (hipStream_t)stream, c);
+        /* where rows have to be counted, up to six rounds of them share that (us with 2048 workgroups / 8192: 9620 groups of rows, 20000 over 70 experts of 519 x 264, 39.2 / 40.4; 15686
+           groups, 30000 over 8 of 2003 x 4093, 314 / 311) */
+        const int64_t groups = (c.rows[0] + c.rows[1] + 256 / c.lanes - 1) / (256 / c.lanes), most = p.counts && groups <= 6 * 2048 ? 2048 : 8192;
+        zb_launch(expert_align_kernel, dim3((unsigned)(groups < most ? groups : most)), dim3(256), 0, (hipStream_t)stream, p, c);
         p.a = (const uint16_t *)c.to[0];
         p.b = (const uint16_t *)c.to[1];
         workspace = c.to[1] + plan.w_bytes;

@@ -160,6 +160,15 @@ __device__ __forceinline__ XSpan x_rows_of(const XgemmParams &p, int e)
     }
 }
 
+/* where the last expert's rows end, for a whole wave: all counts are loaded at once. A lane's sum that stops at the last row leaves the result what it is */
+__device__ __forceinline__ int x_rows_in_all(const XgemmParams &p)
+{
+    uint32_t sum = 0;
+    for (int e = threadIdx.x & 63; e < p.experts; e += 64) sum += x_count(p, e);
+    const uint32_t r = (uint32_t)p.rows, all = (uint32_t)zb_wave_sum_dpp((int)(sum < r ? sum : r));
+    return (int)(all < r ? all : r);
+}
+
 struct XTile { int expert, row_begin, row_end, n_tile; };
 
 /*

@@ -294,6 +294,29 @@ def test_parts_and_copies_give_the_same_bits(buf):
     assert split == 7
 
 
+@pytest.mark.parametrize("rows,E,K,N,counts,long", [(2000, 1, 4099, 1003, [700], False), (2000, 1, 4099, 1003, [0], True), (1087, 1, 5265, 364, [1086], False),
+                                                    (3974, 3, 1651, 1344, [1, 0, 1500], True), (20000, 70, 519, 264, [31] * 70, False),
+                                                    (9566, 8, 1670, 320, [900] * 8, False), (9566, 8, 1670, 320, [2000] * 8, True)])
+def test_copies_leave_rows_of_nobody_alone(buf, rows, E, K, N, counts, long):
+    """rows past the last expert's are neither read nor written, also where unaligned rows are copied to the workspace, x's in front"""
+    import ctypes
+    lib, wide = capi.load(), (K + 15) // 16 * 16
+    g, x, xs, w, ws, _ = make(rows, E, K, N, 6, counts)
+    n = min(rows, sum(counts))
+    ct = torch.tensor(counts, dtype=torch.int64 if long else torch.int32, device="cuda")
+    d = capi.ExpertLinearInt8(w.data_ptr(), ws.data_ptr(), 1, int(long), ct.data_ptr(), 0, capi.DT_FP32, rows, K, N, E)
+    size = lib.zbalhip_expert_linear_int8_workspace(ctypes.byref(d))
+    assert size >= (rows + E * N) * wide                     # the rule copies these
+    part, y = torch.full((size,), 0x5a, dtype=torch.uint8, device="cuda"), torch.full((rows, N), 77.0, device="cuda")
+    assert lib.zbalhip_expert_linear_int8(ctypes.byref(d), x.data_ptr(), xs.data_ptr(), None, 0, None, y.data_ptr(), part.data_ptr(), size,
+                                          torch.cuda.current_stream().cuda_stream) == 0
+    copies = part[:rows * wide].view(rows, wide)
+    assert torch.equal(copies[:n, :K].view(torch.int8), x[:n]) and (copies[:n, K:] == 0).all()
+    assert (copies[n:] == 0x5a).all()
+    want = product64(x, xs, w, ws, counts)
+    assert ((y[:n].double() - want).abs() <= 4 * U * want.abs() + 1e-37).all() and (y[n:] == 77.0).all()
+
+
 def test_residual_in_place(buf):
     g, x, xs, w, ws, _ = make(70, 1, 200, 264, 4)
     r = torch.randn((70, 264), device="cuda").to(torch.bfloat16)

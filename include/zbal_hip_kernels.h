@@ -516,6 +516,11 @@ typedef struct {
     int64_t rows, k, n, experts;
 } zbalhip_expert_linear_int8_t;
 ZBALHIP_API int64_t zbalhip_expert_linear_int8_workspace(const zbalhip_expert_linear_int8_t *linear);
+/*
+ * How a product with that workspace is cut: the kind of its tiles ("256x256" ... "16x64", "rows" for sixteen columns straight from memory; "... flat": rings of two stages,
+ * "... any": rows as they lie, "short": of less than 16 k), the parts along k, and whether rows are copied to aligned ones first. Null: no rows, or sizes that are not allowed.
+ */
+ZBALHIP_API const char *zbalhip_expert_linear_int8_plan(const zbalhip_expert_linear_int8_t *linear, int32_t *parts, int32_t *copied);
 ZBALHIP_API int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t *linear, const void *x, const float *x_scales, const void *bias,
                                    int32_t bias_is_f32, const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream);
 

@@ -237,6 +237,7 @@ SIGNATURES = {
     "zbalhip_rms_norm_backward": (_i32, [ctypes.POINTER(RmsNorm), _vp, _vp, _vp, _vp, _i32, _vp, _i64, _vp]),
     "zbalhip_quantize_rows": (_i32, [ctypes.POINTER(QuantizeRows), _vp, _vp, _vp, _vp]),
     "zbalhip_expert_linear_int8_workspace": (_i64, [ctypes.POINTER(ExpertLinearInt8)]),
+    "zbalhip_expert_linear_int8_plan": (ctypes.c_char_p, [ctypes.POINTER(ExpertLinearInt8), ctypes.POINTER(_i32), ctypes.POINTER(_i32)]),
     "zbalhip_expert_linear_int8": (_i32, [ctypes.POINTER(ExpertLinearInt8), _vp, _vp, _vp, _i32, _vp, _vp, _vp, _i64, _vp]),
 }
 

@@ -836,6 +836,31 @@ extern "C" int64_t zbalhip_expert_linear_int8_workspace(const zbalhip_expert_lin
     return d->rows == 0 ? 0 : plan_int8(d).bytes;
 }
 
+extern "C" const char *zbalhip_expert_linear_int8_plan(const zbalhip_expert_linear_int8_t *d, int32_t *parts, int32_t *copied)
+{
+    if (!int8_sizes_ok(d) || d->rows == 0) return nullptr;
+    const Int8Plan plan = plan_int8(d);
+    if (parts) *parts = plan.cut.splits;
+    if (copied) *copied = plan.copies;
+    switch (plan.cut.cut) {
+        case CUT_WIDE: return "256x256";
+        case CUT_128: return "128x128";
+        case CUT_64_128: return "64x128";
+        case CUT_64: return "64x64";
+        case CUT_32: return "32x128";
+        case CUT_16: return "16x64";
+        case CUT_ROWS: return "rows";
+        case CUT_64_FLAT: return "64x64 flat";
+        case CUT_32_FLAT: return "32x128 flat";
+        case CUT_16_FLAT: return "16x64 flat";
+        case CUT_ANY: return "128x128 any";
+        case CUT_ANY_64: return "64x64 any";
+        case CUT_ANY_16: return "16x128 any";
+        case CUT_SHORT: return "short";
+    }
+    return nullptr;
+}
+
 extern "C" int32_t zbalhip_expert_linear_int8(const zbalhip_expert_linear_int8_t *d, const void *x, const float *x_scales, const void *bias, int32_t bias_is_f32,
                                               const void *residual, void *y, void *workspace, int64_t workspace_bytes, void *stream)
 {

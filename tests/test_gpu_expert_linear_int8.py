@@ -3,6 +3,7 @@ without rows, counts that are wrong, rows of nobody; and a layer that is made of
 import pytest
 import torch
 
+from int8_cuts import CASES
 from memfabric_hybrid_amd import capi
 from memfabric_hybrid_amd.buffer import Buffer
 
@@ -151,6 +152,39 @@ def test_every_kind_of_the_rule(buf, rows, E, K, N, act):
     case(buf, rows, E, K, N, torch.float32, act)
     case(buf, rows, E, K, N, torch.float16, "silu" if act == "none" else act, bias=torch.float16, residual=True, seed=1)
     case(buf, rows, E, K, N, torch.bfloat16, act, bias=torch.float32, scale_type=torch.bfloat16, seed=2)
+
+
+@pytest.mark.parametrize("cut,rows,E,K,N,act", CASES)
+def test_every_kind_by_its_name(buf, cut, rows, E, K, N, act):
+    import ctypes
+    d = capi.ExpertLinearInt8(None, None, 1, 0, None, capi.ACTIVATIONS[act], capi.DT_FP32, rows, K, N, E)
+    parts, copied = ctypes.c_int32(), ctypes.c_int32()
+    assert (capi.load().zbalhip_expert_linear_int8_plan(ctypes.byref(d), ctypes.byref(parts), ctypes.byref(copied)).decode(), parts.value, copied.value) == cut
+    plain = act == "none"
+    case(buf, rows, E, K, N, torch.float32, act)
+    case(buf, rows, E, K, N, torch.float16, "silu" if plain else act, bias=torch.float16, residual=True, seed=1)
+    case(buf, rows, E, K, N, torch.bfloat16, act, bias=torch.float32, scale_type=torch.bfloat16, seed=2)
+    case(buf, rows, E, K, N, torch.float32, "gelu" if plain else act, residual=True, count_dtype=torch.int64, seed=3)
+    if plain:
+        case(buf, rows, E, K, N, torch.bfloat16, "gelu_tanh", seed=4)
+
+
+@pytest.mark.parametrize("cut,rows,E,K,N,act", CASES)
+def test_every_kind_with_rows_of_nobody_and_in_place(buf, cut, rows, E, K, N, act):
+    """rows past the last expert's, whose scales and residuals are NaN, stay what they are; the residual's rows are read before they are written"""
+    n = rows * 2 // 3
+    counts = [n] if E == 1 else [0] + [n // (E - 1)] * (E - 1)
+    n = sum(counts)
+    g, x, xs, w, ws, _ = make(rows, E, K, N, 7, counts)
+    r = torch.randn((rows, N // 2 if act == "swiglu" else N), device="cuda", generator=g)
+    xs[n:], r[n:] = float("nan"), float("nan")
+    ct, b = torch.tensor(counts, dtype=torch.int32, device="cuda"), torch.randn((E, N), device="cuda", generator=g)
+    whole = buf.expert_linear_int8(x[:n].clone(), xs[:n].clone(), w, ws, ct, b, "silu" if act == "none" else act, r[:n].clone(), torch.float32)
+    out = torch.full_like(r, 77.0)
+    buf.expert_linear_int8(x, xs, w, ws, ct, b, "silu" if act == "none" else act, r, torch.float32, out)
+    assert torch.equal(out[:n], whole) and (out[n:] == 77.0).all()
+    buf.expert_linear_int8(x, xs, w, ws, ct, b, "silu" if act == "none" else act, r, torch.float32, r)
+    assert torch.equal(r[:n], whole) and torch.isnan(r[n:]).all()
 
 
 @pytest.mark.parametrize("counts", [[0, 0, 0, 0], [0, 0, 0, 50], [50, 0, 0, 0], [10, 10, 10, 10], [-5, 20, -(1 << 31), 10], [30, 1 << 30, 7, (1 << 31) - 1],

@@ -6,6 +6,7 @@ import subprocess
 
 import pytest
 
+from int8_cuts import CASES
 from memfabric_hybrid_amd import capi
 
 INC = os.path.join(os.path.dirname(os.path.dirname(os.path.abspath(__file__))), "include")
@@ -119,6 +120,37 @@ def test_linear_workspace_sizes(lib):
     assert lib.zbal_moe_expert_linear_int8_workspace_size(4093, 4099, 4093, 1, 0) == 2 * 4093 * 4112
     assert lib.zbal_moe_expert_linear_int8_workspace_size(16, 4001, 1531, 32, 0) == 0
     assert lib.zbal_moe_expert_linear_int8_workspace_size(1 << 20, 4099, 4093, 1, 0) == 0
+
+
+def plan(lib, rows, experts, k, n, act):
+    parts, copied = ctypes.c_int32(-1), ctypes.c_int32(-1)
+    name = lib.zbalhip_expert_linear_int8_plan(ctypes.byref(linear(rows=rows, experts=experts, k=k, n=n, activation=capi.ACTIVATIONS[act])), ctypes.byref(parts), ctypes.byref(copied))
+    return name and (name.decode(), parts.value, copied.value)
+
+
+@pytest.mark.parametrize("cut,rows,experts,k,n,act", CASES)
+def test_linear_plans(lib, cut, rows, experts, k, n, act):
+    """the sizes that the tests on the GPU have for each kind of tiles are cut into them"""
+    assert plan(lib, rows, experts, k, n, act) == cut
+    wide = (k + 15) // 16 * 16
+    cols = -(-n // 8) * 8 if act == "swiglu" and n % 8 else -(-n // 4) * 4            # either half of a swiglu's sums starts at a multiple of four
+    size = lib.zbal_moe_expert_linear_int8_workspace_size(rows, k, n, experts, capi.ACTIVATIONS[act])
+    assert size == (cut[2] and (rows + experts * n) * wide) + (cut[1] > 1 and cut[1] * rows * cols * 4)
+
+
+def test_linear_plans_reach_every_kind(lib):
+    kinds = {name for (name, _, _), *_ in CASES}
+    assert len(kinds) == 14
+    for name in kinds - {"short"}:
+        of = [(c, size) for c, *size in CASES if c[0] == name]
+        assert {size[1] > 1 for _, size in of} == {True, False} and {size[4] for _, size in of} == {"none", "swiglu"}
+        aligned = not name.endswith("any")
+        assert {c[2] for c, _ in of} == ({0, 1} if aligned else {0})
+        parts = {c[1] for c, _ in of}
+        assert 1 in parts and (parts == {1}) == (name in ("256x256", "rows") or name.endswith("flat"))
+    assert plan(lib, 0, 2, 64, 64, "none") is None and plan(lib, 4, 2, 65537, 64, "none") is None
+    assert lib.zbalhip_expert_linear_int8_plan(None, None, None) is None
+    assert lib.zbalhip_expert_linear_int8_plan(ctypes.byref(linear()), None, None)
 
 
 def test_outer_calls_check_their_arguments_first(lib):

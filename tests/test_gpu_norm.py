@@ -169,6 +169,14 @@ def test_gradients(buf, tokens, hidden, dtype):
     backward_case(buf, tokens, hidden, dtype, None, True, torch.float32)
 
 
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,hidden", [(700, 7168), (1100, 4104), (3000, 4104), (600, 8200), (1500, 12000), (600, 16392), (900, 24001), (300, 40000), (600, 33000)])
+def test_gradients_of_several_rows_to_a_workgroup_and_pieces_to_a_lane(buf, tokens, hidden, dtype):
+    """two, four and eight pieces, the latter in 512 lanes and in 1024, over rows that a workgroup takes one after the other"""
+    backward_case(buf, tokens, hidden, dtype, "same", True, None)
+    backward_case(buf, tokens, hidden, dtype, "fp32", False, torch.float32)
+
+
 def test_what_is_not_asked_for(buf):
     g, x, w = make(50, 640, torch.bfloat16, 1)
     grad = torch.randn_like(x)

@@ -89,6 +89,57 @@ def test_norm(buf, tokens, hidden, dtype):
             check_int8(q, scales, want, ERR)
 
 
+# from 2049 rows on a row has half as many lanes and twice as many pieces
+MANY_ROWS = [(2049, 1531), (3000, 2100), (2500, 4104), (4096, 7168), (2048, 7168), (2200, 8200), (2049, 16392), (2100, 33000)]
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("tokens,hidden", MANY_ROWS)
+def test_norm_of_many_rows(buf, tokens, hidden, dtype):
+    for weight, residual, int8, norm in (("same", True, True, True), ("fp32", False, True, False)):
+        g, x, w = make(tokens, hidden, dtype, tokens + hidden, weight)
+        r = torch.randn((tokens, hidden), device="cuda", generator=g).to(dtype) if residual else None
+        y, q, scales, total = buf.rms_norm(x, w, r, EPS, int8, norm)
+        h = x.double() + (r.double() if residual else 0)
+        if residual:
+            close(total, h, U * h.abs(), dtype)
+        want = norm64(h, w)
+        if norm:
+            close(y, want, ERR * want.abs(), dtype)
+        check_int8(q, scales, want, ERR)
+
+
+def test_more_rounds_of_rows_than_one(buf):
+    """A launch has 2^20 workgroups at most: rows past them, and those that the same workgroups had before, are what they are in a call of their own. Rows of
+    three waves, one to a workgroup, and of one wave, four to a workgroup."""
+    for rows, width in (((1 << 20) + 40000, 1032), ((1 << 22) + 90000, 72)):
+        more = rows % (1 << 20)
+        x = torch.empty((rows, width), device="cuda", dtype=torch.bfloat16).normal_()
+        x *= torch.exp2((torch.arange(rows, device="cuda") * 7 % 13 - 6).to(torch.bfloat16))[:, None]      # neighbours of other sizes
+        w = torch.randn((width,), device="cuda").to(torch.bfloat16)
+        parts = (slice(0, more), slice(rows - 2 * more, rows))
+        got = buf.rms_norm(x, w, None, EPS, True, True)
+        for part in parts:
+            want = buf.rms_norm(x[part].clone(), w, None, EPS, True, True)
+            assert all(torch.equal(a[part], b) for a, b in zip(got[:3], want[:3]))
+        del got, want
+        for act in ("none", "silu"):
+            got = buf.quantize_rows(x, activation=act)
+            for part in parts:
+                assert all(torch.equal(a[part], b) for a, b in zip(got, buf.quantize_rows(x[part].clone(), activation=act)))
+            del got
+        count = rows - more // 2
+        got = buf.quantize_rows(x, torch.tensor([count], device="cuda"))
+        part = slice(rows - 2 * more, count)
+        assert all(torch.equal(a[part], b) for a, b in zip(got, buf.quantize_rows(x[part].clone())))
+        del x, got
+    rows = (1 << 20) + 20000
+    x = torch.empty((rows, 2064), device="cuda", dtype=torch.bfloat16).normal_()
+    got = buf.quantize_rows(x, activation="swiglu")
+    for part in (slice(0, 20000), slice(rows - 40000, rows)):
+        assert all(torch.equal(a[part], b) for a, b in zip(got, buf.quantize_rows(x[part].clone(), activation="swiglu")))
+
+
 def test_eps_and_the_norms_own_types(buf):
     for eps in (1e-12, 1e-5, 1.0, 1e6):
         g, x, w = make(5, 640, torch.float32, 3)
@@ -252,6 +303,13 @@ def test_quantize(buf, rows, width, act):
         quantize_case(buf, rows, width, dtype, act)
 
 
+@pytest.mark.parametrize("rows,width,act", [(2049, 1030, "none"), (3000, 2100, "silu"), (2100, 6130, "swiglu"), (4096, 4096, "relu"), (2500, 16392, "gelu"), (2048, 16384, "swiglu"),
+                                            (2049, 33000, "none"), (2100, 65536, "swiglu"), (2500, 8200, "gelu_tanh")])
+def test_quantize_many_rows(buf, rows, width, act):
+    for dtype in TYPES:
+        quantize_case(buf, rows, width, dtype, act)
+
+
 @pytest.mark.parametrize("counts", [[0, 0, 0], [5, 0, 30], [40, 20, 0], [-3, 10, 1 << 30], [1], [0] * 1000 + [7] * 24])
 def test_quantized_rows_of_nobody_stay(buf, counts):
     for act, width in (("swiglu", 528), ("silu", 130)):
@@ -345,6 +403,23 @@ def test_the_sum_in_place(buf):
         code = capi.load().zbal_moe_rms_norm(t(xi), t(w), t(ri), EPS, t(y), t(on), None, None, buf.runtime.comm, capi.stream_ptr(), 0)
         assert code == 0
         assert torch.equal(y, want[0]) and torch.equal(on, want[3])
+
+
+@pytest.mark.parametrize("tokens,hidden", [(3, 600), (700, 4104), (2100, 520)])
+def test_the_gradient_in_place(buf, tokens, hidden):
+    """through the kernel's entry: the rows' gradient in the memory of the one that comes in, or of the sum's"""
+    g, x, w = make(tokens, hidden, torch.bfloat16, 9)
+    grad, total = torch.randn_like(x), torch.randn_like(x)
+    gx, gw = buf.rms_norm_backward(grad, x, w, total, EPS, torch.float32)
+    lib, stream = capi.load(), torch.cuda.current_stream().cuda_stream
+    d = capi.RmsNorm(x.data_ptr(), None, w.data_ptr(), capi.DT_BF16, 0, tokens, hidden, EPS)
+    size = lib.zbalhip_rms_norm_backward_workspace(ctypes.byref(d))
+    ws = torch.empty((max(size, 16),), dtype=torch.uint8, device="cuda")
+    for on_grad in (True, False):
+        a, b, got = grad.clone(), total.clone(), torch.empty_like(gw)
+        on = a if on_grad else b
+        assert lib.zbalhip_rms_norm_backward(ctypes.byref(d), a.data_ptr(), b.data_ptr(), on.data_ptr(), got.data_ptr(), 1, ws.data_ptr(), size, stream) == 0
+        assert torch.equal(on, gx) and torch.equal(got, gw)
 
 
 def test_refusals(buf):

@@ -663,7 +663,7 @@ void in_pairs(XgemmParams *p, int k)
  * few workgroups on the card, and with as many as run side by side), joined with the time that reading the weights takes as the root of the sum of their squares.
  * The figures (us, bytes a us) are fitted to every kind's time, whole and in parts, for 136 products of 1 to 32768 rows, 1 to 64 experts, k and n 64 to 7168, and 34 of
  * unaligned rows: the kind that it picks takes 1.03 times the best one's on average, 1.31 at most (one row of 1001 x 4001: copied 10.1 us, as it lies 7.7). For 27 more, of 1
- * to 1021 rows over 8 to 128 experts, that no figure was fitted to, 1.02 and 1.17. Half precision's rule, for the tiles that both have, had 1.11 and 3.65 here: 512 x 512 x
+ * to 1021 rows over 8 to 128 experts, that no figure was fitted to, 1.03 and 1.17. Half precision's rule, for the tiles that both have, had 1.11 and 3.65 here: 512 x 512 x
  * 512 16.8 by sixteen columns at a time where 16 x 64 takes 4.6; 16384 rows over 8 of 2048 x 1024 128 x 128 71, wide 56. FLAT: rings of two stages and three to eight
  * workgroups to a CU instead of two, which gain where tiles are many and short: 423 rows over 64 experts, k 128 and n 4480, 25 -> 15 us, 425 over 64, k 384 and n 6912, silu
  * 63 -> 43; and lose where they are few and long: 4 rows over 8, k 7168 and n 2048, 16 -> 42.
@@ -717,7 +717,7 @@ Plan plan_int8_cut(const XgemmParams &p, bool aligned, double *us)
 
 /*
  * Rows that are not aligned: multiplied as they lie, or copied to the workspace first, whichever the model expects to be done sooner. A copy is a launch, and writes
- * both operands at 2.4 TB/s: 4093 x 4099 x 4093 194 us as it lies, 83 copied; 16 rows over 32 experts of 4001 x 1531 32 and 114.
+ * both operands at 2.4 TB/s: 4093 x 4099 x 4093 194 us as it lies, 80 copied; 16 rows over 32 experts of 4001 x 1531 32 and 114.
  */
 struct Int8Plan {
     XgemmParams p;

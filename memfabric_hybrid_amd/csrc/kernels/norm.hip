@@ -180,8 +180,8 @@ struct NormParams {
 __device__ __forceinline__ float n_rsqrt(float mean_square, float eps) { return 1.0f / __builtin_sqrtf(mean_square + eps); }
 
 /*
- * Eight elements of the weight, ones without one: of the rows' type (W is DT) or of 32 bits. A lane has the same columns of every row, so they are loaded once, in front of the
- * first row, and are there when its sum is.
+ * Eight elements of the weight, ones without one: of the rows' type (W is DT) or of 32 bits. A lane has the same columns of every row, so they are asked for in front of the
+ * first row, and are there when its sum is: what the norm gains by that, whose workgroups have one round of rows up to 2^20 of them. The gradient's have many and load them once.
  */
 template <int W> __device__ __forceinline__ Piece<W> n_weight(const NormParams &p, int at)
 {
@@ -379,8 +379,9 @@ rms_norm_join_kernel(const float *__restrict__ partial, int count, int ldp, int 
 /* ---- activations in int8 ------------------------------------------------------------------------------------------- */
 
 /*
- * silu in a dozen cycles: an exponential of two and a reciprocal, each a step off (2^-23). The kernel is a stream: with the division of the products' epilogue the vector units
- * took longer than the memory (32768 x 4096, swiglu: 78 us, now 57).
+ * silu in a dozen cycles: an exponential of two and a reciprocal, each a step off (2^-23), and the exponential's argument rounded: about |z| 2^-24 besides, as in the products'
+ * epilogue. Zero from about -88 down, where the exponential ends (silu(-88) is -5.3e-37). For swiglu, whose kernel is a stream: with the division of the products' epilogue the vector
+ * units took longer than the memory (32768 x 4096: 78 us, now 57). silu alone has that division, chosen element by element (97 us, 65 of bytes).
  */
 __device__ __forceinline__ float n_silu(float z) { return z * __builtin_amdgcn_rcpf(1.0f + __builtin_amdgcn_exp2f(z * -1.44269504088896341f)); }
 
@@ -453,7 +454,12 @@ inline Shape shape_of(int64_t width, int most)
     return s;
 }
 
-/* few rows have a lane to a piece as far as that goes; many of them more rows side by side on a CU (8192 x 4096, no activation: 512 lanes 19.3 us, 256 16.5) */
+/*
+ * Few rows have a lane to a piece as far as that goes; many of them more rows side by side on a CU. us with 512 / 256 lanes, bf16, over inputs that change, norm alone and int8 rows
+ * without an activation: 4096 columns, 512 rows 4.1 / 4.0 and 3.8 / 3.8, 1024 5.5 / 5.0 and 4.7 / 4.6, 2048 8.0 / 7.3 and 7.2 / 6.2, 2560 9.3 / 8.4 and 8.5 / 7.7, 8192 29.6 / 22.9 and
+ * 22.5 / 18.2; 7168, 256 rows 3.6 / 4.0 and 3.9 / 3.8, 2560 16.0 / 15.3 and 12.1 / 11.8, 8192 43.0 / 38.6 and 29.8 / 29.1; 8192, 2560 16.2 / 16.3 and 12.8 / 12.5, 8192 44.2 / 42.2 and
+ * 31.8 / 31.8. With residual and int8 besides (4096 x 7168 42.4 / 43.1) and from 14336 columns on (8192 rows 84.9 / 94.2 and 62.1 / 64.4) half the lanes are a few percent slower.
+ */
 inline Shape forward_shape(int64_t width, int64_t rows) { return shape_of(width, rows > 2048 ? 256 : N_LANES); }
 
 /* f(pieces, most lanes) as integral constants */

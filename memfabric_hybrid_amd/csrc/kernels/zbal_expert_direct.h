@@ -1,5 +1,6 @@
 /*
- * The experts' products where every row and column starts at a 16-byte boundary: operands go from memory to the LDS without passing
+ * The experts' products where every row of the operands starts at a 16-byte boundary, in half precision every row of outputs and every half of swiglu's columns, too (int8's
+ * outputs, scales, bias and residual may have any width): operands go from memory to the LDS without passing
  * through registers (buffer loads with the LDS as their target), in a ring of stages, all but one of which are on their way while one is
  * multiplied. For tiles so small, or so few, that the time of a step is that of a transfer.
  *
@@ -246,7 +247,7 @@ expert_gemm_kernel(XgemmParams p)
     constexpr int PASS = MT % 2 == 0 && WM * 32 * (TN + 4) * 4 <= STAGES * STAGE ? 2 : 1, ROWS = WM * PASS * 16, LD = TN + 4, QUADS = TN / 4;
     /*
      * What int8's epilogue reads, asked for in front of the first transfers: behind the last products it would be waited for, twice (1021 x 1001 x 1531 with gelu, bias and
-     * residual, its copies included, 24.6 us, now 17.6).
+     * residual, its copies included, 24.6 us behind them, 17.6 in front; 15.8 with what the epilogue below gained since).
      */
     constexpr int TURNS = ROWS * QUADS / (WAVES * 64), ROW_STEP = WAVES * 64 / QUADS;
     static_assert(!x_is_i8<DT> || (TURNS % 2 == 0 && TURNS * WAVES * 64 == ROWS * QUADS && ROW_STEP * QUADS == WAVES * 64), "a lane has the same columns in every turn");
@@ -321,7 +322,7 @@ expert_gemm_kernel(XgemmParams p)
     }
     asm volatile("s_waitcnt vmcnt(0)" ::: "memory");
 
-    /* ---- epilogue: a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile; cols is a multiple of 8 ---- */
+    /* ---- epilogue: a lane has columns 4 (l / 16) .. + 3 of row l % 16 of every sub-tile; in half precision cols is a multiple of 8 ---- */
     const int q4 = (lane >> 4) * 4;
     if constexpr (REDUCE) {
         auto put = [&](int j, int end, float v) __attribute__((always_inline)) {
